@@ -263,6 +263,59 @@ int tcu_gemm_f16_f32(const void *d_A, const void *d_B, const void *d_C, void *d_
 int tcu_gemv_f16_f16(const void *d_A, const void *d_x, void *d_y, size_t M, size_t K, float alpha, float beta, int variant, void *stream);
 int tcu_gemm_f16_f16(const void *d_A, const void *d_B, const void *d_C, void *d_D, size_t M, size_t N, size_t K, float alpha, float beta, int variant, void *stream);
 
+/* ---- recurrent blocks of language models ------------------------------------------------------
+ *
+ * Operators a gated recurrent block is made of, next to the reductions, scans and products above: the scan with a gate per
+ * element, the norm fused with what stands around it, the product with its epilogue; each with its gradient and with a
+ * form for the few rows of one decoding step.  No counterpart in the reference.  Matrices are row-major with a stride in
+ * elements from row to row (so a slice of a wider matrix can be passed as it is); rows are tokens.  Whole 16-byte accesses
+ * need base pointers aligned to 16 bytes and strides and widths that are multiples of 16 bytes; anything else takes the same
+ * kernels with element-wise accesses.  All sums, states and statistics are fp32; a result is rounded once, to its type.
+ * Calls run on the device of `stream` (NULL: the current device's default stream).  Workspaces follow the two-phase
+ * protocol of the full-array entry points (256-byte aligned, never smaller than 256 bytes, nothing is kept in them from
+ * one call to the next; calls that may overlap in time, captured graphs among them, need one each). */
+
+typedef enum { TCU_F16 = 0, TCU_BF16 = 1, TCU_F32 = 2 } tcu_dtype;
+
+/* Gated scan: h[t] = a[t] h[t-1] + b[t] down the rows of each sequence, every channel by itself, h[-1] = the sequence's
+ * row of d_h0 (0 if d_h0 is NULL). */
+typedef enum {
+  TCU_GATE_DECAY = 0,  /* a = g,          b = x */
+  TCU_GATE_LOG = 1,    /* a = exp(g),     b = x */
+  TCU_GATE_SIGMOID = 2 /* a = sigmoid(g), b = (1 - a) x */
+} tcu_gate;
+
+typedef struct {
+  int dtype;              /* tcu_dtype of all matrices */
+  int gate;               /* tcu_gate */
+  size_t channels;        /* columns */
+  size_t num_rows;        /* rows of every matrix, below 2^31 - 4096 */
+  size_t num_sequences;
+  size_t sequence_length; /* d_offsets NULL: num_rows = num_sequences * sequence_length */
+  const void *d_offsets;  /* or num_sequences + 1 offsets in device memory that do not decrease: sequence j has the rows
+                             offsets[j] ... offsets[j+1] - 1 (none if they are equal) */
+  int offset_bits;        /* 32 or 64 */
+  int zero_outside;       /* rows outside all sequences are not read; in the outputs they are left as they are (0) or set
+                             to zero (anything else) */
+} tcu_gated_scan_shape;
+
+/* d_h = the states after every row, d_h_last (num_sequences x channels fp32, may be NULL) = the state behind each sequence
+ * (behind an empty one: its d_h0, or 0).  d_h0: num_sequences x channels fp32.  d_h may be d_x or d_g (same stride).
+ * Bit-reproducible.  A wait of one tile for another that expires ("lookback_poll_limit") leaves NaN from there to the end
+ * of the sequence, and word 1 of the workspace, where offsets are given or the rows take several tiles, counts it. */
+int tcu_gated_scan(const tcu_gated_scan_shape *shape, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, void *d_h, size_t h_stride, const float *d_h0, float *d_h_last, void *d_workspace, size_t *workspace_bytes, void *stream);
+
+/* The gradient: from d_dh (with respect to d_h) and d_dh_last (with respect to d_h_last, may be NULL), d_dx, d_dg and, if
+ * not NULL, d_dh0 (num_sequences x channels fp32).  d_h: the states the forward call returned; d_x is read for
+ * TCU_GATE_SIGMOID only.  d_dx and d_dg may take the place of d_dh, d_x or d_g, not of d_h.  Bit-reproducible; waits as above. */
+int tcu_gated_scan_backward(const tcu_gated_scan_shape *shape, const void *d_dh, size_t dh_stride, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, const void *d_h, size_t h_stride, const float *d_h0, const float *d_dh_last, void *d_dx, size_t dx_stride, void *d_dg, size_t dg_stride, float *d_dh0, void *d_workspace, size_t *workspace_bytes, void *stream);
+
+/* One token for each of num_rows running sequences: row i advances the state in slot d_slots[i] of d_state (num_slots x
+ * channels fp32; d_slots NULL: slot i), writes it to the same slot of d_new_state (which may be d_state; slots that no row
+ * names are not written) and, rounded, to row i of d_h.  Rows whose slot is negative or not below num_slots are padding:
+ * not read, and in d_h left as they are (zero_padding 0) or set to zero.  Rows that name the same slot advance it one after the other, in row order. */
+int tcu_gated_scan_step(int dtype, int gate, size_t channels, size_t num_rows, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, void *d_h, size_t h_stride, const float *d_state, float *d_new_state, size_t num_slots, const int32_t *d_slots, int zero_padding, void *stream);
+
 /* ---- fills, conversions, inputs ---------------------------------------------------------------- */
 
 /* d[i] = (half) value.  Replaces cuda_memory_set / setFP16 (reference

@@ -13,6 +13,7 @@ from .binding import (  # noqa: F401
     FullStrategy,
     FULL_MFMA,
     Dist,
+    Gate,
     add_partial_sums,
     build,
     device_info,
@@ -20,6 +21,9 @@ from .binding import (  # noqa: F401
     convert_f32_to_f16,
     full_reduce,
     full_scan,
+    gated_scan,
+    gated_scan_backward,
+    gated_scan_step,
     gemm,
     gemv,
     gemv_col_major,

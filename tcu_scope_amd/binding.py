@@ -13,6 +13,7 @@ EXPORTS = [
     "tcu_abi_version", "tcu_last_error", "tcu_init", "tcu_device_info", "tcu_set_option",
     "tcu_seg_reduce_f16", "tcu_seg_reduce_offsets_f16", "tcu_seg_scan_f16", "tcu_seg_scan_f16_noalloc", "tcu_seg_scan_offsets_f16", "tcu_seg_scan_by_key_f16", "tcu_seg_reduce_by_key_f16", "tcu_add_partial_sums_f16",
     "tcu_full_reduce_f16", "tcu_full_scan_f16", "tcu_gemv_f16_f32", "tcu_gemm_f16_f32", "tcu_gemv_f16_f16", "tcu_gemm_f16_f16", "tcu_gemv_col_major_f16_f32", "tcu_gemv_col_major_f16_f16",
+    "tcu_gated_scan", "tcu_gated_scan_backward", "tcu_gated_scan_step",
     "tcu_fill_f16", "tcu_convert_f32_to_f16", "tcu_generate_f16", "tcu_stream_probe", "tcu_time_next_launch", "tcu_lane_probe", "tcu_temporary_allocations",
 ]
 
@@ -49,6 +50,21 @@ class Dist(enum.IntEnum):
     SMALLINT = 3
 
 
+class Gate(enum.IntEnum):
+    """How a gated scan reads its gate g: a = g, a = exp(g), or a = sigmoid(g) with the input weighted by 1 - a."""
+
+    DECAY = 0
+    LOG = 1
+    SIGMOID = 2
+
+
+class GatedScanShape(ctypes.Structure):
+    """tcu_gated_scan_shape."""
+
+    _fields_ = [("dtype", ctypes.c_int), ("gate", ctypes.c_int), ("channels", ctypes.c_size_t), ("num_rows", ctypes.c_size_t), ("num_sequences", ctypes.c_size_t), ("sequence_length", ctypes.c_size_t),
+                ("d_offsets", ctypes.c_void_p), ("offset_bits", ctypes.c_int), ("zero_outside", ctypes.c_int)]
+
+
 class TcuError(RuntimeError):
     """A non-zero tcu_status; .status is 1 invalid argument, 2 unsupported, 3 runtime, 4 workspace."""
 
@@ -64,7 +80,7 @@ def library_path():
 def build():
     """Compile the HIP sources for gfx950 into libtcu_scope_amd.so (needs hipcc, no GPU)."""
     subprocess.check_call(["make", "-C", _CSRC, "clean"], stdout=subprocess.DEVNULL)
-    subprocess.check_call(["make", "-C", _CSRC], stdout=subprocess.DEVNULL)
+    subprocess.check_call(["make", "-j4", "-C", _CSRC], stdout=subprocess.DEVNULL)
     return _LIB
 
 
@@ -109,6 +125,10 @@ def lib():
         L.tcu_time_next_launch.argtypes = [vp, vp]
         L.tcu_temporary_allocations.argtypes = []
         L.tcu_temporary_allocations.restype = c.c_ulong
+        shape, psz = c.POINTER(GatedScanShape), c.POINTER(sz)
+        L.tcu_gated_scan.argtypes = [shape, vp, sz, vp, sz, vp, sz, vp, vp, vp, psz, vp]
+        L.tcu_gated_scan_backward.argtypes = [shape, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, sz, vp, sz, vp, vp, psz, vp]
+        L.tcu_gated_scan_step.argtypes = [ci, ci, sz, sz, vp, sz, vp, sz, vp, sz, vp, vp, sz, vp, ci, vp]
         for name in EXPORTS:
             if name not in ("tcu_last_error", "tcu_temporary_allocations"):
                 getattr(L, name).restype = ci
@@ -371,6 +391,197 @@ def gemm(A, Bt, alpha=1.0, beta=0.0, C=None, out=None, variant=Variant.AUTO, str
     entry = _out_entry(out, "out", lib().tcu_gemm_f16_f32, lib().tcu_gemm_f16_f16)
     _check(entry(_ptr(A), _ptr(Bt), _ptr(C), _ptr(out), M, N, K, alpha, beta, int(variant), _stream(stream)))
     return out
+
+
+# ---- recurrent blocks of language models ------------------------------------------------------------------------
+
+
+def _dtype_code(t, name):
+    torch = _torch()
+    code = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be a float16, bfloat16 or float32 tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return code
+
+
+def _enum(kind, value):
+    """A member of the enumeration `kind` from a member, a number or a name in any case."""
+    if isinstance(value, str):
+        try:
+            return int(kind[value.upper()])
+        except KeyError:
+            raise ValueError(f"{value!r} is none of {', '.join(m.name.lower() for m in kind)}") from None
+    return int(kind(value))
+
+
+def _matrix(t, name, like=None):
+    """(pointer, rows, row stride) of a tensor whose leading dimensions can be read as one: rows of contiguous elements at an even distance."""
+    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape != like.shape):
+        raise ValueError(f"{name} must have the shape, type and device of the other operands ({tuple(like.shape)}, {like.dtype}, {like.device}); got {tuple(t.shape)}, {t.dtype}, {t.device}")
+    sizes, strides = t.shape, t.stride()
+    if len(sizes) < 2:
+        raise ValueError(f"{name} must have at least two dimensions")
+    width = sizes[-1]
+    if width > 1 and strides[-1] != 1:
+        raise ValueError(f"{name} must be contiguous along its last dimension")
+    rows, stride, ok = 1, None, True
+    for n, s in zip(reversed(sizes[:-1]), reversed(strides[:-1])):
+        if n != 1:
+            if stride is None:
+                stride = s
+            elif s != stride * rows:
+                ok = False
+            rows *= n
+    if rows > 1 and not ok:
+        raise ValueError(f"the rows of {name} are not evenly spaced: pass a contiguous tensor")
+    return t.data_ptr(), rows, width if stride is None or rows <= 1 else stride
+
+
+def _vector_f32(t, name, shape, device):
+    torch = _torch()
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of shape {tuple(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _launch_on(device, stream, body):
+    """body(raw stream) with `device`, and the stream asked for, current: what the body allocates belongs to that stream."""
+    torch = _torch()
+    if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+        with torch.cuda.stream(stream):
+            return body(stream.cuda_stream)
+    if torch.cuda.current_device() == device.index:
+        return body(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return body(torch.cuda.current_stream().cuda_stream)
+
+
+def _workspace_of(fn, args, workspace, device):
+    """(pointer, size) of a workspace for the call: the caller's, or a new one of the size the call asks for."""
+    if workspace is None:
+        need = ctypes.c_size_t(0)
+        _check(fn(*args, None, ctypes.byref(need), None))
+        workspace = _torch().empty(need.value, dtype=_torch().uint8, device=device)
+    elif workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    return workspace, ctypes.c_size_t(workspace.numel() * workspace.element_size())
+
+
+def _scan_shape(x, gate, offsets, h0, name="x"):
+    torch = _torch()
+    dtype = _dtype_code(x, name)
+    s = GatedScanShape(dtype=dtype, gate=_enum(Gate, gate), channels=x.shape[-1])
+    if offsets is not None:
+        if x.dim() != 2:
+            raise ValueError(f"with offsets {name} is a matrix of all rows")
+        if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != x.device or offsets.dim() != 1 or offsets.numel() < 1 or not offsets.is_contiguous():
+            raise ValueError("offsets must be a contiguous int32 or int64 vector on the same device, one entry more than there are sequences")
+        s.num_rows, s.num_sequences = x.shape[0], offsets.numel() - 1
+        s.d_offsets, s.offset_bits = offsets.data_ptr(), 32 if offsets.dtype == torch.int32 else 64
+    else:
+        if x.dim() not in (2, 3):
+            raise ValueError(f"{name} must be (sequences, tokens, channels), or (tokens, channels) of one sequence")
+        s.num_sequences = x.shape[0] if x.dim() == 3 else 1
+        s.sequence_length = x.shape[-2]
+        s.num_rows = s.num_sequences * s.sequence_length
+    return s
+
+
+def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=None, workspace=None, stream=None):
+    """h[t] = a[t] h[t-1] + b[t] along each sequence (tcu_gated_scan): returns (h, h_last).
+
+    x, g: (sequences, tokens, channels) or (tokens, channels), float16, bfloat16 or float32, or with `offsets` (int32 or
+    int64, one more than there are sequences, not decreasing) the rows of all sequences as one matrix.  gate: a Gate, or its
+    name: "decay" (a = g, b = x), "log" (a = exp(g), b = x), "sigmoid" (a = sigmoid(g), b = (1 - a) x).  h0, h_last:
+    (sequences, channels) float32, the states in front of and behind the sequences.  Rows outside all sequences
+    are left as they are in `out`, and zero in a result this call allocates.  out may be x or g."""
+    torch = _torch()
+    s = _scan_shape(x, gate, offsets, h0)
+    states = (s.num_sequences, s.channels)
+    px, _, sx = _matrix(x, "x")
+    pg, _, sg = _matrix(g, "g", x)
+    p0 = _vector_f32(h0, "h0", states, x.device)
+    s.zero_outside = out is None
+
+    def body(raw):
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+        last = torch.empty(states, dtype=torch.float32, device=x.device) if h_last is None else h_last
+        ph, _, sh = _matrix(h, "out", x)
+        args = (ctypes.byref(s), px, sx, pg, sg, ph, sh, p0, _vector_f32(last, "h_last", states, x.device))
+        ws, have = _workspace_of(lib().tcu_gated_scan, args, workspace, x.device)
+        _check(lib().tcu_gated_scan(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        return h, last
+
+    return _launch_on(x.device, stream, body)
+
+
+def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, offsets=None, dx=None, dg=None, workspace=None, stream=None):
+    """The gradient of gated_scan (tcu_gated_scan_backward): returns (dx, dg, dh0).
+
+    dh, dh_last: gradients with respect to h and h_last (dh_last may be None); h: what gated_scan returned; x is read for
+    the sigmoid gate only and may be None for the others.  dh0 is (sequences, channels) float32.  dx and dg may be given
+    (both or neither), and be dh, x or g; rows outside all sequences are then left as they are, and otherwise zero."""
+    torch = _torch()
+    s = _scan_shape(g, gate, offsets, h0, "g")
+    states = (s.num_sequences, s.channels)
+    if x is None and s.gate == Gate.SIGMOID:
+        raise ValueError("the sigmoid gate's gradient needs x")
+    px, _, sx = _matrix(x, "x", g) if x is not None else (None, 0, 0)
+    pg, _, sg = _matrix(g, "g")
+    pd, _, sd = _matrix(dh, "dh", g)
+    ph, _, sh = _matrix(h, "h", g)
+    p0, pl = _vector_f32(h0, "h0", states, g.device), _vector_f32(dh_last, "dh_last", states, g.device)
+    if (dx is None) != (dg is None):
+        raise ValueError("dx and dg are given both or neither")
+    s.zero_outside = dx is None
+
+    def body(raw):
+        out_x, out_g = (dx, dg) if dx is not None else (torch.empty(g.shape, dtype=g.dtype, device=g.device) for _ in range(2))
+        dh0 = torch.empty(states, dtype=torch.float32, device=g.device)
+        pox, _, sox = _matrix(out_x, "dx", g)
+        pog, _, sog = _matrix(out_g, "dg", g)
+        args = (ctypes.byref(s), pd, sd, px, sx, pg, sg, ph, sh, p0, pl, pox, sox, pog, sog, dh0.data_ptr())
+        ws, have = _workspace_of(lib().tcu_gated_scan_backward, args, workspace, g.device)
+        _check(lib().tcu_gated_scan_backward(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        return out_x, out_g, dh0
+
+    return _launch_on(g.device, stream, body)
+
+
+def gated_scan_step(x, g, state, gate=Gate.SIGMOID, slots=None, new_state=None, out=None, stream=None):
+    """One token for each running sequence (tcu_gated_scan_step): returns h (rows, channels).
+
+    x, g: (rows, channels); state: (slots, channels) float32; slots: int32, the slot of each row (None: row i uses slot i; a
+    negative or too large one marks padding, whose row of `out` is left as it is, or zero in a result this call allocates).  The new states go to `new_state`, by
+    default `state` itself; slots that no row names are not written."""
+    torch = _torch()
+    dtype = _dtype_code(x, "x")
+    if x.dim() != 2:
+        raise ValueError("x must be (rows, channels)")
+    rows, channels = x.shape
+    px, _, sx = _matrix(x, "x")
+    pg, _, sg = _matrix(g, "g", x)
+    if state.dim() != 2:
+        raise ValueError("state must be (slots, channels)")
+    shape = (state.shape[0], channels)
+    ps = _vector_f32(state, "state", shape, x.device)
+    pn = ps if new_state is None else _vector_f32(new_state, "new_state", shape, x.device)
+    if slots is not None and (slots.dtype != torch.int32 or slots.device != x.device or tuple(slots.shape) != (rows,) or not slots.is_contiguous()):
+        raise ValueError("slots must be a contiguous int32 vector with one entry per row, on the same device")
+
+    def body(raw):
+        h = torch.empty((rows, channels), dtype=x.dtype, device=x.device) if out is None else out
+        ph, _, sh = _matrix(h, "out", x)
+        _check(lib().tcu_gated_scan_step(dtype, _enum(Gate, gate), channels, rows, px, sx, pg, sg, ph, sh, ps, pn, shape[0], slots.data_ptr() if slots is not None else None, out is None, raw))
+        return h
+
+    return _launch_on(x.device, stream, body)
 
 
 def fill(t, value, stream=None):

@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "dispatch.hpp"
+#include "host_support.hpp"
 
 // Partition descriptors of tcu_seg_scan_f16_noalloc: a ticket counter (64 words) and one 64-bit
 // descriptor for each partition of 65536 halves: 256 bytes apart for up to 4096 partitions, closer
@@ -84,6 +85,13 @@ int after_launch(const char *what, unsigned long launches_before, int rc) {
 }
 
 }  // namespace
+
+namespace tcu {
+int report_failure(int code, const std::string &message) { return fail(code, message); }
+unsigned shared_poll_limit() { return options().lookback_poll_limit; }
+unsigned shared_mute_partition() { return options().test_mute_partition; }
+int launch_outcome(const char *what, unsigned long launches_before, int rc) { return after_launch(what, launches_before, rc); }
+}  // namespace tcu
 
 extern "C" {
 

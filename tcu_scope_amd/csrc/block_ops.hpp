@@ -1,0 +1,29 @@
+// What the recurrent-block operators (gated scan, fused norm, fused matrix product) use beyond wave_ops.hpp: element
+// types behind a 16-byte chunk, the transcendental instructions, cross-lane reads by lane number.
+//
+// A chunk is 16 bytes of one row: 8 elements of 16 bits or 4 of 32.  Everything is computed in fp32; the one rounding to
+// 16 bits is the conversion of a result to the type its tensor has (to nearest even).
+#ifndef TCU_BLOCK_OPS_HPP
+#define TCU_BLOCK_OPS_HPP
+
+#include "wave_ops.hpp"
+
+namespace tcu {
+
+// 2^x, 1/x, 1/sqrt(x): the hardware's instructions, within 1 ulp (results below 2^-126 are 0)
+TCU_DEVICE float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+TCU_DEVICE float hw_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+TCU_DEVICE float hw_rsqrt(float x) { return __builtin_amdgcn_rsqf(x); }
+
+// value of `x` in lane `l` (may differ from lane to lane)
+TCU_DEVICE float read_lane_of(float x, int l) { return __int_as_float(__builtin_amdgcn_ds_bpermute(l << 2, __float_as_int(x))); }
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+TCU_DEVICE unsigned pack_bf16x2(float lo, float hi) {
+  bf16x2_t v = {(__bf16)lo, (__bf16)hi};
+  return __builtin_bit_cast(unsigned, v);
+}
+TCU_DEVICE uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
+
+}  // namespace tcu
+#endif  // TCU_BLOCK_OPS_HPP

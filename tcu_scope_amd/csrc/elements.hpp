@@ -1,0 +1,169 @@
+// Element types of the recurrent-block operators: 16-byte chunks of fp16, bf16 or fp32 to and from fp32 values, with
+// whole-chunk accesses where rows are aligned and element-by-element ones where they are not; activations.
+#pragma once
+
+#include "block_ops.hpp"
+
+namespace tcu {
+
+constexpr int kF16 = 0, kBF16 = 1, kF32 = 2;  // tcu_dtype
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<kF16> {
+  using word_t = uint16_t;
+  static constexpr int V = 8;  // elements per 16-byte chunk
+  TCU_DEVICE static float load(uint16_t w) { return (float)__builtin_bit_cast(half_t, w); }
+  TCU_DEVICE static uint16_t round(float v) { return f16_bits(v); }
+  TCU_DEVICE static unsigned pack(float lo, float hi) { return pack_f16x2(lo, hi); }
+};
+template <>
+struct Elem<kBF16> {
+  using word_t = uint16_t;
+  static constexpr int V = 8;
+  TCU_DEVICE static float load(uint16_t w) { return __uint_as_float((unsigned)w << 16); }
+  TCU_DEVICE static uint16_t round(float v) { return bf16_bits(v); }
+  TCU_DEVICE static unsigned pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+};
+template <>
+struct Elem<kF32> {
+  using word_t = uint32_t;
+  static constexpr int V = 4;
+  TCU_DEVICE static float load(uint32_t w) { return __uint_as_float(w); }
+  TCU_DEVICE static uint32_t round(float v) { return __float_as_uint(v); }
+};
+
+// chunk -> V fp32 values
+template <int DT>
+TCU_DEVICE void unpack_chunk(const uint4_t &c, float (&v)[Elem<DT>::V]) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const unsigned w = c[i];
+    if constexpr (DT == kF32) {
+      v[i] = __uint_as_float(w);
+    } else {
+      v[2 * i] = Elem<DT>::load((uint16_t)(w & 0xffffu));
+      v[2 * i + 1] = Elem<DT>::load((uint16_t)(w >> 16));
+    }
+  }
+}
+template <int DT>
+TCU_DEVICE uint4_t pack_chunk(const float (&v)[Elem<DT>::V]) {
+  uint4_t c;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if constexpr (DT == kF32)
+      c[i] = __float_as_uint(v[i]);
+    else
+      c[i] = Elem<DT>::pack(v[2 * i], v[2 * i + 1]);
+  }
+  return c;
+}
+
+// The chunk at element `at` of p, of which `count` elements exist (count <= 0: none; the others read as 0).
+// ALIGNED: p + at is 16-byte aligned and count is 0 or at least V.
+template <int DT, bool ALIGNED, bool NT = true>
+TCU_DEVICE uint4_t load_chunk_of(const void *p, size_t at, int count) {
+  constexpr int V = Elem<DT>::V;
+  uint4_t c = {0u, 0u, 0u, 0u};
+  if constexpr (ALIGNED) {
+    if (count > 0) {
+      const uint4_t *q = reinterpret_cast<const uint4_t *>(static_cast<const typename Elem<DT>::word_t *>(p) + at);
+      if constexpr (NT)
+        c = __builtin_nontemporal_load(q);
+      else
+        c = *q;
+    }
+  } else {
+    const typename Elem<DT>::word_t *q = static_cast<const typename Elem<DT>::word_t *>(p) + at;
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      if (e < count) {
+        const unsigned w = q[e];
+        if constexpr (DT == kF32)
+          c[e] = w;
+        else
+          c[e / 2] |= w << (16 * (e % 2));
+      }
+    }
+  }
+  return c;
+}
+template <int DT, bool ALIGNED, bool NT = true>
+TCU_DEVICE void store_chunk_of(void *p, size_t at, int count, const float (&v)[Elem<DT>::V]) {
+  constexpr int V = Elem<DT>::V;
+  if constexpr (ALIGNED) {
+    if (count > 0) {
+      uint4_t *q = reinterpret_cast<uint4_t *>(static_cast<typename Elem<DT>::word_t *>(p) + at);
+      const uint4_t c = pack_chunk<DT>(v);
+      if constexpr (NT)
+        __builtin_nontemporal_store(c, q);
+      else
+        *q = c;
+    }
+  } else {
+    typename Elem<DT>::word_t *q = static_cast<typename Elem<DT>::word_t *>(p) + at;
+#pragma unroll
+    for (int e = 0; e < V; e++)
+      if (e < count) q[e] = Elem<DT>::round(v[e]);
+  }
+}
+
+// V fp32 values at element `at` of a fp32 vector, the same conventions
+template <int V, bool ALIGNED>
+TCU_DEVICE void load_floats(const float *p, size_t at, int count, float (&v)[V]) {
+  if constexpr (ALIGNED) {
+    if (count > 0) {
+#pragma unroll
+      for (int i = 0; i < V / 4; i++) {
+        const float4_t q = *reinterpret_cast<const float4_t *>(p + at + 4 * i);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[4 * i + e] = q[e];
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < V; e++) v[e] = e < count ? p[at + e] : 0.0f;
+}
+template <int V, bool ALIGNED>
+TCU_DEVICE void store_floats(float *p, size_t at, int count, const float (&v)[V]) {
+  if constexpr (ALIGNED) {
+    if (count > 0) {
+#pragma unroll
+      for (int i = 0; i < V / 4; i++) *reinterpret_cast<float4_t *>(p + at + 4 * i) = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e++)
+      if (e < count) p[at + e] = v[e];
+  }
+}
+
+// e^x.  EXACT carries the rounding error of x * log2(e) along (a relative error of |x| 2^-24 otherwise, which results that
+// are rounded to 16 bits do not show and fp32 ones would).
+template <bool EXACT>
+TCU_DEVICE float exp_of(float x) {
+  constexpr float kLog2E = 1.44269504088896340736f, kLog2ELow = 1.92596299112661746887e-8f, kLn2 = 0.69314718055994530942f;
+  const float hi = x * kLog2E;
+  if constexpr (EXACT) {
+    float lo = __builtin_fmaf(x, kLog2E, -hi);
+    lo = __builtin_fmaf(x, kLog2ELow, lo);
+    const float e = hw_exp2(hi);
+    // beyond the range of fp32 (and for an infinite x, whose error term is not a number) e is already the answer
+    return __builtin_fabsf(hi) < 128.0f ? __builtin_fmaf(e * lo, kLn2, e) : e;
+  }
+  return hw_exp2(hi);
+}
+// s = 1 / (1 + e^-x) and 1 - s, the second as e^-x s: 1 - s would lose the digits that matter where s is close to 1.
+// e^-x is held below 2^126 so that both stay finite numbers (a NaN stays a NaN: it fails the comparison).
+template <bool EXACT>
+TCU_DEVICE void sigmoid_pair(float x, float *s, float *one_minus) {
+  const float y = x < -87.0f ? -87.0f : x;
+  const float e = exp_of<EXACT>(-y);
+  *s = hw_rcp(1.0f + e);
+  *one_minus = e * *s;
+}
+
+}  // namespace tcu

@@ -1,0 +1,36 @@
+// Builds the recurrent-block operators of tcu_scope_amd/csrc against the CPU lane emulator (TEST INFRASTRUCTURE ONLY).
+#include "wave_ops_emu.hpp"
+//
+#include "block_ops_emu.hpp"
+//
+#include "../../tcu_scope_amd/csrc/gated_scan_host.hpp"
+
+namespace tcu {
+static std::string g_error;
+static unsigned g_poll_limit = 1u << 20, g_mute = 0;
+int report_failure(int code, const std::string &message) {
+  g_error = message;
+  return code;
+}
+unsigned shared_poll_limit() { return g_poll_limit; }
+unsigned shared_mute_partition() { return g_mute; }
+}  // namespace tcu
+
+extern "C" {
+const char *emu_last_error() { return tcu::g_error.c_str(); }
+void emu_waits(unsigned poll_limit, unsigned mute) {
+  tcu::g_poll_limit = poll_limit;
+  tcu::g_mute = mute;
+}
+int emu_gated_scan(const tcu_gated_scan_shape *s, const void *x, size_t xs, const void *g, size_t gs, void *h, size_t hs, const void *h0, void *h_last, void *ws, size_t *wb) {
+  return tcu::gated_scan_dispatch(s, x, xs, g, gs, h, hs, h0, h_last, ws, wb, nullptr);
+}
+int emu_gated_scan_backward(const tcu_gated_scan_shape *s, const void *dh, size_t dhs, const void *x, size_t xs, const void *g, size_t gs, const void *h, size_t hs, const void *h0, const void *dh_last, void *dx,
+                            size_t dxs, void *dg, size_t dgs, void *dh0, void *ws, size_t *wb) {
+  return tcu::gated_scan_backward_dispatch(s, dh, dhs, x, xs, g, gs, h, hs, h0, dh_last, dx, dxs, dg, dgs, dh0, ws, wb, nullptr);
+}
+int emu_gated_scan_step(int dtype, int gate, size_t channels, size_t rows, const void *x, size_t xs, const void *g, size_t gs, void *h, size_t hs, const void *state, void *new_state, size_t num_slots,
+                        const void *slots, int zero_padding) {
+  return tcu::gated_scan_step_dispatch(dtype, gate, channels, rows, x, xs, g, gs, h, hs, state, new_state, num_slots, slots, zero_padding, nullptr);
+}
+}

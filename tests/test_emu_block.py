@@ -1,0 +1,354 @@
+"""The recurrent-block operators' kernel sources (gated scan, fused norm, fused product) run lane by lane on the CPU, as
+tests/test_emu_kernels.py does for the others: every array ends at an inaccessible page, so an access out of bounds ends the
+run.  References and bounds: tests/block_reference.py."""
+import ctypes
+import itertools
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+import block_reference as ref
+from test_emu_kernels import CLANG, EMU, HERE, aligned
+
+DTYPES = {"f16": 0, "bf16": 1, "f32": 2}
+GATES = {"decay": 0, "log": 1, "sigmoid": 2}
+vp, sz, ci, cf = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int, ctypes.c_float
+
+
+class Shape(ctypes.Structure):
+    _fields_ = [("dtype", ci), ("gate", ci), ("channels", sz), ("num_rows", sz), ("num_sequences", sz), ("sequence_length", sz), ("d_offsets", vp), ("offset_bits", ci), ("zero_outside", ci)]
+
+
+@pytest.fixture(scope="module")
+def emu():
+    if not os.path.exists(CLANG):
+        pytest.skip("host clang++ (ROCm LLVM) not available")
+    lib = os.path.join(EMU, "libtcu_emu_block.so")
+    csrc = os.path.join(HERE, "..", "tcu_scope_amd", "csrc")
+    srcs = [os.path.join(EMU, f) for f in ("emu_block_driver.cpp", "block_ops_emu.hpp", "wave_ops_emu.hpp")] + [os.path.join(csrc, f) for f in os.listdir(csrc) if f.endswith(".hpp")]
+    srcs.append(os.path.join(HERE, "..", "include", "tcu_scope.h"))
+    if not os.path.exists(lib) or any(os.path.getmtime(s) > os.path.getmtime(lib) for s in srcs):
+        subprocess.check_call([CLANG, "-x", "c++", "-std=c++17", "-O1", "-fPIC", "-shared", "-Wno-psabi", "-I" + EMU, "-o", lib, os.path.join(EMU, "emu_block_driver.cpp")])
+    L = ctypes.CDLL(lib)
+    shape, psz = ctypes.POINTER(Shape), ctypes.POINTER(sz)
+    L.emu_gated_scan.argtypes = [shape, vp, sz, vp, sz, vp, sz, vp, vp, vp, psz]
+    L.emu_gated_scan_backward.argtypes = [shape, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, sz, vp, sz, vp, vp, psz]
+    L.emu_gated_scan_step.argtypes = [ci, ci, sz, sz, vp, sz, vp, sz, vp, sz, vp, vp, sz, vp, ci]
+    L.emu_waits.argtypes = [ctypes.c_uint, ctypes.c_uint]
+    L.emu_last_error.restype = ctypes.c_char_p
+    return L
+
+
+def storage(dtype):
+    return np.float32 if dtype == "f32" else np.uint16
+
+
+class Matrix:
+    """rows x width elements of a guarded array, `stride` apart, `shift` elements behind its start; what lies between holds a marker."""
+
+    def __init__(self, values, dtype, stride=None, shift=0):
+        self.dtype, (self.rows, self.width), self.shift = dtype, values.shape, shift
+        self.stride = stride or self.width
+        n = shift + max(self.rows - 1, 0) * self.stride + self.width if self.rows else shift
+        self.flat = aligned(max(n, 1), storage(dtype))
+        self.flat[:] = ref.to_bits(np.full(self.flat.size, -77.0), dtype)
+        self.put(values)
+
+    def view(self):
+        return np.lib.stride_tricks.as_strided(self.flat[self.shift:], (self.rows, self.width), (self.stride * self.flat.itemsize, self.flat.itemsize))
+
+    def put(self, values):
+        if self.rows:
+            self.view()[...] = ref.to_bits(values, self.dtype)
+
+    @property
+    def ptr(self):
+        return self.flat.ctypes.data + self.shift * self.flat.itemsize
+
+    def get(self):
+        return ref.to_f64(np.ascontiguousarray(self.view()), self.dtype) if self.rows else np.zeros((0, self.width))
+
+    def untouched_between(self):
+        mark = ref.to_bits(np.full(1, -77.0), self.dtype)[0]
+        mask = np.ones(self.flat.size, bool)
+        for r in range(self.rows):
+            mask[self.shift + r * self.stride:self.shift + r * self.stride + self.width] = False
+        return (self.flat[mask] == mark).all()
+
+
+def floats(values):
+    a = aligned(max(values.size, 1), np.float32)
+    a[:values.size] = np.asarray(values, dtype=np.float32).reshape(-1)
+    return a
+
+
+def gates(rng, gate, shape):
+    z = rng.standard_normal(shape)
+    return {"sigmoid": z * 1.5 + 2, "log": -np.exp(z * 1.2 - 3), "decay": ref.sigmoid(z * 1.5 + 2) * np.where(rng.random(shape) < 0.2, -1, 1)}[gate]
+
+
+def scan_case(rng, dtype, gate, offsets, rows, channels, stride=None, shift=0):
+    f = lambda v: ref.to_f64(ref.to_bits(v, dtype), dtype)
+    x, g = f(rng.standard_normal((rows, channels))), f(gates(rng, gate, (rows, channels)))
+    h0 = rng.standard_normal((len(offsets) - 1, channels)).astype(np.float32).astype(np.float64)
+    return x, g, h0
+
+
+def shape_of(dtype, gate, rows, channels, offsets=None, bits=32, sequences=None, zero_outside=0):
+    s = Shape(dtype=DTYPES[dtype], gate=GATES[gate], channels=channels, num_rows=rows, zero_outside=zero_outside)
+    keep = None
+    if offsets is not None:
+        keep = aligned(len(offsets), np.int32 if bits == 32 else np.int64)
+        keep[:] = offsets
+        s.num_sequences, s.d_offsets, s.offset_bits = len(offsets) - 1, keep.ctypes.data, bits
+    else:
+        s.num_sequences, s.sequence_length = sequences, rows // sequences if sequences else 0
+    return s, keep
+
+
+def workspace_for(call):
+    need = sz(0)
+    assert call(None, ctypes.byref(need)) == 0
+    # the emulator hands out 16-byte alignment at least; a workspace is 256-byte aligned
+    ws = aligned(need.value + 256, np.uint8, 0xA5)
+    off = -ws.ctypes.data % 256
+    return ws, ws.ctypes.data + off, sz(need.value)
+
+
+def run_scan(emu, s, x, g, h, h0, last):
+    call = lambda ws, need: emu.emu_gated_scan(ctypes.byref(s), x.ptr, x.stride, g.ptr, g.stride, h.ptr, h.stride, h0, last, ws, need)
+    keep, ws, have = workspace_for(call)
+    return call(ws, ctypes.byref(have))
+
+
+LAYOUTS = [
+    # rows, channels, offsets or number of equal sequences, stride - channels, shift
+    (1, 8, 1, 0, 0),
+    (5, 1, 1, 0, 0),
+    (6, 13, 3, 0, 0),
+    (131, 24, 1, 8, 8),
+    (300, 136, 2, 0, 0),
+    (290, 20, 290, 0, 0),
+    (1300, 16, 1, 0, 0),
+    (400, 40, [0, 0, 1, 130, 130, 257, 399, 399], 0, 0),
+    (257, 9, [3, 3, 100, 129, 240], 5, 3),
+    (64, 8, [64, 64], 0, 0),
+    (1200, 8, [0, 5, 1190], 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype,gate", [("f16", "sigmoid"), ("bf16", "log"), ("f32", "decay"), ("f32", "sigmoid"), ("f32", "log")])
+@pytest.mark.parametrize("layout", LAYOUTS, ids=lambda v: f"{v[0]}x{v[1]}" + ("p" if isinstance(v[2], list) else f"s{v[2]}"))
+def test_gated_scan_and_gradient(emu, dtype, gate, layout):
+    rows, channels, seqs, gap, shift = layout
+    rng = np.random.default_rng(rows * 31 + channels)
+    packed = isinstance(seqs, list)
+    offsets = seqs if packed else [j * (rows // seqs) for j in range(seqs + 1)]
+    x, g, h0 = scan_case(rng, dtype, gate, offsets, rows, channels)
+    mx, mg = Matrix(x, dtype, channels + gap, shift), Matrix(g, dtype, channels + 2 * gap, shift)
+    mh = Matrix(np.full((rows, channels), 5.0), dtype, channels + gap, 0)
+    s, keep = shape_of(dtype, gate, rows, channels, seqs if packed else None, 64 if channels % 2 else 32, None if packed else seqs)
+    f0, last = floats(h0), floats(np.full(h0.shape, 9.0))
+    assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0, emu.emu_last_error()
+    h, want_last, e, elast = ref.scan(gate, x, g, offsets, h0)
+    outside = np.isnan(h[:, 0])
+    ref.check(mh.get()[~outside], h[~outside], e[~outside], dtype, "h")
+    assert (mh.get()[outside] == 5.0).all() and mh.untouched_between() and mx.untouched_between()
+    ref.check(last.reshape(h0.shape), want_last, elast, "f32", "h_last")
+    # without states, outputs in the place of an input, zeros outside
+    s.zero_outside = 1
+    inplace = Matrix(x, dtype, channels + gap, 0)
+    assert run_scan(emu, s, inplace, mg, inplace, None, None) == 0
+    h, _, e, _ = ref.scan(gate, x, g, offsets, np.zeros(h0.shape))
+    ref.check(inplace.get(), np.where(np.isnan(h), 0, h), e, dtype, "h in place")
+    # the gradient, from states of any origin
+    hs = ref.to_f64(ref.to_bits(rng.standard_normal((rows, channels)), dtype), dtype)
+    dh = ref.to_f64(ref.to_bits(rng.standard_normal((rows, channels)), dtype), dtype)
+    dlast = rng.standard_normal(h0.shape).astype(np.float32).astype(np.float64)
+    mhs, mdh = Matrix(hs, dtype, channels + gap, shift), Matrix(dh, dtype)
+    mdx, mdg = Matrix(np.full((rows, channels), 5.0), dtype), Matrix(np.full((rows, channels), 5.0), dtype, channels + gap)
+    for with_states in (True, False):
+        s.zero_outside = 0 if with_states else 1
+        fl, d0 = floats(dlast), floats(np.full(h0.shape, 9.0))
+        call = lambda ws, need: emu.emu_gated_scan_backward(ctypes.byref(s), mdh.ptr, mdh.stride, mx.ptr if gate == "sigmoid" else None, mx.stride, mg.ptr, mg.stride, mhs.ptr, mhs.stride, f0.ctypes.data if with_states else None,
+                                                            fl.ctypes.data if with_states else None, mdx.ptr, mdx.stride, mdg.ptr, mdg.stride, d0.ctypes.data if with_states else None, ws, need)
+        kept, ws, have = workspace_for(call)
+        assert call(ws, ctypes.byref(have)) == 0, emu.emu_last_error()
+        zero = np.zeros(h0.shape)
+        (dx, dg, dh0), (ex, eg, e0) = ref.scan_backward(gate, x, g, hs, dh, offsets, h0 if with_states else zero, dlast if with_states else zero)
+        fillv = 5.0 if with_states else 0.0
+        ref.check(mdx.get(), np.where(np.isnan(dx), fillv, dx), ex, dtype, "dx")
+        ref.check(mdg.get(), np.where(np.isnan(dg), fillv, dg), eg, dtype, "dg")
+        if with_states:
+            ref.check(d0.reshape(h0.shape), dh0, e0, "f32", "dh0")
+    assert mdg.untouched_between()
+
+
+def test_gradient_against_differences(emu):
+    """dx, dg and dh0 against central differences of the 64-bit forward recurrence (step 1e-5: off by about 1e-9)."""
+    rng = np.random.default_rng(3)
+    offsets, rows, channels = [0, 3, 3, 7], 7, 4
+    for gate in GATES:
+        x, g, h0 = scan_case(rng, "f32", gate, offsets, rows, channels)
+        dh = rng.standard_normal((rows, channels))
+        dl = rng.standard_normal(h0.shape)
+        loss = lambda x, g, h0: (lambda r: float((r[0] * dh).sum() + (r[1] * dl).sum()))(ref.scan(gate, x, g, offsets, h0))
+        h = ref.scan(gate, x, g, offsets, h0)[0]
+        (dx, dg, dh0), _ = ref.scan_backward(gate, x, g, h, dh, offsets, h0, dl)
+        for k, (v, d) in enumerate(((x, dx), (g, dg), (h0, dh0))):
+            for at in itertools.product(*(range(n) for n in v.shape)):
+                lo, hi = v.copy(), v.copy()
+                lo[at] -= 1e-5
+                hi[at] += 1e-5
+                args = lambda w: tuple(w if i == k else u for i, u in enumerate((x, g, h0)))
+                assert abs((loss(*args(hi)) - loss(*args(lo))) / 2e-5 - d[at]) < 1e-7
+
+
+def test_no_rows_and_empty_sequences(emu):
+    h0 = np.arange(12, dtype=np.float64).reshape(3, 4)
+    empty = Matrix(np.zeros((0, 4)), "f32")
+    for seqs in (3, [0, 0, 0, 0]):
+        s, keep = shape_of("f32", "log", 0, 4, seqs if isinstance(seqs, list) else None, 32, seqs)
+        f0, last = floats(h0), floats(np.full(h0.shape, 9.0))
+        assert run_scan(emu, s, empty, empty, empty, f0.ctypes.data, last.ctypes.data) == 0
+        assert (last.reshape(3, 4) == h0).all()
+        assert run_scan(emu, s, empty, empty, empty, None, last.ctypes.data) == 0
+        assert (last == 0).all()
+    s, keep = shape_of("f32", "log", 0, 4, [0], 32)
+    assert run_scan(emu, s, empty, empty, empty, None, None) == 0
+
+
+def test_states_do_not_pass_between_sequences(emu):
+    """An infinite or NaN state stays in its sequence: a sequence's beginning replaces what came before, it does not multiply it by 0."""
+    rows, channels = 400, 8
+    offsets = [0, 150, 400]
+    rng = np.random.default_rng(5)
+    for bad in (np.inf, np.nan):
+        x, g, h0 = scan_case(rng, "f32", "decay", offsets, rows, channels)
+        g = np.abs(g) + 0.01
+        x[10] = bad
+        mx, mg, mh = Matrix(x, "f32"), Matrix(g, "f32"), Matrix(np.zeros((rows, channels)), "f32")
+        s, keep = shape_of("f32", "decay", rows, channels, offsets)
+        f0, last = floats(h0), floats(h0)
+        assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0
+        got = mh.get()
+        assert np.isfinite(got[:10]).all() and np.isfinite(got[150:]).all() and not np.isfinite(got[10:150]).any()
+
+
+def test_gate_extremes(emu):
+    """Gates at the ends of their range, and a NaN gate, which has to show."""
+    g = np.array([[-np.inf, -200.0, -87.5, 0.0, 87.5, 200.0, np.inf, np.nan]])
+    x, h0 = np.full(g.shape, 3.0), np.full(g.shape, 2.0)
+    for dtype in DTYPES:
+        mx, mg, mh = Matrix(x, dtype), Matrix(g, dtype), Matrix(x, dtype)
+        s, keep = shape_of(dtype, "sigmoid", 1, 8, None, 32, 1)
+        f0, last = floats(h0), floats(h0)
+        assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0
+        got = mh.get()[0]
+        assert np.allclose(got[:7], [3, 3, 3, 2.5, 2, 2, 2], rtol=2.0 ** -8, atol=0) and np.isnan(got[7])
+        gl = np.array([[-np.inf, -200.0, -1.0, 0.0, 1.0, 2.0, np.inf, np.nan]])
+        mg = Matrix(gl, dtype)
+        s, keep = shape_of(dtype, "log", 1, 8, None, 32, 1)
+        assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0
+        got = mh.get()[0]
+        assert np.allclose(got[:6], [3, 3, 3 + 2 * np.exp(-1), 5, 3 + 2 * np.exp(1), 3 + 2 * np.exp(2)], rtol=2.0 ** -8) and got[6] == np.inf and np.isnan(got[7])
+
+
+def test_waits_that_expire_leave_nan(emu):
+    """A tile that publishes nothing (test switch) and a poll limit of 3: everything that depended on it is NaN up to the end of the sequence, nothing else is."""
+    rows, channels = 2600, 8  # 128 places a tile: tiles 0 ... 20, one strip
+    offsets = [0, 2000, 2600]
+    rng = np.random.default_rng(9)
+    x, g, h0 = scan_case(rng, "f16", "sigmoid", offsets, rows, channels)
+    want, want_last, e, _ = ref.scan("sigmoid", x, g, offsets, h0)
+    mx, mg, mh = Matrix(x, "f16"), Matrix(g, "f16"), Matrix(np.zeros((rows, channels)), "f16")
+    s, keep = shape_of("f16", "sigmoid", rows, channels, offsets)
+    f0, last = floats(h0), floats(h0)
+    emu.emu_waits(3, 1 + 4)  # tile 4 is mute
+    try:
+        assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0
+    finally:
+        emu.emu_waits(1 << 20, 0)
+    got, tile = mh.get(), 128
+    ok = np.r_[0:5 * tile, 2000:rows]
+    ref.check(got[ok], want[ok], e[ok], "f16", "what did not wait")
+    assert np.isnan(got[5 * tile:2000]).all() and np.isnan(last.reshape(2, channels)[0]).all() and np.isfinite(last.reshape(2, channels)[1]).all()
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("gate", list(GATES))
+@pytest.mark.parametrize("rows,channels,slots,gap", [(1, 8, None, 0), (3, 520, None, 8), (5, 13, [4, 0, 6, 1, 2], 3), (7, 16, [3, -1, 3, 9, 3, 1, -5], 0), (70, 8, "many", 0)])
+def test_gated_scan_step(emu, dtype, gate, rows, channels, slots, gap):
+    rng = np.random.default_rng(rows)
+    x, g, _ = scan_case(rng, dtype, gate, [0], rows, channels)
+    num_slots = 7 if slots != "many" else 5
+    at = list(range(rows)) if slots is None else [int(v) for v in rng.integers(-1, 5, rows)] if slots == "many" else slots
+    state = rng.standard_normal((num_slots, channels)).astype(np.float32).astype(np.float64)
+    mx, mg, mh = Matrix(x, dtype, channels + gap), Matrix(g, dtype, channels + gap), Matrix(np.full((rows, channels), 5.0), dtype)
+    ps = None
+    if slots is not None:
+        ps = aligned(rows, np.int32)
+        ps[:] = at
+    a, keep, c = ref.gate_terms(gate, g)
+    c = np.broadcast_to(c, g.shape)
+    want_state, err = state.copy(), np.zeros(state.shape)
+    want_h, eh = np.full((rows, channels), 5.0), np.zeros((rows, channels))
+    for i, j in enumerate(at):
+        if 0 <= j < num_slots:
+            m = np.abs(a[i] * want_state[j]) + np.abs(keep[i] * x[i])
+            want_state[j] = a[i] * want_state[j] + keep[i] * x[i]
+            err[j] = np.abs(a[i]) * err[j] + (c[i] + 4.0) * ref.EPS32 * m
+            want_h[i], eh[i] = want_state[j], err[j]
+    for inplace in (False, True):
+        st = floats(state)
+        new = st if inplace else floats(np.full(state.shape, 9.0))
+        assert emu.emu_gated_scan_step(DTYPES[dtype], GATES[gate], channels, rows, mx.ptr, mx.stride, mg.ptr, mg.stride, mh.ptr, mh.stride, st.ctypes.data, new.ctypes.data, num_slots, ps.ctypes.data if ps is not None else None, 0) == 0
+        ref.check(mh.get(), want_h, eh, dtype, "h")
+        named = sorted({j for j in at if 0 <= j < num_slots})
+        ref.check(new.reshape(state.shape)[named], want_state[named], err[named], "f32", "state")
+        rest = [j for j in range(num_slots) if j not in named]
+        assert (new.reshape(state.shape)[rest] == (state[rest].astype(np.float32) if inplace else 9.0)).all()
+
+
+def test_gated_scan_refusals(emu):
+    buf = aligned(4096, np.uint8, 0)
+    p = buf.ctypes.data
+    err = lambda: emu.emu_last_error().decode()
+    need = sz(0)
+    big = sz(1 << 40)
+
+    def scan(s, x=p, xs=8, g=p, gs=8, h=p, hs=8, h0=None, last=None, ws=p // 256 * 256 + 256, have=big):
+        return emu.emu_gated_scan(ctypes.byref(s) if s else None, x, xs, g, gs, h, hs, h0, last, ws, ctypes.byref(have) if have else None)
+
+    ok = lambda **k: Shape(**{**dict(dtype=0, gate=2, channels=8, num_rows=0, num_sequences=1, sequence_length=0), **k})
+    assert scan(None) == 1 and "null shape" in err()
+    assert scan(ok(dtype=3)) == 1 and "dtype" in err()
+    assert scan(ok(gate=3)) == 1 and "gate" in err()
+    assert scan(ok(channels=0)) == 1 and "channels" in err()
+    assert scan(ok(num_rows=5)) == 1 and "num_rows" in err()
+    assert scan(ok(num_sequences=1 << 20, sequence_length=1 << 20, num_rows=1 << 40)) == 2 and "rows" in err()
+    assert scan(ok(d_offsets=p, offset_bits=16)) == 1 and "offset_bits" in err()
+    assert scan(ok(d_offsets=p + 2, offset_bits=32)) == 1 and "aligned" in err()
+    assert scan(ok(), have=None) == 1 and "workspace_bytes" in err()
+    two = ok(num_rows=2, sequence_length=2)
+    assert emu.emu_gated_scan(ctypes.byref(two), None, 8, None, 8, None, 8, None, None, None, ctypes.byref(need)) == 0 and need.value == 256
+    assert scan(two, have=sz(255)) == 4 and "workspace" in err()
+    assert scan(two, ws=p // 256 * 256 + 264) == 1 and "256-byte" in err()
+    assert scan(two, x=None) == 1 and "d_x is null" in err()
+    assert scan(two, gs=7) == 1 and "d_g overlap" in err()
+    assert scan(two, h=p + 1) == 1 and "d_h is not aligned" in err()
+    assert scan(two, xs=1 << 63) == 1 and "overflows" in err()
+    assert scan(two, h0=p + 2) == 1 and "d_h0" in err()
+    back = lambda s, dx, dg, h=p: emu.emu_gated_scan_backward(ctypes.byref(s), p, 8, p, 8, p, 8, h, 8, None, None, dx, 8, dg, 8, None, p // 256 * 256 + 256, ctypes.byref(big))
+    assert back(two, p, p + 64) == 1 and "d_h" in err()
+    assert back(two, p + 64, p + 64) == 1 and "same buffer" in err()
+    assert back(two, None, p + 64) == 1 and "d_dx is null" in err()
+    step = lambda rows=2, num_slots=2, slots=None, state=p, channels=8, dtype=0: emu.emu_gated_scan_step(dtype, 2, channels, rows, p, 8, p, 8, p, 8, state, state, num_slots, slots, 0)
+    assert step(num_slots=1) == 1 and "slots" in err()
+    assert step(num_slots=0, slots=p) == 1 and "num_slots" in err()
+    assert step(slots=p + 2) == 1 and "d_slots" in err()
+    assert step(state=None) == 1 and "d_state" in err()
+    assert step(dtype=7) == 1 and "dtype" in err()
+    assert step(rows=0) == 0
