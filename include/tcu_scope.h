@@ -277,6 +277,14 @@ int tcu_gemm_f16_f16(const void *d_A, const void *d_B, const void *d_C, void *d_
 
 typedef enum { TCU_F16 = 0, TCU_BF16 = 1, TCU_F32 = 2 } tcu_dtype;
 
+typedef enum {
+  TCU_ACT_NONE = 0,
+  TCU_ACT_RELU = 1,
+  TCU_ACT_GELU = 2, /* the tanh form: z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) / 2 */
+  TCU_ACT_SILU = 3,
+  TCU_ACT_SIGMOID = 4
+} tcu_activation;
+
 /* Gated scan: h[t] = a[t] h[t-1] + b[t] down the rows of each sequence, every channel by itself, h[-1] = the sequence's
  * row of d_h0 (0 if d_h0 is NULL). */
 typedef enum {
@@ -315,6 +323,36 @@ int tcu_gated_scan_backward(const tcu_gated_scan_shape *shape, const void *d_dh,
  * names are not written) and, rounded, to row i of d_h.  Rows whose slot is negative or not below num_slots are padding:
  * not read, and in d_h left as they are (zero_padding 0) or set to zero.  Rows that name the same slot advance it one after the other, in row order. */
 int tcu_gated_scan_step(int dtype, int gate, size_t channels, size_t num_rows, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, void *d_h, size_t h_stride, const float *d_state, float *d_new_state, size_t num_slots, const int32_t *d_slots, int zero_padding, void *stream);
+
+/* Fused norm of every row, with s = scale * d_channel_scale (one number per channel, NULL: 1):
+ *   TCU_ORDER_ADD_NORM  z = residual + s x (z = x without a residual, and no scale then); out = act(gate) y(z); z is
+ *                       written to d_residual_out (NULL: it is not kept)
+ *   TCU_ORDER_NORM_ADD  out = residual + s act(gate) y(x) (without a residual: s act(gate) y(x))
+ *   y(z) = (z - mean) rho weight + bias, where TCU_NORM_RMS has mean = 0, rho = 1 / sqrt(mean of z^2 + eps) and
+ *   TCU_NORM_LAYER the mean of the row, rho = 1 / sqrt(mean of (z - mean)^2 + eps).
+ * weight NULL: 1, bias NULL: 0, gate NULL: 1.  The norm is taken of the fp32 sum, before z is rounded. */
+typedef enum { TCU_NORM_RMS = 0, TCU_NORM_LAYER = 1 } tcu_norm;
+typedef enum { TCU_ORDER_ADD_NORM = 0, TCU_ORDER_NORM_ADD = 1 } tcu_norm_order;
+typedef struct {
+  int dtype;      /* tcu_dtype of all matrices and of weight, bias and channel scale */
+  int norm;       /* tcu_norm */
+  int order;      /* tcu_norm_order */
+  int activation; /* tcu_activation of the gate; TCU_ACT_NONE without one */
+  size_t rows;    /* below 2^31 */
+  size_t dim;     /* 1 ... 32768 */
+  float eps, scale;
+} tcu_fused_norm_shape;
+
+/* d_out and d_residual_out (not the same buffer) may each take the place of an input with the same stride. */
+int tcu_fused_norm(const tcu_fused_norm_shape *shape, const void *d_x, size_t x_stride, const void *d_residual, size_t residual_stride, const void *d_gate, size_t gate_stride, const void *d_weight, const void *d_bias, const void *d_channel_scale, void *d_out, size_t out_stride, void *d_residual_out, size_t residual_out_stride, void *stream);
+
+/* The gradient.  d_z: what was normed (ADD_NORM with a residual: d_residual_out as the forward call wrote it; otherwise x).
+ * d_dresidual_out (ADD_NORM, may be NULL): the gradient with respect to d_residual_out, added to that of z.  Written: d_dx,
+ * and those of d_dgate, d_dresidual (ADD_NORM; with NORM_ADD the residual's gradient is d_dout itself), d_dweight, d_dbias
+ * and d_dchannel_scale that are not NULL; the last three are fp32, summed over all rows (zero without rows).
+ * d_dchannel_scale with ADD_NORM reads d_x.  A gradient may take the place of a matrix with the same stride.
+ * Bit-reproducible. */
+int tcu_fused_norm_backward(const tcu_fused_norm_shape *shape, const void *d_dout, size_t dout_stride, const void *d_z, size_t z_stride, const void *d_gate, size_t gate_stride, const void *d_weight, const void *d_bias, const void *d_channel_scale, const void *d_x, size_t x_stride, const void *d_dresidual_out, size_t dresidual_out_stride, void *d_dx, size_t dx_stride, void *d_dgate, size_t dgate_stride, void *d_dresidual, size_t dresidual_stride, float *d_dweight, float *d_dbias, float *d_dchannel_scale, void *d_workspace, size_t *workspace_bytes, void *stream);
 
 /* ---- fills, conversions, inputs ---------------------------------------------------------------- */
 

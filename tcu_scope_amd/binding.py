@@ -13,7 +13,7 @@ EXPORTS = [
     "tcu_abi_version", "tcu_last_error", "tcu_init", "tcu_device_info", "tcu_set_option",
     "tcu_seg_reduce_f16", "tcu_seg_reduce_offsets_f16", "tcu_seg_scan_f16", "tcu_seg_scan_f16_noalloc", "tcu_seg_scan_offsets_f16", "tcu_seg_scan_by_key_f16", "tcu_seg_reduce_by_key_f16", "tcu_add_partial_sums_f16",
     "tcu_full_reduce_f16", "tcu_full_scan_f16", "tcu_gemv_f16_f32", "tcu_gemm_f16_f32", "tcu_gemv_f16_f16", "tcu_gemm_f16_f16", "tcu_gemv_col_major_f16_f32", "tcu_gemv_col_major_f16_f16",
-    "tcu_gated_scan", "tcu_gated_scan_backward", "tcu_gated_scan_step",
+    "tcu_gated_scan", "tcu_gated_scan_backward", "tcu_gated_scan_step", "tcu_fused_norm", "tcu_fused_norm_backward",
     "tcu_fill_f16", "tcu_convert_f32_to_f16", "tcu_generate_f16", "tcu_stream_probe", "tcu_time_next_launch", "tcu_lane_probe", "tcu_temporary_allocations",
 ]
 
@@ -58,11 +58,40 @@ class Gate(enum.IntEnum):
     SIGMOID = 2
 
 
+class Activation(enum.IntEnum):
+    """Activations of a gate and of a product's epilogue; GELU is the tanh form."""
+
+    NONE = 0
+    RELU = 1
+    GELU = 2
+    SILU = 3
+    SIGMOID = 4
+
+
+class Norm(enum.IntEnum):
+    RMS = 0
+    LAYER = 1
+
+
+class NormOrder(enum.IntEnum):
+    """ADD_NORM: the norm of residual + s x; NORM_ADD: residual + s times the (gated) norm of x."""
+
+    ADD_NORM = 0
+    NORM_ADD = 1
+
+
 class GatedScanShape(ctypes.Structure):
     """tcu_gated_scan_shape."""
 
     _fields_ = [("dtype", ctypes.c_int), ("gate", ctypes.c_int), ("channels", ctypes.c_size_t), ("num_rows", ctypes.c_size_t), ("num_sequences", ctypes.c_size_t), ("sequence_length", ctypes.c_size_t),
                 ("d_offsets", ctypes.c_void_p), ("offset_bits", ctypes.c_int), ("zero_outside", ctypes.c_int)]
+
+
+class FusedNormShape(ctypes.Structure):
+    """tcu_fused_norm_shape."""
+
+    _fields_ = [("dtype", ctypes.c_int), ("norm", ctypes.c_int), ("order", ctypes.c_int), ("activation", ctypes.c_int), ("rows", ctypes.c_size_t), ("dim", ctypes.c_size_t), ("eps", ctypes.c_float),
+                ("scale", ctypes.c_float)]
 
 
 class TcuError(RuntimeError):
@@ -129,6 +158,9 @@ def lib():
         L.tcu_gated_scan.argtypes = [shape, vp, sz, vp, sz, vp, sz, vp, vp, vp, psz, vp]
         L.tcu_gated_scan_backward.argtypes = [shape, vp, sz, vp, sz, vp, sz, vp, sz, vp, vp, vp, sz, vp, sz, vp, vp, psz, vp]
         L.tcu_gated_scan_step.argtypes = [ci, ci, sz, sz, vp, sz, vp, sz, vp, sz, vp, vp, sz, vp, ci, vp]
+        norm, m = c.POINTER(FusedNormShape), [vp, sz]
+        L.tcu_fused_norm.argtypes = [norm, *m * 3, vp, vp, vp, *m * 2, vp]
+        L.tcu_fused_norm_backward.argtypes = [norm, *m * 3, vp, vp, vp, *m * 5, vp, vp, vp, vp, psz, vp]
         for name in EXPORTS:
             if name not in ("tcu_last_error", "tcu_temporary_allocations"):
                 getattr(L, name).restype = ci
@@ -582,6 +614,89 @@ def gated_scan_step(x, g, state, gate=Gate.SIGMOID, slots=None, new_state=None, 
         return h
 
     return _launch_on(x.device, stream, body)
+
+
+def _vector(t, name, n, like):
+    """Pointer of a vector operand of `like`'s type with n entries (None: null)."""
+    if t is None:
+        return None
+    if t.dtype != like.dtype or t.device != like.device or tuple(t.shape) != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous vector of {n} entries of {like.dtype} on {like.device}")
+    return t.data_ptr()
+
+
+def _optional(t, name, like):
+    return (None, 0) if t is None else _matrix(t, name, like)[::2]
+
+
+def _norm_shape(x, gate, norm, order, activation, eps, scale, name):
+    dtype = _dtype_code(x, name)
+    if activation is None:
+        activation = Activation.NONE if gate is None else Activation.SILU
+    p, rows, stride = _matrix(x, name)
+    return p, stride, FusedNormShape(dtype=dtype, norm=_enum(Norm, norm), order=_enum(NormOrder, order), activation=_enum(Activation, activation), rows=rows, dim=x.shape[-1], eps=eps, scale=scale)
+
+
+def fused_norm(x, weight=None, bias=None, residual=None, gate=None, scale=1.0, channel_scale=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, out=None, residual_out=None, stream=None):
+    """Norm of every row of x (..., dim), fused with a residual, its scale and a gate (tcu_fused_norm); s = scale * channel_scale.
+
+    order "add_norm": z = residual + s x, returns (act(gate) y(z), z), or act(gate) y(x) alone without a residual.
+    order "norm_add": returns residual + s act(gate) y(x).  y is the rms or layer norm times weight plus bias.
+    activation: of the gate, by default silu.  weight, bias, channel_scale: vectors of x's type."""
+    torch = _torch()
+    px, sx, s = _norm_shape(x, gate, norm, order, activation, eps, scale, "x")
+    pr, pg = _optional(residual, "residual", x), _optional(gate, "gate", x)
+    vectors = [_vector(t, n, s.dim, x) for t, n in ((weight, "weight"), (bias, "bias"), (channel_scale, "channel_scale"))]
+    keep = s.order == NormOrder.ADD_NORM and residual is not None
+    if residual_out is not None and not keep:
+        raise ValueError("residual_out goes with the order add_norm and a residual")
+
+    def body(raw):
+        o = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
+        z = None if not keep else torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual_out is None else residual_out
+        _check(lib().tcu_fused_norm(ctypes.byref(s), px, sx, *pr, *pg, *vectors, *_optional(o, "out", x), *_optional(z, "residual_out", x), raw))
+        return (o, z) if keep else o
+
+    return _launch_on(x.device, stream, body)
+
+
+def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, channel_scale=None, x=None, dresidual_out=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, workspace=None,
+                        stream=None):
+    """The gradient of fused_norm (tcu_fused_norm_backward): a dict with "dx" and, where the operand is there, "dgate",
+    "dweight", "dbias", "dscale" (of channel_scale) and "dresidual".
+
+    z: what was normed: the residual_out of the forward call (order add_norm with a residual), else its x.  order add_norm:
+    dresidual_out is the gradient with respect to residual_out and "dresidual" is returned if it is given; the gradient of
+    channel_scale needs the forward call's x.  order norm_add: the residual's gradient is dout itself.  The vectors'
+    gradients are float32."""
+    torch = _torch()
+    pd, sd, s = _norm_shape(dout, gate, norm, order, activation, eps, scale, "dout")
+    add_norm = s.order == NormOrder.ADD_NORM
+    pz, pg = _matrix(z, "z", dout)[::2], _optional(gate, "gate", dout)
+    vectors = [_vector(t, n, s.dim, dout) for t, n in ((weight, "weight"), (bias, "bias"), (channel_scale, "channel_scale"))]
+    ps = _optional(dresidual_out, "dresidual_out", dout)
+    if add_norm and channel_scale is not None and x is None:
+        raise ValueError("the gradient of channel_scale needs x")
+    px = _optional(x if add_norm and channel_scale is not None else None, "x", dout)
+
+    def body(raw):
+        new = lambda: torch.empty(dout.shape, dtype=dout.dtype, device=dout.device)
+        column = lambda: torch.empty(s.dim, dtype=torch.float32, device=dout.device)
+        got = {"dx": new()}
+        if gate is not None:
+            got["dgate"] = new()
+        if dresidual_out is not None:
+            got["dresidual"] = new()
+        for name, t in (("dweight", weight), ("dbias", bias), ("dscale", channel_scale)):
+            if t is not None:
+                got[name] = column()
+        args = (ctypes.byref(s), pd, sd, *pz, *pg, *vectors, *px, *ps, *(v for n in ("dx", "dgate", "dresidual") for v in ((got[n].data_ptr(), s.dim) if n in got else (None, 0))),
+                *(got[n].data_ptr() if n in got else None for n in ("dweight", "dbias", "dscale")))
+        ws, have = _workspace_of(lib().tcu_fused_norm_backward, args, workspace, dout.device)
+        _check(lib().tcu_fused_norm_backward(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        return got
+
+    return _launch_on(dout.device, stream, body)
 
 
 def fill(t, value, stream=None):

@@ -166,4 +166,51 @@ TCU_DEVICE void sigmoid_pair(float x, float *s, float *one_minus) {
   *one_minus = e * *s;
 }
 
+// Activations (tcu_activation) and their slopes.
+constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSigmoid = 4;
+// act(z); the gelu is its tanh form, z (1 + tanh u) / 2 = z sigmoid(2 u) with u = sqrt(2/pi) (z + 0.044715 z^3)
+template <bool EXACT>
+TCU_DEVICE float activation(int act, float z) {
+  constexpr float kTwoA = 1.59576912160573071176f, kB = 0.044715f;  // 2 sqrt(2/pi)
+  if (act == kActNone) return z;
+  if (act == kActRelu) return z < 0.0f ? 0.0f : z;  // a NaN stays one
+  float s, r;
+  sigmoid_pair<EXACT>(act == kActGelu ? kTwoA * z * __builtin_fmaf(kB * z, z, 1.0f) : z, &s, &r);
+  return act == kActSigmoid ? s : z * s;
+}
+// act(z) and act'(z)
+template <bool EXACT>
+TCU_DEVICE void activation_slope(int act, float z, float *value, float *slope) {
+  constexpr float kTwoA = 1.59576912160573071176f, kB = 0.044715f;
+  if (act == kActNone) {
+    *value = z;
+    *slope = 1.0f;
+    return;
+  }
+  if (act == kActRelu) {
+    *value = z < 0.0f ? 0.0f : z;
+    *slope = z > 0.0f ? 1.0f : 0.0f;
+    return;
+  }
+  float s, r;  // sigmoid of the argument and 1 - sigmoid
+  sigmoid_pair<EXACT>(act == kActGelu ? kTwoA * z * __builtin_fmaf(kB * z, z, 1.0f) : z, &s, &r);
+  if (act == kActSigmoid) {
+    *value = s;
+    *slope = s * r;
+  } else {  // z s(v): s + z s (1 - s) v'
+    *value = z * s;
+    const float dv = act == kActGelu ? kTwoA * __builtin_fmaf(3.0f * kB * z, z, 1.0f) : 1.0f;
+    *slope = __builtin_fmaf(z * dv * r, s, s);
+  }
+}
+
+// sum of x over the wave, in every lane (a fixed order)
+TCU_DEVICE float wave_sum(float x) {
+  x += dpp<DPP_QUAD_XOR1>(x, x);
+  x += dpp<DPP_QUAD_XOR2>(x, x);
+  x += dpp<DPP_ROW_HALF_MIRROR>(x, x);
+  x += dpp<DPP_ROW_MIRROR>(x, x);
+  return add_xor32(add_xor16(x));
+}
+
 }  // namespace tcu

@@ -1,0 +1,332 @@
+// Norm of every row fused with the residual addition, the scale of the residual branch and a gate:
+//
+//   add_norm:  z = residual + s x (z = x without a residual),  out = act(gate) y(z),  z is written too (the residual stream)
+//   norm_add:  out = residual + s act(gate) y(x)
+//   y(z) = n weight + bias,  n = (z - mean) rho;  rms: mean = 0, rho = 1 / sqrt(mean z^2 + eps);
+//   layer: mean of the row, rho = 1 / sqrt(mean (z - mean)^2 + eps);  s = scale * channel_scale, one number per channel.
+//
+// Gradient, with d the gradient with respect to act(gate) y (norm_add: s dout; add_norm: dout):
+//   dy = d act(gate),  dgate = d y act'(gate),  dweight = sum dy n,  dbias = sum dy  (sums over rows)
+//   dn = dy weight,  dz = rho (dn - n mean(dn n) - [layer] mean(dn))
+//   norm_add: dx = dz, dchannel_scale = scale sum dout act(gate) y
+//   add_norm: dz += dstream (the gradient of the written z), dresidual = dz, dx = s dz, dchannel_scale = scale sum dz x
+//
+// Bound by HBM traffic: every operand is read once and every result written once.  A row lives in the registers of the
+// WAVES waves that share it (CHUNKS 16-byte chunks per lane), so the statistics take no second read; the variance is that of
+// the centred values (two sums one after the other), which a difference of sums would lose the digits of.  The gradients
+// of the vectors are sums over rows: a block walks many rows with its columns' sums in registers, writes them once as
+// partial sums, and a second launch adds the partial sums of each column in a fixed order (no atomics: the same input
+// gives the same bits).
+#pragma once
+
+#include "elements.hpp"
+
+namespace tcu {
+
+constexpr int kNormRms = 0, kNormLayer = 1;      // tcu_norm
+constexpr int kOrderAddNorm = 0, kOrderNormAdd = 1;  // tcu_norm_order
+
+struct FusedNormParams {
+  const void *x, *residual, *gate, *weight, *bias, *channel_scale;  // all but x may be null
+  void *out, *z_out;                                                // z_out may be null
+  size_t x_stride, residual_stride, gate_stride, out_stride, z_out_stride;
+  size_t rows;
+  unsigned dim;
+  float eps, scale;
+  int norm, order, act;
+};
+
+// sums over the WAVES waves that share a row, in every lane; `lds` has 4 * WAVES floats per parity, and consecutive
+// calls alternate the parity, so one barrier a call is enough
+template <int WAVES, int N>
+TCU_DEVICE void row_sums(float (&v)[N], float *lds, int wave, int parity) {
+#pragma unroll
+  for (int i = 0; i < N; i++) v[i] = wave_sum(v[i]);
+  if constexpr (WAVES > 1) {
+    float *slot = lds + parity * (4 * WAVES);
+    if (lane_id() == 0) {
+#pragma unroll
+      for (int i = 0; i < N; i++) slot[i * WAVES + wave] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; w++) s += slot[i * WAVES + w];
+      v[i] = s;
+    }
+  }
+}
+
+// V values of a vector operand of the row (null: `missing` everywhere)
+template <int DT, bool ALIGNED>
+TCU_DEVICE void load_vector(const void *p, unsigned at, int count, float missing, float (&v)[Elem<DT>::V]) {
+  if (p) {
+    unpack_chunk<DT>(load_chunk_of<DT, ALIGNED, false>(p, at, count), v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < Elem<DT>::V; e++) v[e] = missing;
+  }
+}
+
+// WAVES waves share a row; a block has BLOCK_WAVES waves, i.e. BLOCK_WAVES / WAVES rows.
+template <int DT, bool ALIGNED, int WAVES, int CHUNKS, int BLOCK_WAVES>
+__global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_kernel(FusedNormParams p) {
+  constexpr int V = Elem<DT>::V;
+  constexpr bool EXACT = DT == kF32;
+  __shared__ float lds[WAVES > 1 ? 8 * WAVES : 1];
+  static_assert(WAVES == 1 || WAVES == BLOCK_WAVES, "rows that share a block share no sums");
+  const int wave = wave_in_block();
+  const size_t row = WAVES == 1 ? (size_t)blockIdx.x * BLOCK_WAVES + wave : blockIdx.x;
+  if (row >= p.rows) return;  // a whole wave, of rows that need no barrier
+  const int lane = WAVES == 1 ? lane_id() : (int)threadIdx.x;
+  auto column = [&](int k) { return (unsigned)(k * 64 * WAVES + lane) * V; };
+  auto exists = [&](int k) { return (int)p.dim - (int)column(k); };
+
+  const bool add_first = p.order == kOrderAddNorm && p.residual != nullptr;
+  float z[CHUNKS][V];
+  uint4_t cr[CHUNKS], cg[CHUNKS];
+#pragma unroll
+  for (int k = 0; k < CHUNKS; k++) {
+    unpack_chunk<DT>(load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + column(k), exists(k)), z[k]);
+    if (p.residual) cr[k] = load_chunk_of<DT, ALIGNED>(p.residual, row * p.residual_stride + column(k), exists(k));
+    if (p.gate) cg[k] = load_chunk_of<DT, ALIGNED>(p.gate, row * p.gate_stride + column(k), exists(k));
+  }
+  if (add_first) {
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+      float s[V], r[V];
+      load_vector<DT, ALIGNED>(p.channel_scale, column(k), exists(k), 1.0f, s);
+      unpack_chunk<DT>(cr[k], r);
+#pragma unroll
+      for (int e = 0; e < V; e++) z[k][e] = __builtin_fmaf(p.scale * s[e], z[k][e], r[e]);
+      if (p.z_out) store_chunk_of<DT, ALIGNED>(p.z_out, row * p.z_out_stride + column(k), exists(k), z[k]);
+    }
+  }
+  const float inv = 1.0f / (float)p.dim;
+  float mean = 0.0f, sum[1];
+  if (p.norm == kNormLayer) {
+    sum[0] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++)
+#pragma unroll
+      for (int e = 0; e < V; e++) sum[0] += z[k][e];  // columns beyond the row hold 0
+    row_sums<WAVES>(sum, lds, wave, 0);
+    mean = sum[0] * inv;
+  }
+  sum[0] = 0.0f;
+#pragma unroll
+  for (int k = 0; k < CHUNKS; k++)
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      z[k][e] -= mean;
+      if (e < exists(k)) sum[0] = __builtin_fmaf(z[k][e], z[k][e], sum[0]);
+    }
+  row_sums<WAVES>(sum, lds, wave, 1);
+  const float rho = hw_rsqrt(__builtin_fmaf(sum[0], inv, p.eps));
+#pragma unroll
+  for (int k = 0; k < CHUNKS; k++) {
+    float w[V], b[V], y[V];
+    load_vector<DT, ALIGNED>(p.weight, column(k), exists(k), 1.0f, w);
+    load_vector<DT, ALIGNED>(p.bias, column(k), exists(k), 0.0f, b);
+#pragma unroll
+    for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(z[k][e] * rho, w[e], b[e]);
+    if (p.gate) {
+      float g[V];
+      unpack_chunk<DT>(cg[k], g);
+#pragma unroll
+      for (int e = 0; e < V; e++) y[e] *= activation<EXACT>(p.act, g[e]);
+    }
+    if (p.order == kOrderNormAdd) {
+      float s[V], r[V];
+      load_vector<DT, ALIGNED>(p.channel_scale, column(k), exists(k), 1.0f, s);
+#pragma unroll
+      for (int e = 0; e < V; e++) r[e] = 0.0f;
+      if (p.residual) unpack_chunk<DT>(cr[k], r);
+#pragma unroll
+      for (int e = 0; e < V; e++) y[e] = __builtin_fmaf(p.scale * s[e], y[e], r[e]);
+    }
+    store_chunk_of<DT, ALIGNED>(p.out, row * p.out_stride + column(k), exists(k), y);
+  }
+}
+
+struct FusedNormBackParams {
+  const void *dout, *z, *gate, *weight, *bias, *channel_scale, *x, *dstream;  // all but dout and z may be null
+  void *dx, *dgate, *dresidual;                                              // all but dx may be null
+  size_t dout_stride, z_stride, gate_stride, x_stride, dstream_stride, dx_stride, dgate_stride, dresidual_stride;
+  float *partial;  // [part][vector][dim]: dweight, dbias, dchannel_scale, those that are asked for
+  size_t rows;
+  unsigned dim;
+  float eps, scale;
+  int norm, order, act;
+  bool want_weight, want_bias, want_scale;
+};
+
+template <int DT, bool ALIGNED, int WAVES, int CHUNKS, int BLOCK_WAVES>
+__global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_backward_kernel(FusedNormBackParams p) {
+  constexpr int V = Elem<DT>::V;
+  constexpr bool EXACT = DT == kF32;
+  __shared__ float lds[WAVES > 1 ? 8 * WAVES : 1];
+  static_assert(WAVES == 1 || WAVES == BLOCK_WAVES, "rows that share a block share no sums");
+  const int wave = wave_in_block();
+  const size_t part = WAVES == 1 ? (size_t)blockIdx.x * BLOCK_WAVES + wave : blockIdx.x;
+  const size_t parts = WAVES == 1 ? (size_t)gridDim.x * BLOCK_WAVES : gridDim.x;
+  const int lane = WAVES == 1 ? lane_id() : (int)threadIdx.x;
+  auto column = [&](int k) { return (unsigned)(k * 64 * WAVES + lane) * V; };
+  auto exists = [&](int k) { return (int)p.dim - (int)column(k); };
+  const bool add_norm = p.order == kOrderAddNorm;
+  const float inv = 1.0f / (float)p.dim;
+
+  float sw[CHUNKS][V], sb[CHUNKS][V], ss[CHUNKS][V];  // column sums of dweight, dbias, dchannel_scale
+#pragma unroll
+  for (int k = 0; k < CHUNKS; k++)
+#pragma unroll
+    for (int e = 0; e < V; e++) sw[k][e] = sb[k][e] = ss[k][e] = 0.0f;
+
+  int parity = 0;
+  for (size_t row = part; row < p.rows; row += parts) {
+    float z[CHUNKS][V], d[CHUNKS][V];  // z, centred; dout, then dy
+    uint4_t cg[CHUNKS], cs[CHUNKS], cx[CHUNKS];
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+      unpack_chunk<DT>(load_chunk_of<DT, ALIGNED>(p.z, row * p.z_stride + column(k), exists(k)), z[k]);
+      unpack_chunk<DT>(load_chunk_of<DT, ALIGNED>(p.dout, row * p.dout_stride + column(k), exists(k)), d[k]);
+      if (p.gate) cg[k] = load_chunk_of<DT, ALIGNED>(p.gate, row * p.gate_stride + column(k), exists(k));
+      if (p.dstream) cs[k] = load_chunk_of<DT, ALIGNED>(p.dstream, row * p.dstream_stride + column(k), exists(k));
+      if (p.want_scale && add_norm) cx[k] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + column(k), exists(k));
+    }
+    float mean = 0.0f;
+    if (p.norm == kNormLayer) {
+      float s[1] = {0.0f};
+#pragma unroll
+      for (int k = 0; k < CHUNKS; k++)
+#pragma unroll
+        for (int e = 0; e < V; e++) s[0] += z[k][e];
+      row_sums<WAVES>(s, lds, wave, parity);
+      parity ^= 1;
+      mean = s[0] * inv;
+    }
+    // sums of z^2, dn z and dn over the row (z centred); columns beyond the row have d = 0
+    float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+      float w[V], f[V], c[V];
+      load_vector<DT, ALIGNED>(p.weight, column(k), exists(k), 1.0f, w);
+#pragma unroll
+      for (int e = 0; e < V; e++) f[e] = 1.0f;
+      if (p.gate) {
+        float g[V];
+        unpack_chunk<DT>(cg[k], g);
+#pragma unroll
+        for (int e = 0; e < V; e++) f[e] = activation<EXACT>(p.act, g[e]);
+      }
+      if (!add_norm) {
+        load_vector<DT, ALIGNED>(p.channel_scale, column(k), exists(k), 1.0f, c);
+#pragma unroll
+        for (int e = 0; e < V; e++) f[e] *= p.scale * c[e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        z[k][e] -= mean;
+        if (e < exists(k)) {
+          const float dn = d[k][e] * f[e] * w[e];
+          s[0] = __builtin_fmaf(z[k][e], z[k][e], s[0]);
+          s[1] = __builtin_fmaf(dn, z[k][e], s[1]);
+          s[2] += dn;
+        }
+      }
+    }
+    row_sums<WAVES>(s, lds, wave, parity);
+    parity ^= 1;
+    const float rho = hw_rsqrt(__builtin_fmaf(s[0], inv, p.eps));
+    const float mean_dnn = s[1] * rho * inv, mean_dn = p.norm == kNormLayer ? s[2] * inv : 0.0f;
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+      float w[V], b[V], c[V], dx[V], dg[V];
+      load_vector<DT, ALIGNED>(p.weight, column(k), exists(k), 1.0f, w);
+      load_vector<DT, ALIGNED>(p.bias, column(k), exists(k), 0.0f, b);
+      load_vector<DT, ALIGNED>(p.channel_scale, column(k), exists(k), 1.0f, c);
+      float g[V], extra[V], x[V];
+#pragma unroll
+      for (int e = 0; e < V; e++) g[e] = extra[e] = x[e] = 0.0f;
+      if (p.gate) unpack_chunk<DT>(cg[k], g);
+      if (p.dstream) unpack_chunk<DT>(cs[k], extra);
+      if (p.want_scale && add_norm) unpack_chunk<DT>(cx[k], x);
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float n = z[k][e] * rho, y = __builtin_fmaf(n, w[e], b[e]), sc = p.scale * c[e];
+        float f = 1.0f, slope = 0.0f;
+        if (p.gate) activation_slope<EXACT>(p.act, g[e], &f, &slope);
+        const float up = add_norm ? d[k][e] : sc * d[k][e];  // gradient with respect to act(gate) y
+        const float dy = up * f;
+        dg[e] = up * y * slope;
+        sw[k][e] = __builtin_fmaf(dy, n, sw[k][e]);
+        sb[k][e] += dy;
+        if (!add_norm) ss[k][e] = __builtin_fmaf(d[k][e], f * y, ss[k][e]);
+        float dz = rho * (__builtin_fmaf(-n, mean_dnn, dy * w[e]) - mean_dn);
+        if (add_norm) {
+          dz += extra[e];
+          ss[k][e] = __builtin_fmaf(dz, x[e], ss[k][e]);
+        }
+        dx[e] = dz;
+      }
+      if (p.dresidual) store_chunk_of<DT, ALIGNED>(p.dresidual, row * p.dresidual_stride + column(k), exists(k), dx);
+      if (add_norm) {
+#pragma unroll
+        for (int e = 0; e < V; e++) dx[e] *= p.scale * c[e];
+      }
+      store_chunk_of<DT, ALIGNED>(p.dx, row * p.dx_stride + column(k), exists(k), dx);
+      if (p.dgate) store_chunk_of<DT, ALIGNED>(p.dgate, row * p.dgate_stride + column(k), exists(k), dg);
+    }
+  }
+  const int vectors = (int)p.want_weight + (int)p.want_bias + (int)p.want_scale;
+  float *to = p.partial + part * vectors * p.dim;
+#pragma unroll
+  for (int k = 0; k < CHUNKS; k++) {
+    float *q = to;
+#pragma unroll
+    for (int e = 0; e < V; e++) ss[k][e] *= p.scale;
+    if (p.want_weight) {
+      store_floats<V, ALIGNED>(q, column(k), exists(k), sw[k]);
+      q += p.dim;
+    }
+    if (p.want_bias) {
+      store_floats<V, ALIGNED>(q, column(k), exists(k), sb[k]);
+      q += p.dim;
+    }
+    if (p.want_scale) store_floats<V, ALIGNED>(q, column(k), exists(k), ss[k]);
+  }
+}
+
+// out[v][c] = sum over parts of partial[part][v][c], in a fixed order: 64 columns per block, the parts dealt to its waves
+struct ColumnSumParams {
+  const float *partial;
+  float *out[3];
+  size_t parts;
+  unsigned columns, vectors;  // columns of one vector
+};
+constexpr int kColumnSumWaves = 8;
+__global__ __launch_bounds__(64 * kColumnSumWaves) inline void column_sum_kernel(ColumnSumParams p) {
+  __shared__ float lds[kColumnSumWaves * 64];
+  const size_t width = (size_t)p.columns * p.vectors, at = (size_t)blockIdx.x * 64 + lane_id();
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (at < width) {
+    size_t i = wave_in_block();
+    for (; i + 3 * kColumnSumWaves < p.parts; i += 4 * kColumnSumWaves) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) s[u] += p.partial[(i + u * kColumnSumWaves) * width + at];
+    }
+    for (; i < p.parts; i += kColumnSumWaves) s[0] += p.partial[i * width + at];
+  }
+  lds[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+  __syncthreads();
+  if (threadIdx.x < 64 && at < width) {
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kColumnSumWaves; w++) t += lds[w * 64 + threadIdx.x];
+    p.out[at / p.columns][at % p.columns] = t;
+  }
+}
+
+}  // namespace tcu

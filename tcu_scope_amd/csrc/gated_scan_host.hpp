@@ -1,15 +1,11 @@
 // Argument checks, workspace layout and kernel selection of the gated scan's entry points.
 #pragma once
 
+#include "checks.hpp"
 #include "gated_scan.hpp"
-#include "host_support.hpp"
 #include "launch.hpp"
 
 namespace tcu {
-
-inline bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-inline size_t element_bytes(int dtype) { return dtype == TCU_F32 ? 4 : 2; }
-inline bool known_dtype(int dtype) { return dtype == TCU_F16 || dtype == TCU_BF16 || dtype == TCU_F32; }
 
 // Tiles: 16 lanes (256 bytes of a row) x 16 groups.  Places per thread: the (a, b) of every place stay in registers.
 constexpr int kScanLanes = 16, kScanThreads = 256, kScanPlaces = 8, kScanBackPlaces = 4;
@@ -48,24 +44,6 @@ inline int plan_gated_scan(const char *what, const tcu_gated_scan_shape *s, unsi
   plan->desc_at = plan->rows_at + (s->d_offsets ? (plan->rows * 4 + 255) / 256 * 256 : 0);
   plan->desc_bytes = plan->chained ? plan->strips * plan->chunks * tc * 16 : 0;
   plan->bytes = plan->desc_at + plan->desc_bytes;
-  return TCU_OK;
-}
-
-// a matrix of `rows` x channels whose rows are `stride` elements apart
-inline int check_matrix(const std::string &w, const char *name, const void *p, size_t stride, const tcu_gated_scan_shape *s, size_t rows, bool *whole_chunks) {
-  if (!p) return report_failure(TCU_ERR_INVALID_ARG, w + ": " + name + " is null");
-  if (rows > 1 && stride < s->channels) return report_failure(TCU_ERR_INVALID_ARG, w + ": the rows of " + name + " overlap (stride below channels)");
-  size_t elements = 0;
-  if (rows && !product_fits(stride, rows - 1, &elements)) return report_failure(TCU_ERR_INVALID_ARG, w + ": " + name + ": stride * rows overflows");
-  const size_t e = element_bytes(s->dtype);
-  if (elements > (~(size_t)0) / e - s->channels) return report_failure(TCU_ERR_INVALID_ARG, w + ": " + name + ": stride * rows overflows");
-  if (!aligned_to(p, e)) return report_failure(TCU_ERR_INVALID_ARG, w + ": " + name + " is not aligned to its elements");
-  if (!aligned_to(p, 16) || (rows > 1 && stride * e % 16 != 0)) *whole_chunks = false;
-  return TCU_OK;
-}
-inline int check_states(const std::string &w, const char *name, const void *p, bool *whole_chunks) {
-  if (p && !aligned_to(p, 4)) return report_failure(TCU_ERR_INVALID_ARG, w + ": " + name + " is not aligned to floats");
-  if (p && !aligned_to(p, 16)) *whole_chunks = false;
   return TCU_OK;
 }
 
@@ -126,12 +104,6 @@ inline int run_gated_scan(const tcu_gated_scan_shape *s, const GatedScanPlan &pl
   return TCU_OK;
 }
 
-inline int check_workspace(const std::string &w, const void *workspace, size_t have, size_t need) {
-  if (have < need) return report_failure(TCU_ERR_WORKSPACE, w + ": workspace of " + std::to_string(have) + " bytes, needs " + std::to_string(need));
-  if (!aligned_to(workspace, 256)) return report_failure(TCU_ERR_INVALID_ARG, w + ": the workspace must be 256-byte aligned");
-  return TCU_OK;
-}
-
 inline int gated_scan_dispatch(const tcu_gated_scan_shape *s, const void *x, size_t x_stride, const void *g, size_t g_stride, void *h, size_t h_stride, const void *h0, void *h_last, void *workspace,
                                size_t *workspace_bytes, void *stream) {
   const char *what = "tcu_gated_scan";
@@ -146,12 +118,12 @@ inline int gated_scan_dispatch(const tcu_gated_scan_shape *s, const void *x, siz
   if (int rc = check_workspace(w, workspace, *workspace_bytes, plan.bytes)) return rc;
   bool aligned = s->channels % (16 / element_bytes(s->dtype)) == 0;
   if (plan.rows) {
-    if (int rc = check_matrix(w, "d_x", x, x_stride, s, plan.rows, &aligned)) return rc;
-    if (int rc = check_matrix(w, "d_g", g, g_stride, s, plan.rows, &aligned)) return rc;
-    if (int rc = check_matrix(w, "d_h", h, h_stride, s, plan.rows, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_x", x, x_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_g", g, g_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_h", h, h_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
   }
-  if (int rc = check_states(w, "d_h0", h0, &aligned)) return rc;
-  if (int rc = check_states(w, "d_h_last", h_last, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_h0", h0, 4, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_h_last", h_last, 4, &aligned)) return rc;
   if (s->num_sequences == 0) return TCU_OK;
   GatedScanParams p{};
   p.x = x;
@@ -179,19 +151,19 @@ inline int gated_scan_backward_dispatch(const tcu_gated_scan_shape *s, const voi
   if (int rc = check_workspace(w, workspace, *workspace_bytes, plan.bytes)) return rc;
   bool aligned = s->channels % (16 / element_bytes(s->dtype)) == 0;
   if (plan.rows) {
-    if (int rc = check_matrix(w, "d_dh", dh, dh_stride, s, plan.rows, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_dh", dh, dh_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
     if (s->gate == TCU_GATE_SIGMOID)
-      if (int rc = check_matrix(w, "d_x", x, x_stride, s, plan.rows, &aligned)) return rc;
-    if (int rc = check_matrix(w, "d_g", g, g_stride, s, plan.rows, &aligned)) return rc;
-    if (int rc = check_matrix(w, "d_h", h, h_stride, s, plan.rows, &aligned)) return rc;
-    if (int rc = check_matrix(w, "d_dx", dx, dx_stride, s, plan.rows, &aligned)) return rc;
-    if (int rc = check_matrix(w, "d_dg", dg, dg_stride, s, plan.rows, &aligned)) return rc;
+      if (int rc = check_matrix(w, "d_x", x, x_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_g", g, g_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_h", h, h_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_dx", dx, dx_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
+    if (int rc = check_matrix(w, "d_dg", dg, dg_stride, plan.rows, s->channels, s->dtype, &aligned)) return rc;
     if (dx == h || dg == h) return report_failure(TCU_ERR_INVALID_ARG, w + ": a gradient must not take the place of d_h (other tiles still read it)");
     if (dx == dg) return report_failure(TCU_ERR_INVALID_ARG, w + ": d_dx and d_dg are the same buffer");
   }
-  if (int rc = check_states(w, "d_h0", h0, &aligned)) return rc;
-  if (int rc = check_states(w, "d_dh_last", dh_last, &aligned)) return rc;
-  if (int rc = check_states(w, "d_dh0", dh0, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_h0", h0, 4, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_dh_last", dh_last, 4, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_dh0", dh0, 4, &aligned)) return rc;
   if (s->num_sequences == 0) return TCU_OK;
   GatedScanParams p{};
   p.dh = dh;
@@ -229,12 +201,12 @@ inline int gated_scan_step_dispatch(int dtype, int gate, size_t channels, size_t
   if (!slots && num_slots < rows) return report_failure(TCU_ERR_INVALID_ARG, w + ": fewer slots than rows, and no d_slots to say which");
   if (slots && !aligned_to(slots, 4)) return report_failure(TCU_ERR_INVALID_ARG, w + ": d_slots is not aligned to its integers");
   bool aligned = channels % (16 / element_bytes(dtype)) == 0;
-  if (int rc = check_matrix(w, "d_x", x, x_stride, &s, rows, &aligned)) return rc;
-  if (int rc = check_matrix(w, "d_g", g, g_stride, &s, rows, &aligned)) return rc;
-  if (int rc = check_matrix(w, "d_h", h, h_stride, &s, rows, &aligned)) return rc;
+  if (int rc = check_matrix(w, "d_x", x, x_stride, rows, channels, dtype, &aligned)) return rc;
+  if (int rc = check_matrix(w, "d_g", g, g_stride, rows, channels, dtype, &aligned)) return rc;
+  if (int rc = check_matrix(w, "d_h", h, h_stride, rows, channels, dtype, &aligned)) return rc;
   if (!state || !new_state) return report_failure(TCU_ERR_INVALID_ARG, w + ": d_state or d_new_state is null");
-  if (int rc = check_states(w, "d_state", state, &aligned)) return rc;
-  if (int rc = check_states(w, "d_new_state", new_state, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_state", state, 4, &aligned)) return rc;
+  if (int rc = check_vector(w, "d_new_state", new_state, 4, &aligned)) return rc;
   GatedStepParams p{};
   p.x = x;
   p.g = g;

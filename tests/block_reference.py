@@ -111,3 +111,90 @@ def check(got, want, err, dtype, what):
     if bad.any():
         k = int(np.argmax(np.where(bad, off / np.maximum(may, 1e-300), 0)))
         raise AssertionError(f"{what}: {bad.sum()} of {bad.size} outside the bound, worst {got[fine][k]} for {want[fine][k]}, {off[k]:.3g} off where {may[k]:.3g} is allowed")
+
+
+# ---- activations and norms --------------------------------------------------------------------------------------
+
+GELU_A, GELU_B = np.sqrt(2.0 / np.pi), 0.044715
+
+
+def act(name, z):
+    """act(z), act'(z), and how many roundings relative to |act(z)| (+ |z| |act'| for the slope) their fp32 forms carry: the
+    sigmoid's |argument| + 6 (gate_terms), the argument of gelu 4 more that the exponential turns into 4 |argument|, and the products."""
+    one = np.ones_like(z)
+    with np.errstate(over="ignore", invalid="ignore"):
+        if name == "none":
+            return z, one, 0.0 * one
+        if name == "relu":
+            return np.where(z < 0, 0.0, z), (z > 0).astype(np.float64), 0.0 * one
+        v = 2 * GELU_A * (z + GELU_B * z ** 3) if name == "gelu" else z
+        s, r = sigmoid(v), sigmoid(-v)
+        c = np.minimum(np.abs(v), 128) * (5.0 if name == "gelu" else 1.0) + 10.0
+        if name == "sigmoid":
+            return s, s * r, c
+        dv = 2 * GELU_A * (1 + 3 * GELU_B * z ** 2) if name == "gelu" else one
+        return z * s, s + z * s * r * dv, c
+
+
+def _stats(kind, z, ez, eps):
+    """centred rows, 1 / sigma, and their bounds.  A sum over a row adds along chains of at most 64 + 24 values."""
+    chain = 100.0 * EPS32
+    mean = z.mean(-1, keepdims=True) if kind == "layer" else 0.0
+    c = z - mean
+    ec = ez + (chain * np.abs(z).mean(-1, keepdims=True) + ez.mean(-1, keepdims=True) + EPS32 * np.abs(c) if kind == "layer" else 0.0)
+    var = (c * c).mean(-1, keepdims=True)
+    rho = 1.0 / np.sqrt(var + eps)
+    rel = 0.5 * ((chain * var + 2 * (np.abs(c) * ec).mean(-1, keepdims=True)) / (var + eps) + 2 * EPS32) + 4 * EPS32
+    return c, ec, rho, rel
+
+
+def norm(kind, order, name, x, residual, gate, weight, bias, scale, eps):
+    """(out, z, bound on out, on z); scale: the vector s."""
+    add = order == "add_norm" and residual is not None
+    z = residual + scale * x if add else x
+    ez = 3 * EPS32 * (np.abs(residual) + np.abs(scale * x)) if add else np.zeros_like(x)
+    c, ec, rho, rel = _stats(kind, z, ez, eps)
+    y = c * rho * weight + bias
+    ey = np.abs(weight) * rho * (ec + np.abs(c) * (rel + 2 * EPS32)) + 2 * EPS32 * (np.abs(c * rho * weight) + np.abs(bias))
+    f, _, cf = act(name, gate) if gate is not None else (np.ones_like(x), None, np.zeros_like(x))
+    u, eu = y * f, ey * np.abs(f) + (cf + 1) * EPS32 * np.abs(y * f)
+    if order == "norm_add":
+        base = residual if residual is not None else np.zeros_like(x)
+        return base + scale * u, z, np.abs(scale) * eu + 3 * EPS32 * (np.abs(scale * u) + np.abs(base)), ez
+    return u, z, eu, ez
+
+
+def norm_backward(kind, order, name, dout, z, gate, weight, bias, scale, eps, x, dstream):
+    """dict of gradients (dscale with respect to the vector s) and dict of bounds."""
+    c, ec, rho, rel = _stats(kind, z, np.zeros_like(z), eps)
+    n, en = c * rho, rho * ec + np.abs(c * rho) * (rel + EPS32)
+    y, ey = n * weight + bias, np.abs(weight) * en + 2 * EPS32 * (np.abs(n * weight) + np.abs(bias))
+    f, slope, cf = act(name, gate) if gate is not None else (np.ones_like(z), np.zeros_like(z), np.zeros_like(z))
+    mag = np.abs(f) + np.abs(gate) if gate is not None else np.abs(f)  # terms of the slope: s and z s (1 - s) v', each below this
+    up = scale * dout if order == "norm_add" else dout
+    dy, edy = up * f, (cf + 3) * EPS32 * np.abs(up * f)
+    dn, edn = dy * weight, (cf + 4) * EPS32 * np.abs(dy * weight)
+    mean = lambda v: v.mean(-1, keepdims=True)
+    m1, em1 = mean(dn * n), 104 * EPS32 * mean(np.abs(dn * n)) + mean(np.abs(dn) * en + edn * np.abs(n)) + rel * np.abs(mean(dn * n))
+    m2, em2 = (mean(dn), 104 * EPS32 * mean(np.abs(dn)) + mean(edn)) if kind == "layer" else (0.0, 0.0)
+    inner = dn - n * m1 - m2
+    einner = edn + en * np.abs(m1) + np.abs(n) * em1 + em2 + 4 * EPS32 * (np.abs(dn) + np.abs(n * m1) + np.abs(m2))
+    dz, edz = rho * inner, rho * einner + (rel + EPS32) * rho * (np.abs(dn) + np.abs(n * m1) + np.abs(m2))
+    got, err = {}, {}
+    # a column's sum: the rows of one block in a chain, then the blocks' partial sums
+    rows = z.shape[0]
+    column = lambda t, e: (t.sum(0), (rows / 512 + 100) * EPS32 * np.abs(t).sum(0) + e.sum(0))
+    got["dgate"], err["dgate"] = up * y * slope, np.abs(up) * (ey * np.abs(slope) + (3 * cf + 8) * EPS32 * np.abs(y) * mag)
+    got["dweight"], err["dweight"] = column(dy * n, edy * np.abs(n) + np.abs(dy) * en + EPS32 * np.abs(dy * n))
+    got["dbias"], err["dbias"] = column(dy, edy)
+    if order == "norm_add":
+        got["dscale"], err["dscale"] = column(dout * f * y, np.abs(dout) * (np.abs(f) * ey + (cf + 3) * EPS32 * np.abs(f * y)))
+    else:
+        extra = dstream if dstream is not None else 0.0
+        dz, edz = dz + extra, edz + 2 * EPS32 * (np.abs(dz) + np.abs(extra))
+        got["dresidual"], err["dresidual"] = dz, edz
+        if x is not None:
+            got["dscale"], err["dscale"] = column(dz * x, np.abs(x) * edz + EPS32 * np.abs(dz * x))
+        dz, edz = scale * dz, np.abs(scale) * (edz + 2 * EPS32 * np.abs(dz))
+    got["dx"], err["dx"] = dz, edz
+    return got, err

@@ -34,3 +34,15 @@ int emu_gated_scan_step(int dtype, int gate, size_t channels, size_t rows, const
   return tcu::gated_scan_step_dispatch(dtype, gate, channels, rows, x, xs, g, gs, h, hs, state, new_state, num_slots, slots, zero_padding, nullptr);
 }
 }
+#include "../../tcu_scope_amd/csrc/fused_norm_host.hpp"
+
+extern "C" {
+int emu_fused_norm(const tcu_fused_norm_shape *s, const void *x, size_t xs, const void *res, size_t rs, const void *gate, size_t gs, const void *w, const void *b, const void *cs, void *out, size_t os, void *zo,
+                   size_t zs) {
+  return tcu::fused_norm_dispatch(s, x, xs, res, rs, gate, gs, w, b, cs, out, os, zo, zs, nullptr);
+}
+int emu_fused_norm_backward(const tcu_fused_norm_shape *s, const void *dout, size_t dos, const void *z, size_t zs, const void *gate, size_t gs, const void *w, const void *b, const void *cs, const void *x,
+                            size_t xs, const void *dro, size_t dros, void *dx, size_t dxs, void *dg, size_t dgs, void *dr, size_t drs, float *dw, float *db, float *dcs, void *ws, size_t *wb) {
+  return tcu::fused_norm_backward_dispatch(s, dout, dos, z, zs, gate, gs, w, b, cs, x, xs, dro, dros, dx, dxs, dg, dgs, dr, drs, dw, db, dcs, ws, wb, nullptr);
+}
+}

@@ -352,3 +352,187 @@ def test_gated_scan_refusals(emu):
     assert step(state=None) == 1 and "d_state" in err()
     assert step(dtype=7) == 1 and "dtype" in err()
     assert step(rows=0) == 0
+
+
+# ---- fused norm -------------------------------------------------------------------------------------------------
+
+
+class NormShape(ctypes.Structure):
+    _fields_ = [("dtype", ci), ("norm", ci), ("order", ci), ("activation", ci), ("rows", sz), ("dim", sz), ("eps", cf), ("scale", cf)]
+
+
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "sigmoid": 4}
+NULL = (None, 0)
+EPS = float(np.float32(1e-5))
+
+
+def norm_emu(emu):
+    shape, psz, m = ctypes.POINTER(NormShape), ctypes.POINTER(sz), [vp, sz]
+    emu.emu_fused_norm.argtypes = [shape, *m * 3, vp, vp, vp, *m * 2]
+    emu.emu_fused_norm_backward.argtypes = [shape, *m * 3, vp, vp, vp, *m * 5, vp, vp, vp, vp, psz]
+    return emu
+
+
+def vector(values, dtype):
+    a = aligned(values.size, storage(dtype))
+    a[:] = ref.to_bits(values, dtype)
+    return a
+
+
+def operand(m):
+    return (m.ptr, m.stride) if m is not None else NULL
+
+
+# rows, dim, stride - dim, shift, norm, order, activation of the gate (None: no gate), residual, weight, bias, channel scale, scale
+NORMS = [
+    (1, 1, 0, 0, "rms", "add_norm", None, False, True, False, False, 1.0),
+    (3, 8, 0, 0, "layer", "add_norm", "silu", True, True, True, True, 0.5),
+    (5, 100, 3, 1, "rms", "norm_add", "silu", True, True, False, True, 1.5),
+    (2, 520, 8, 0, "layer", "norm_add", "sigmoid", False, True, True, False, 1.0),
+    (4, 1032, 0, 8, "rms", "add_norm", "gelu", True, False, False, False, 1.0),
+    (2, 2056, 0, 0, "layer", "add_norm", None, True, True, True, True, 1.0),
+    (3, 2049, 0, 0, "rms", "norm_add", "relu", True, True, True, True, 1.0),
+    (2, 4104, 0, 0, "rms", "norm_add", None, True, True, False, False, 0.25),
+    (1, 8200, 0, 0, "layer", "norm_add", "silu", True, True, True, True, 1.0),
+    (1, 20000, 0, 0, "rms", "add_norm", "silu", True, True, False, True, 1.0),
+]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("case", NORMS, ids=lambda c: f"{c[0]}x{c[1]}-{c[4]}-{c[5]}-{c[6]}")
+def test_fused_norm_and_gradient(emu, dtype, case):
+    rows, dim, gap, shift, kind, order, actn, with_res, with_w, with_b, with_cs, scale = case
+    emu = norm_emu(emu)
+    rng = np.random.default_rng(dim)
+    f = lambda v: ref.to_f64(ref.to_bits(v, dtype), dtype)
+    mat = lambda mean=0.0, s=1.0: f(rng.standard_normal((rows, dim)) * s + mean)
+    x, res, gate = mat(0.3), mat(0.1, 2.0) if with_res else None, mat() if actn else None
+    w, b, cs = (f(rng.standard_normal(dim) * 0.3 + 1) if have else None for have in (with_w, with_b, with_cs))
+    s = scale * (cs if with_cs else np.ones(dim))
+    one, zero = np.ones(dim), np.zeros(dim)
+    out, z, eo, ez = ref.norm(kind, order, actn, x, res, gate, w if with_w else one, b if with_b else zero, s, EPS)
+    keep = order == "add_norm" and with_res
+    mx, mr, mg = Matrix(x, dtype, dim + gap, shift), Matrix(res, dtype) if with_res else None, Matrix(gate, dtype, dim + gap, shift) if actn else None
+    vw, vb, vc = (vector(v, dtype) if v is not None else None for v in (w, b, cs))
+    at = lambda v: v.ctypes.data if v is not None else None
+    mo, mz = Matrix(x, dtype, dim + gap), Matrix(x, dtype) if keep else None
+    shape = NormShape(DTYPES[dtype], {"rms": 0, "layer": 1}[kind], {"add_norm": 0, "norm_add": 1}[order], ACTS[actn or "none"], rows, dim, EPS, scale)
+    assert emu.emu_fused_norm(ctypes.byref(shape), *operand(mx), *operand(mr), *operand(mg), at(vw), at(vb), at(vc), *operand(mo), *operand(mz)) == 0, emu.emu_last_error()
+    ref.check(mo.get(), out, eo, dtype, "out")
+    assert mo.untouched_between() and mx.untouched_between()
+    if keep:
+        ref.check(mz.get(), z, ez, dtype, "residual_out")
+        # outputs in the place of inputs
+        assert emu.emu_fused_norm(ctypes.byref(shape), *operand(mx), *operand(mr), *operand(mg), at(vw), at(vb), at(vc), *operand(mx), *operand(mr)) == 0
+        assert (mx.get() == mo.get()).all() and (mr.get() == mz.get()).all()
+        mx.put(x)
+    # the gradient
+    dout, dstream = mat(), mat() if keep else None
+    zs = f(z)
+    md, mzs, mds = Matrix(dout, dtype, dim + gap, shift), Matrix(zs, dtype), Matrix(dstream, dtype) if keep else None
+    mdx, mdg, mdr = Matrix(x, dtype, dim + gap), Matrix(x, dtype) if actn else None, Matrix(x, dtype) if keep else None
+    dw, db, dc = (floats(np.full(dim, 9.0)) if have else None for have in (with_w, with_b, with_cs))
+    call = lambda ws, need: emu.emu_fused_norm_backward(ctypes.byref(shape), *operand(md), *operand(mzs), *operand(mg), at(vw), at(vb), at(vc), *(operand(mx) if with_cs and order == "add_norm" else NULL), *operand(mds),
+                                                        *operand(mdx), *operand(mdg), *operand(mdr), at(dw), at(db), at(dc), ws, need)
+    kept, ws, have = workspace_for(call)
+    assert call(ws, ctypes.byref(have)) == 0, emu.emu_last_error()
+    got, err = ref.norm_backward(kind, order, actn, dout, zs, gate, w if with_w else one, b if with_b else zero, s, EPS, x, dstream)
+    ref.check(mdx.get(), got["dx"], err["dx"], dtype, "dx")
+    if actn:
+        ref.check(mdg.get(), got["dgate"], err["dgate"], dtype, "dgate")
+    if keep:
+        ref.check(mdr.get(), got["dresidual"], err["dresidual"], dtype, "dresidual")
+    for name, v, factor in (("dweight", dw, 1.0), ("dbias", db, 1.0), ("dscale", dc, scale)):
+        if v is not None:
+            ref.check(v, got[name] * factor, err[name] * abs(factor) * 1.01, "f32", name)
+
+
+def test_fused_norm_many_rows(emu):
+    """More rows than blocks in the gradient's kernel, one wave per row with several rows per block, and rows without any content."""
+    emu = norm_emu(emu)
+    rng = np.random.default_rng(2)
+    rows, dim = 2100, 24
+    x, dout = rng.standard_normal((rows, dim)), rng.standard_normal((rows, dim))
+    x[7] = 0.0
+    mx, md, mo, mdx = (Matrix(v, "f32") for v in (x, dout, x, x))
+    x, dout = mx.get(), md.get()
+    w = rng.standard_normal(dim).astype(np.float32).astype(np.float64)
+    vw, dw = vector(w, "f32"), floats(np.full(dim, 9.0))
+    shape = NormShape(2, 0, 0, 0, rows, dim, EPS, 1.0)
+    assert emu.emu_fused_norm(ctypes.byref(shape), *operand(mx), *NULL, *NULL, vw.ctypes.data, None, None, *operand(mo), *NULL) == 0
+    out, _, eo, _ = ref.norm("rms", "add_norm", None, x, None, None, w, 0.0, 1.0, EPS)
+    ref.check(mo.get(), out, eo, "f32", "out")
+    call = lambda ws, need: emu.emu_fused_norm_backward(ctypes.byref(shape), *operand(md), *operand(mx), *NULL, vw.ctypes.data, None, None, *NULL, *NULL, *operand(mdx), *NULL, *NULL, dw.ctypes.data, None, None, ws, need)
+    kept, ws, have = workspace_for(call)
+    assert call(ws, ctypes.byref(have)) == 0
+    got, err = ref.norm_backward("rms", "add_norm", None, dout, x, None, w, 0.0, 1.0, EPS, None, None)
+    ref.check(mdx.get(), got["dx"], err["dx"], "f32", "dx")
+    ref.check(dw, got["dweight"], err["dweight"], "f32", "dweight")
+    shape.rows = 0  # no rows: the vectors' gradients are 0
+    assert emu.emu_fused_norm_backward(ctypes.byref(shape), *NULL, *NULL, *NULL, vw.ctypes.data, None, None, *NULL, *NULL, *NULL, *NULL, *NULL, dw.ctypes.data, None, None, ws, ctypes.byref(have)) == 0
+    assert (dw == 0).all()
+
+
+def test_norm_gradient_against_differences(emu):
+    rng = np.random.default_rng(3)
+    for kind, order, actn in itertools.product(("rms", "layer"), ("add_norm", "norm_add"), ("silu", "gelu", "sigmoid")):
+        x, res, gate, dout, dz = (rng.standard_normal((3, 5)) for _ in range(5))
+        w, b, s = (rng.standard_normal(5) for _ in range(3))
+        add = order == "add_norm"
+
+        def loss(x, res, gate, w, b, s):
+            out, z, _, _ = ref.norm(kind, order, actn, x, res, gate, w, b, s, 1e-3)
+            return float((out * dout).sum() + ((z * dz).sum() if add else 0.0))
+
+        z = res + s * x if add else x
+        got, _ = ref.norm_backward(kind, order, actn, dout, z, gate, w, b, s, 1e-3, x, dz if add else None)
+        args = [x, res, gate, w, b, s]
+        for k, name in enumerate(("dx", "dresidual", "dgate", "dweight", "dbias", "dscale")):
+            if name not in got:
+                continue
+            for at in itertools.product(*(range(n) for n in args[k].shape)):
+                lo, hi = [v.copy() for v in args], [v.copy() for v in args]
+                lo[k][at] -= 1e-5
+                hi[k][at] += 1e-5
+                assert abs((loss(*hi) - loss(*lo)) / 2e-5 - got[name][at]) < 1e-6, (kind, order, actn, name)
+
+
+def test_fused_norm_refusals(emu):
+    emu = norm_emu(emu)
+    buf = aligned(8192, np.uint8, 0)
+    p = buf.ctypes.data
+    err = lambda: emu.emu_last_error().decode()
+    big = sz(1 << 40)
+    ok = dict(dtype=0, norm=0, order=0, activation=0, rows=2, dim=8, eps=1e-6, scale=1.0)
+    m = lambda k: (p + 64 * k, 8)
+
+    def fwd(x=m(0), res=NULL, gate=NULL, cs=None, out=m(1), z=NULL, **k):
+        return emu.emu_fused_norm(ctypes.byref(NormShape(**{**ok, **k})), *x, *res, *gate, None, None, cs, *out, *z)
+
+    assert emu.emu_fused_norm(None, *NULL, *NULL, *NULL, None, None, None, *NULL, *NULL) == 1 and "null shape" in err()
+    assert fwd(dtype=5) == 1 and "dtype" in err()
+    assert fwd(norm=2) == 1 and "norm" in err()
+    assert fwd(order=2) == 1 and "order" in err()
+    assert fwd(activation=5) == 1 and "activation" in err()
+    assert fwd(activation=3) == 1 and "without a gate" in err()
+    assert fwd(dim=0) == 1 and fwd(dim=32769) == 2 and fwd(rows=1 << 31) == 2
+    assert fwd(scale=2.0) == 1 and "without a residual" in err()
+    assert fwd(cs=p) == 1 and "without a residual" in err()
+    assert fwd(z=m(2)) == 1 and "residual_out" in err()
+    assert fwd(res=m(2), z=m(1)) == 1 and "same buffer" in err()
+    assert fwd(x=(None, 8)) == 1 and "d_x is null" in err()
+    assert fwd(out=(p + 1, 8)) == 1 and "aligned" in err()
+    assert fwd(x=(p, 7)) == 1 and "overlap" in err()
+    assert fwd(rows=0, x=NULL, out=NULL) == 0
+
+    def back(dout=m(0), z=m(1), gate=NULL, x=NULL, dro=NULL, dx=m(2), dg=NULL, dr=NULL, dw=None, dc=None, ws=p // 256 * 256 + 1024, have=big, **k):
+        return emu.emu_fused_norm_backward(ctypes.byref(NormShape(**{**ok, **k})), *dout, *z, *gate, None, None, None, *x, *dro, *dx, *dg, *dr, dw, None, dc, ws, ctypes.byref(have))
+
+    assert back(have=sz(8)) == 4 and back(ws=p // 256 * 256 + 1032) == 1
+    assert back(dg=m(3)) == 1 and "without a gate" in err()
+    assert back(order=1, dr=m(3)) == 1 and "d_dout itself" in err()
+    assert back(dc=p) == 1 and "needs d_x" in err()
+    assert back(dr=m(2)) == 1 and "same buffer" in err()
+    assert back(dw=p + 2) == 1 and "d_dweight" in err()
+    need = sz(0)
+    assert back(ws=None, have=need, dw=p) == 0 and need.value == 256
