@@ -354,6 +354,26 @@ int tcu_fused_norm(const tcu_fused_norm_shape *shape, const void *d_x, size_t x_
  * Bit-reproducible. */
 int tcu_fused_norm_backward(const tcu_fused_norm_shape *shape, const void *d_dout, size_t dout_stride, const void *d_z, size_t z_stride, const void *d_gate, size_t gate_stride, const void *d_weight, const void *d_bias, const void *d_channel_scale, const void *d_x, size_t x_stride, const void *d_dresidual_out, size_t dresidual_out_stride, void *d_dx, size_t dx_stride, void *d_dgate, size_t dgate_stride, void *d_dresidual, size_t dresidual_stride, float *d_dweight, float *d_dbias, float *d_dchannel_scale, void *d_workspace, size_t *workspace_bytes, void *stream);
 
+/* Product with its epilogue: D = act(A B + bias) + beta C; A: M x K, B: K x N given as N rows of K (the operand layouts of
+ * tcu_gemm_*), C, D, Z: M x N, all row-major with the leading dimension next to them; bias: N values of the same type (NULL: 0).
+ * d_Z (NULL: not kept) receives A B + bias, which the gradient of an activation needs.  C is not read when beta == 0 and may be
+ * the same buffer as D (same leading dimension).  Sums in fp32, each result rounded once. */
+typedef struct {
+  int dtype;      /* TCU_F16 or TCU_BF16 */
+  int activation; /* tcu_activation */
+  size_t M, N, K; /* K up to 2^22 */
+  float beta;
+} tcu_fused_gemm_shape;
+
+/* The size query (d_workspace NULL) goes by the same arguments as the call: operands whose rows do not begin on 16 bytes are
+ * laid out anew in the workspace where the output has more than 64 rows. */
+int tcu_fused_gemm(const tcu_fused_gemm_shape *shape, const void *d_A, size_t lda, const void *d_B, size_t ldb, const void *d_bias, const void *d_C, size_t ldc, void *d_D, size_t ldd, void *d_Z, size_t ldz, void *d_workspace, size_t *workspace_bytes, void *stream);
+
+/* The gradient: with dZ = dD act'(Z) (TCU_ACT_NONE: dD, and d_Z is not read), dA = dZ B^T (M x K), dB (N rows of K) = dZ^T A and
+ * dbias (N fp32 values) = the sums of dZ over its rows, those that are not NULL; the gradient of C is beta dD.  shape->beta is
+ * not used.  dZ is rounded to the operands' type in front of the products, not of its sums.  M, N and K up to 2^22. */
+int tcu_fused_gemm_backward(const tcu_fused_gemm_shape *shape, const void *d_dD, size_t lddd, const void *d_A, size_t lda, const void *d_B, size_t ldb, const void *d_Z, size_t ldz, void *d_dA, size_t ldda, void *d_dB, size_t lddb, float *d_dbias, void *d_workspace, size_t *workspace_bytes, void *stream);
+
 /* ---- fills, conversions, inputs ---------------------------------------------------------------- */
 
 /* d[i] = (half) value.  Replaces cuda_memory_set / setFP16 (reference

@@ -13,7 +13,7 @@ EXPORTS = [
     "tcu_abi_version", "tcu_last_error", "tcu_init", "tcu_device_info", "tcu_set_option",
     "tcu_seg_reduce_f16", "tcu_seg_reduce_offsets_f16", "tcu_seg_scan_f16", "tcu_seg_scan_f16_noalloc", "tcu_seg_scan_offsets_f16", "tcu_seg_scan_by_key_f16", "tcu_seg_reduce_by_key_f16", "tcu_add_partial_sums_f16",
     "tcu_full_reduce_f16", "tcu_full_scan_f16", "tcu_gemv_f16_f32", "tcu_gemm_f16_f32", "tcu_gemv_f16_f16", "tcu_gemm_f16_f16", "tcu_gemv_col_major_f16_f32", "tcu_gemv_col_major_f16_f16",
-    "tcu_gated_scan", "tcu_gated_scan_backward", "tcu_gated_scan_step", "tcu_fused_norm", "tcu_fused_norm_backward",
+    "tcu_gated_scan", "tcu_gated_scan_backward", "tcu_gated_scan_step", "tcu_fused_norm", "tcu_fused_norm_backward", "tcu_fused_gemm", "tcu_fused_gemm_backward",
     "tcu_fill_f16", "tcu_convert_f32_to_f16", "tcu_generate_f16", "tcu_stream_probe", "tcu_time_next_launch", "tcu_lane_probe", "tcu_temporary_allocations",
 ]
 
@@ -94,6 +94,12 @@ class FusedNormShape(ctypes.Structure):
                 ("scale", ctypes.c_float)]
 
 
+class FusedGemmShape(ctypes.Structure):
+    """tcu_fused_gemm_shape."""
+
+    _fields_ = [("dtype", ctypes.c_int), ("activation", ctypes.c_int), ("M", ctypes.c_size_t), ("N", ctypes.c_size_t), ("K", ctypes.c_size_t), ("beta", ctypes.c_float)]
+
+
 class TcuError(RuntimeError):
     """A non-zero tcu_status; .status is 1 invalid argument, 2 unsupported, 3 runtime, 4 workspace."""
 
@@ -161,6 +167,9 @@ def lib():
         norm, m = c.POINTER(FusedNormShape), [vp, sz]
         L.tcu_fused_norm.argtypes = [norm, *m * 3, vp, vp, vp, *m * 2, vp]
         L.tcu_fused_norm_backward.argtypes = [norm, *m * 3, vp, vp, vp, *m * 5, vp, vp, vp, vp, psz, vp]
+        product = c.POINTER(FusedGemmShape)
+        L.tcu_fused_gemm.argtypes = [product, *m * 2, vp, *m * 3, vp, psz, vp]
+        L.tcu_fused_gemm_backward.argtypes = [product, *m * 6, vp, vp, psz, vp]
         for name in EXPORTS:
             if name not in ("tcu_last_error", "tcu_temporary_allocations"):
                 getattr(L, name).restype = ci
@@ -697,6 +706,72 @@ def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, c
         return got
 
     return _launch_on(dout.device, stream, body)
+
+
+def _operand(t, name, rows, columns, like):
+    """(pointer, leading dimension) of a matrix operand of the fused product (None: null)."""
+    if t is None:
+        return None, 0
+    if t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must have the type and device of the other operands ({like.dtype}, {like.device})")
+    p, n, stride = _matrix(t, name)
+    if n != rows or t.shape[-1] != columns:
+        raise ValueError(f"{name} must be {rows} x {columns}; got {tuple(t.shape)}")
+    return p, stride
+
+
+def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, out=None, preactivation=None, return_preactivation=False, workspace=None, stream=None):
+    """D = act(A @ Bt.T + bias) + beta * C (tcu_fused_gemm): A (..., K), Bt (N, K), bias (N,), C and D (..., N), float16 or bfloat16.
+
+    Returns D, or with return_preactivation or a `preactivation` tensor to fill (D, A @ Bt.T + bias); the second is what
+    fused_gemm_backward wants as Z.  C is not read when beta is 0; out may be C."""
+    torch = _torch()
+    dtype = _dtype_code(A, "A")
+    pa, M, lda = _matrix(A, "A")
+    if Bt.dim() != 2 or Bt.shape[-1] != A.shape[-1]:
+        raise ValueError("Bt must be (N, K) with the K of A")
+    N, K = Bt.shape
+    s = FusedGemmShape(dtype=dtype, activation=_enum(Activation, activation), M=M, N=N, K=K, beta=beta if C is not None else 0.0)
+    pb, pbias, pc = _operand(Bt, "Bt", N, K, A), _vector(bias, "bias", N, A), _operand(C, "C", M, N, A)
+
+    def body(raw):
+        new = lambda: torch.empty((*A.shape[:-1], N), dtype=A.dtype, device=A.device)
+        D = new() if out is None else out
+        Z = new() if preactivation is None and return_preactivation else preactivation
+        args = (ctypes.byref(s), pa, lda, *pb, pbias, *pc, *_operand(D, "out", M, N, A), *_operand(Z, "preactivation", M, N, A))
+        ws, have = _workspace_of(lib().tcu_fused_gemm, args, workspace, A.device)
+        _check(lib().tcu_fused_gemm(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        return D if Z is None else (D, Z)
+
+    return _launch_on(A.device, stream, body)
+
+
+def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_gradient=True, input_gradient=True, weight_gradient=True, workspace=None, stream=None):
+    """The gradient of fused_gemm (tcu_fused_gemm_backward): a dict with "dA" (like A), "dB" (like Bt) and "dbias" (float32),
+    those that are asked for.  Z: what fused_gemm returned as the activation's argument; the gradient of C is beta * dD."""
+    torch = _torch()
+    dtype = _dtype_code(A, "A")
+    pa, M, lda = _matrix(A, "A")
+    if Bt.dim() != 2 or Bt.shape[-1] != A.shape[-1]:
+        raise ValueError("Bt must be (N, K) with the K of A")
+    N, K = Bt.shape
+    s = FusedGemmShape(dtype=dtype, activation=_enum(Activation, activation), M=M, N=N, K=K)
+    pd, pb, pz = _operand(dD, "dD", M, N, A), _operand(Bt, "Bt", N, K, A), _operand(Z, "Z", M, N, A)
+
+    def body(raw):
+        got = {}
+        if input_gradient:
+            got["dA"] = torch.empty(A.shape, dtype=A.dtype, device=A.device)
+        if weight_gradient:
+            got["dB"] = torch.empty(Bt.shape, dtype=A.dtype, device=A.device)
+        if bias_gradient:
+            got["dbias"] = torch.empty(N, dtype=torch.float32, device=A.device)
+        args = (ctypes.byref(s), *pd, pa, lda, *pb, *pz, *(v for n in ("dA", "dB") for v in ((got[n].data_ptr(), K) if n in got else (None, 0))), got["dbias"].data_ptr() if bias_gradient else None)
+        ws, have = _workspace_of(lib().tcu_fused_gemm_backward, args, workspace, A.device)
+        _check(lib().tcu_fused_gemm_backward(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        return got
+
+    return _launch_on(A.device, stream, body)
 
 
 def fill(t, value, stream=None):

@@ -25,5 +25,15 @@ TCU_DEVICE unsigned pack_bf16x2(float lo, float hi) {
 }
 TCU_DEVICE uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
+// D = A B + C on 16x16x32 MFMAs of either 16-bit type, operands as 16-byte chunks (layouts: wave_ops.hpp)
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+template <bool BF16>
+TCU_DEVICE float4_t mfma_16x16x32_chunks(uint4_t a, uint4_t b, float4_t c) {
+  if constexpr (BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+  else
+    return mfma_16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
+}
+
 }  // namespace tcu
 #endif  // TCU_BLOCK_OPS_HPP

@@ -62,21 +62,21 @@ TCU_DEVICE uint4_t pack_chunk(const float (&v)[Elem<DT>::V]) {
 }
 
 // The chunk at element `at` of p, of which `count` elements exist (count <= 0: none; the others read as 0).
-// ALIGNED: p + at is 16-byte aligned and count is 0 or at least V.
-template <int DT, bool ALIGNED, bool NT = true>
+// WHOLE: count is at most 0 or at least V, and p + at is 16-byte aligned.  Otherwise a whole chunk is still one access
+// (the hardware takes 16-byte accesses at any element's address), and a part of one is read element by element.
+typedef unsigned any_chunk_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef float any_floats_t __attribute__((ext_vector_type(4), aligned(4)));
+
+template <int DT, bool WHOLE, bool NT = true>
 TCU_DEVICE uint4_t load_chunk_of(const void *p, size_t at, int count) {
   constexpr int V = Elem<DT>::V;
+  const typename Elem<DT>::word_t *q = static_cast<const typename Elem<DT>::word_t *>(p) + at;
   uint4_t c = {0u, 0u, 0u, 0u};
-  if constexpr (ALIGNED) {
-    if (count > 0) {
-      const uint4_t *q = reinterpret_cast<const uint4_t *>(static_cast<const typename Elem<DT>::word_t *>(p) + at);
-      if constexpr (NT)
-        c = __builtin_nontemporal_load(q);
-      else
-        c = *q;
-    }
-  } else {
-    const typename Elem<DT>::word_t *q = static_cast<const typename Elem<DT>::word_t *>(p) + at;
+  if (WHOLE ? count > 0 : count >= V) {
+    if constexpr (WHOLE && NT) c = __builtin_nontemporal_load(reinterpret_cast<const uint4_t *>(q));
+    if constexpr (WHOLE && !NT) c = *reinterpret_cast<const uint4_t *>(q);
+    if constexpr (!WHOLE) c = *reinterpret_cast<const any_chunk_t *>(q);  // neighbouring chunks share lines: cached
+  } else if constexpr (!WHOLE) {
 #pragma unroll
     for (int e = 0; e < V; e++) {
       if (e < count) {
@@ -90,20 +90,16 @@ TCU_DEVICE uint4_t load_chunk_of(const void *p, size_t at, int count) {
   }
   return c;
 }
-template <int DT, bool ALIGNED, bool NT = true>
+template <int DT, bool WHOLE, bool NT = true>
 TCU_DEVICE void store_chunk_of(void *p, size_t at, int count, const float (&v)[Elem<DT>::V]) {
   constexpr int V = Elem<DT>::V;
-  if constexpr (ALIGNED) {
-    if (count > 0) {
-      uint4_t *q = reinterpret_cast<uint4_t *>(static_cast<typename Elem<DT>::word_t *>(p) + at);
-      const uint4_t c = pack_chunk<DT>(v);
-      if constexpr (NT)
-        __builtin_nontemporal_store(c, q);
-      else
-        *q = c;
-    }
-  } else {
-    typename Elem<DT>::word_t *q = static_cast<typename Elem<DT>::word_t *>(p) + at;
+  typename Elem<DT>::word_t *q = static_cast<typename Elem<DT>::word_t *>(p) + at;
+  if (WHOLE ? count > 0 : count >= V) {
+    const uint4_t c = pack_chunk<DT>(v);
+    if constexpr (WHOLE && NT) __builtin_nontemporal_store(c, reinterpret_cast<uint4_t *>(q));
+    if constexpr (WHOLE && !NT) *reinterpret_cast<uint4_t *>(q) = c;
+    if constexpr (!WHOLE) *reinterpret_cast<any_chunk_t *>(q) = c;
+  } else if constexpr (!WHOLE) {
 #pragma unroll
     for (int e = 0; e < V; e++)
       if (e < count) q[e] = Elem<DT>::round(v[e]);
@@ -111,30 +107,36 @@ TCU_DEVICE void store_chunk_of(void *p, size_t at, int count, const float (&v)[E
 }
 
 // V fp32 values at element `at` of a fp32 vector, the same conventions
-template <int V, bool ALIGNED>
+template <int V, bool WHOLE>
 TCU_DEVICE void load_floats(const float *p, size_t at, int count, float (&v)[V]) {
-  if constexpr (ALIGNED) {
-    if (count > 0) {
+  if (WHOLE ? count > 0 : count >= V) {
 #pragma unroll
-      for (int i = 0; i < V / 4; i++) {
-        const float4_t q = *reinterpret_cast<const float4_t *>(p + at + 4 * i);
+    for (int i = 0; i < V / 4; i++) {
+      float4_t q;
+      if constexpr (WHOLE)
+        q = *reinterpret_cast<const float4_t *>(p + at + 4 * i);
+      else
+        q = *reinterpret_cast<const any_floats_t *>(p + at + 4 * i);
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[4 * i + e] = q[e];
-      }
-      return;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < V; e++) v[e] = e < count ? p[at + e] : 0.0f;
-}
-template <int V, bool ALIGNED>
-TCU_DEVICE void store_floats(float *p, size_t at, int count, const float (&v)[V]) {
-  if constexpr (ALIGNED) {
-    if (count > 0) {
-#pragma unroll
-      for (int i = 0; i < V / 4; i++) *reinterpret_cast<float4_t *>(p + at + 4 * i) = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+      for (int e = 0; e < 4; e++) v[4 * i + e] = q[e];
     }
   } else {
+#pragma unroll
+    for (int e = 0; e < V; e++) v[e] = !WHOLE && e < count ? p[at + e] : 0.0f;
+  }
+}
+template <int V, bool WHOLE>
+TCU_DEVICE void store_floats(float *p, size_t at, int count, const float (&v)[V]) {
+  if (WHOLE ? count > 0 : count >= V) {
+#pragma unroll
+    for (int i = 0; i < V / 4; i++) {
+      const float4_t q = float4_t{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+      if constexpr (WHOLE)
+        *reinterpret_cast<float4_t *>(p + at + 4 * i) = q;
+      else
+        *reinterpret_cast<any_floats_t *>(p + at + 4 * i) = q;
+    }
+  } else if constexpr (!WHOLE) {
 #pragma unroll
     for (int e = 0; e < V; e++)
       if (e < count) p[at + e] = v[e];

@@ -1,0 +1,394 @@
+// Matrix product with its epilogue, in fp16 or bf16:  D = act(A B + bias) + beta C,  and Z = A B + bias where a backward
+// pass will want it.  A: M x K row-major, B: K x N given as N rows of K (a weight matrix as models hold it), bias: N.
+//
+// Gradient: dZ = dD * act'(Z) element by element, dA = dZ B^T (M x K), dB = dZ^T A (N rows of K), dbias = the column sums of
+// dZ, dC = beta dD.  The two products sum over N and over M, along which B and A (and dZ for the second) are not contiguous:
+// they run on transposed copies, which one pass each writes into the workspace; dZ and its transpose come out of the same pass.
+//
+//   fused_gemm_tile_kernel : many rows.  256 x 256 or 128 x 128 block tiles on 16x16x32 MFMAs, K steps of 64, operands moved
+//                global -> LDS by transfers that run two steps ahead (three buffers for A, two for B), the loop of
+//                gemm_dlds_a3b2_m16_kernel.  M and N may be anything (rows beyond the last one are read as the last one and
+//                not stored), K too (a step with what is left of K goes through registers, zero-filled).
+//                Bound by the matrix unit.  Where the tiles are fewer than the compute units, several blocks share a tile's
+//                K steps and fused_gemm_join_kernel adds their fp32 shares in a fixed order.
+//   fused_gemm_few_rows_kernel : up to 64 rows.  Bound by reading B once: a block takes 16 columns of the output and all rows,
+//                its waves share K and meet in LDS.
+// Sums are fp32; the epilogue is applied to the fp32 sum and each result rounded once.  dZ is rounded to the operands' type,
+// because the matrix unit takes operands of 16 bits; its column sums are taken before that.
+#pragma once
+
+#include "elements.hpp"
+#include "gemm.hpp"
+
+namespace tcu {
+
+struct FusedGemmParams {
+  const void *A, *B, *bias, *C;  // bias, C may be null
+  void *D, *Z;                   // Z may be null
+  size_t lda, ldb, ldc, ldd, ldz;
+  size_t M, N, K;
+  float beta;
+  int act;
+  float *shares;           // null: the blocks finish their tiles; else raw sums, [split][M][share_ld]
+  size_t share_ld;
+  unsigned splits, tiles;  // blocks: splits * tiles, the splits of K outermost
+};
+
+// z = sum + bias, d = act(z) + beta c for the chunk at (row, col), of which `count` columns exist
+template <int DT, bool WHOLE>
+TCU_DEVICE void fused_gemm_finish(const FusedGemmParams &p, size_t row, size_t col, int count, float (&v)[8], const float (&bias)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] += bias[e];
+  if (p.Z) store_chunk_of<DT, WHOLE>(p.Z, row * p.ldz + col, count, v);
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = activation<false>(p.act, v[e]);
+  if (p.C) {
+    float c[8];
+    unpack_chunk<DT>(load_chunk_of<DT, WHOLE>(p.C, row * p.ldc + col, count), c);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(p.beta, c[e], v[e]);
+  }
+  store_chunk_of<DT, WHOLE>(p.D, row * p.ldd + col, count, v);
+}
+
+// One block tile (W8 = 8: 256 x 256, W8 = 4: 128 x 128; waves of 16 W8 x 16 W8).  Rows of A and B begin on 16 bytes; a tile's
+// rows of either lie within 4 GiB.  The product is formed transposed (B fragment first), so a lane owns row (lane & 15)
+// and four adjacent columns of every 16 x 16 tile.
+template <int DT, bool WHOLE, int W8>
+TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t tile_n, size_t step0, size_t steps, bool tail, float *share) {
+  constexpr int BK = 64, ROWH = BK, CPR = 8, RPT = 8, RS = 1, SUB = 2, NA = 3, NB = 2;
+  constexpr int TILE = 32 * W8, WT = 16 * W8;
+  constexpr int NM = W8 * W8;
+  constexpr int OPH = TILE * ROWH;
+  constexpr int TPW = TILE / RPT / 4;
+  constexpr int TEVERY = NM / 2 / TPW;
+  constexpr bool BF16 = DT == kBF16;
+  static_assert(W8 == 8 || W8 == 4, "fragment reads and transfers must fit a substep");
+  __shared__ __attribute__((aligned(1024))) half_t lds_a[NA][OPH];
+  __shared__ __attribute__((aligned(1024))) half_t lds_b[NB][OPH];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave >> 1, wn = wave & 1;
+  const size_t row0 = tile_m * TILE, col0 = tile_n * TILE;
+  const unsigned last_a = (unsigned)(p.M - row0 < TILE ? p.M - row0 : TILE) - 1, last_b = (unsigned)(p.N - col0 < TILE ? p.N - col0 : TILE) - 1;
+  const char *A = static_cast<const char *>(p.A) + row0 * p.lda * 2, *B = static_cast<const char *>(p.B) + col0 * p.ldb * 2;
+
+  float4_t acc[W8][W8];
+#pragma unroll
+  for (int i = 0; i < W8; i++)
+#pragma unroll
+    for (int j = 0; j < W8; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+  const int frow = lane & 15, kq = lane >> 4, fsw = (frow >> RS) & (CPR - 1);
+  const int fa0 = (wm * WT + frow) * ROWH, fb0 = (wn * WT + frow) * ROWH;
+  int ko[SUB];
+#pragma unroll
+  for (int kk = 0; kk < SUB; kk++) ko[kk] = ((4 * kk + kq) ^ fsw) * 8;
+  auto fragment = [](const half_t *q) { return *reinterpret_cast<const uint4_t *>(q); };
+
+  if (steps) {  // the same for the whole block
+    uint32_t off_a[TPW], off_b[TPW];
+#pragma unroll
+    for (int t = 0; t < TPW; t++) {
+      const unsigned row = (unsigned)((wave * TPW + t) * RPT + lane / CPR);
+      const unsigned chunk = (unsigned)(lane % CPR) ^ ((row >> RS) & (CPR - 1));
+      const unsigned ra = row < last_a ? row : last_a, rb = row < last_b ? row : last_b;
+      off_a[t] = (uint32_t)((ra * p.lda + chunk * 8) * 2);
+      off_b[t] = (uint32_t)((rb * p.ldb + chunk * 8) * 2);
+    }
+    constexpr lds_addr_t STAGE = OPH * 2, TBYTES = 1024, STEPB = BK * 2;
+    const char *ga = A + step0 * STEPB, *gb = B + step0 * STEPB;
+    const lds_addr_t ta = wave_uniform(lds_address_of(&lds_a[0][0]) + wave * TPW * TBYTES);
+    const lds_addr_t tb = wave_uniform(lds_address_of(&lds_b[0][0]) + wave * TPW * TBYTES);
+    // steps past the end: a harmless re-read of the last step into a free buffer
+    auto issue_a = [&](size_t step, int buf, int t) { load_chunk_to_lds(ga + (step < steps ? step : steps - 1) * STEPB, off_a[t], ta + buf * STAGE + t * TBYTES); };
+    auto issue_b = [&](size_t step, int buf, int t) { load_chunk_to_lds(gb + (step < steps ? step : steps - 1) * STEPB, off_b[t], tb + buf * STAGE + t * TBYTES); };
+    // in flight at the first barrier: A0 B0 | A1 B1 (the wave's counter returns in issue order)
+#pragma unroll
+    for (int t = 0; t < TPW; t++) issue_a(0, 0, t);
+#pragma unroll
+    for (int t = 0; t < TPW; t++) issue_b(0, 0, t);
+#pragma unroll
+    for (int t = 0; t < TPW; t++) issue_a(1, 1, t);
+#pragma unroll
+    for (int t = 0; t < TPW; t++) issue_b(1, 1, t);
+    wait_vector_loads<2 * TPW>();
+    block_barrier_lds_only();
+    uint4_t fa[2][W8], fb[2][W8];
+#pragma unroll
+    for (int i = 0; i < W8; i++) {
+      fa[0][i] = fragment(&lds_a[0][fa0 + i * 16 * ROWH + ko[0]]);
+      fb[0][i] = fragment(&lds_b[0][fb0 + i * 16 * ROWH + ko[0]]);
+    }
+    int ca = 0, cb = 0;  // s % NA, s % NB
+    for (size_t s = 0; s < steps; s++) {
+      const int na = ca + 1 == NA ? 0 : ca + 1, nb = cb ^ 1;
+      const int fill_a = ca == 0 ? NA - 1 : ca - 1;  // A buffer of step s - 1 = of step s + 2
+      // substep 0: MFMA t works on tile (t / W8, t % W8); the fragments of substep 1 are read under it, the A tile of
+      // step s + 2 goes out under its second half
+#pragma unroll
+      for (int t = 0; t < NM; t++) {
+        if (t < 4 * W8 && t % 2 == 0) {
+          const int k = t / 2;
+          if (k == 0) fa[1][0] = fragment(&lds_a[ca][fa0 + ko[1]]);
+          else if (k <= W8) fb[1][k - 1] = fragment(&lds_b[cb][fb0 + (k - 1) * 16 * ROWH + ko[1]]);
+          else fa[1][k - W8] = fragment(&lds_a[ca][fa0 + (k - W8) * 16 * ROWH + ko[1]]);
+        }
+        if (t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_a(s + 2, fill_a, (t - NM / 2) / TEVERY);
+        acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[0][t % W8], fa[0][t / W8], acc[t / W8][t % W8]);
+        sched_fence();
+      }
+      // substep 1: own transfers of step s + 1 done (the A tile of step s + 2 may still fly), barrier, fragments of step
+      // s + 1; the B tile of step s + 2 into the B buffer of step s
+      wait_vector_loads<TPW>();
+      block_barrier_lds_only();
+      sched_fence();
+#pragma unroll
+      for (int t = 0; t < NM; t++) {
+        if (t < 4 * W8 && t % 2 == 0) {
+          const int k = t / 2;
+          if (k == 0) fa[0][0] = fragment(&lds_a[na][fa0 + ko[0]]);
+          else if (k <= W8) fb[0][k - 1] = fragment(&lds_b[nb][fb0 + (k - 1) * 16 * ROWH + ko[0]]);
+          else fa[0][k - W8] = fragment(&lds_a[na][fa0 + (k - W8) * 16 * ROWH + ko[0]]);
+        }
+        if (t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_b(s + 2, cb, (t - NM / 2) / TEVERY);
+        acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[1][t % W8], fa[1][t / W8], acc[t / W8][t % W8]);
+        sched_fence();
+      }
+      ca = na;
+      cb = nb;
+    }
+    wait_vector_loads<0>();  // the re-reads past the last step must land before the buffers are used for anything else
+  }
+  if (tail) {  // the same for the whole block: the last K % 64, zero-filled, through registers into the first buffers
+    const size_t k0 = p.K / BK * BK;
+    const int left = (int)(p.K - k0);
+    block_barrier_lds_only();
+#pragma unroll
+    for (int t = 0; t < TILE * CPR / 256; t++) {
+      const int row = (t * 256 + tid) / CPR, chunk = (t * 256 + tid) % CPR;
+      const unsigned ra = (unsigned)row < last_a ? (unsigned)row : last_a, rb = (unsigned)row < last_b ? (unsigned)row : last_b;
+      const int slot = row * ROWH + (chunk ^ ((row >> RS) & (CPR - 1))) * 8;
+      *reinterpret_cast<uint4_t *>(&lds_a[0][slot]) = load_chunk_of<DT, false>(A, ra * p.lda + k0 + chunk * 8, left - chunk * 8);
+      *reinterpret_cast<uint4_t *>(&lds_b[0][slot]) = load_chunk_of<DT, false>(B, rb * p.ldb + k0 + chunk * 8, left - chunk * 8);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < SUB; kk++) {
+      uint4_t fa[W8], fb[W8];
+#pragma unroll
+      for (int i = 0; i < W8; i++) {
+        fa[i] = fragment(&lds_a[0][fa0 + i * 16 * ROWH + ko[kk]]);
+        fb[i] = fragment(&lds_b[0][fb0 + i * 16 * ROWH + ko[kk]]);
+      }
+#pragma unroll
+      for (int t = 0; t < NM; t++) acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[t % W8], fa[t / W8], acc[t / W8][t % W8]);
+    }
+  }
+  // Epilogue: a row of W8 tiles (16 rows x 16 W8 columns) is turned through LDS, so that a lane finishes 8 adjacent columns of
+  // a row and global memory sees whole rows of the wave's tile.
+  constexpr int SROW = 16 * W8 + 4, LPR = 2 * W8, RPA = 64 / LPR;  // floats per parked row, lanes per row, rows per access
+  static_assert(4 * 2 * 16 * SROW * sizeof(float) <= sizeof(lds_a), "parking area of four waves");
+  block_barrier_lds_only();  // the other waves have read their last fragments
+  float *park = reinterpret_cast<float *>(&lds_a[0][0]) + wave * (2 * 16 * SROW);
+  const int rr = lane / LPR, rc = (lane % LPR) * 8;
+  const size_t col = col0 + wn * WT + rc;
+  const int count = col < p.N ? (int)(p.N - col < 8 ? p.N - col : 8) : 0;
+  float bias[8] = {};
+  if (p.bias && !share) unpack_chunk<DT>(load_chunk_of<DT, WHOLE, false>(p.bias, col, count), bias);
+#pragma unroll
+  for (int i = 0; i < W8; i++) {
+    float *buf = park + (i & 1) * (16 * SROW);
+#pragma unroll
+    for (int j = 0; j < W8; j++) *reinterpret_cast<float4_t *>(buf + frow * SROW + 16 * j + 4 * kq) = acc[i][j];
+    wave_lds_fence();
+#pragma unroll
+    for (int t = 0; t < 16 / RPA; t++) {
+      const int r = t * RPA + rr;
+      const size_t row = row0 + wm * WT + 16 * i + r;
+      if (row >= p.M) continue;
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const float4_t q = *reinterpret_cast<const float4_t *>(buf + r * SROW + rc + e);
+        v[e] = q[0];
+        v[e + 1] = q[1];
+        v[e + 2] = q[2];
+        v[e + 3] = q[3];
+      }
+      if (share)
+        store_floats<8, true>(share, row * p.share_ld + col, col < p.share_ld ? 8 : 0, v);  // share_ld: N up to a multiple of 8
+      else
+        fused_gemm_finish<DT, WHOLE>(p, row, col, count, v, bias);
+    }
+  }
+}
+
+template <int DT, bool WHOLE, int W8>
+__global__ __launch_bounds__(256, W8 == 4 ? 2 : 1) void fused_gemm_tile_kernel(FusedGemmParams p) {
+  constexpr int TILE = 32 * W8;
+  const unsigned split = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
+  size_t tile_m, tile_n;
+  gemm_tile_of_block((p.M + TILE - 1) / TILE, (p.N + TILE - 1) / TILE, tile, &tile_m, &tile_n);
+  const size_t full = p.K / 64, per = (full + p.splits - 1) / p.splits;
+  const size_t step0 = split * per < full ? split * per : full, end = step0 + per < full ? step0 + per : full;
+  fused_gemm_tile<DT, WHOLE, W8>(p, tile_m, tile_n, step0, end - step0, split + 1 == p.splits && p.K % 64 != 0, p.shares ? p.shares + (size_t)split * p.M * p.share_ld : nullptr);
+}
+
+// The epilogue over the sum of the shares, one thread per 8 adjacent columns, the shares in order.
+template <int DT, bool WHOLE>
+__global__ __launch_bounds__(256) void fused_gemm_join_kernel(FusedGemmParams p) {
+  const size_t chunks = p.share_ld / 8, at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.M * chunks) return;
+  const size_t row = at / chunks, col = at % chunks * 8;
+  const int count = p.N - col < 8 ? (int)(p.N - col) : 8;
+  float v[8] = {}, bias[8] = {};
+  for (unsigned s = 0; s < p.splits; s++) {
+    float w[8];
+    load_floats<8, true>(p.shares, ((size_t)s * p.M + row) * p.share_ld + col, 8, w);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] += w[e];
+  }
+  if (p.bias) unpack_chunk<DT>(load_chunk_of<DT, WHOLE, false>(p.bias, col, count), bias);
+  fused_gemm_finish<DT, WHOLE>(p, row, col, count, v, bias);
+}
+
+// Up to 16 * MT rows: a block of WAVES waves takes 16 columns; wave w takes the K steps of 32 * UNROLL elements w, w + WAVES, ...
+// of its split (a lane reads row (lane & 15) of 16 rows of B, 16 bytes at k = 8 (lane >> 4): 64 bytes of each row per
+// instruction, UNROLL instructions in flight).
+template <int DT, bool WHOLE, int MT, int WAVES, int UNROLL>
+__global__ __launch_bounds__(64 * WAVES) void fused_gemm_few_rows_kernel(FusedGemmParams p) {
+  constexpr bool BF16 = DT == kBF16;
+  constexpr int STEP = 32 * UNROLL;
+  __shared__ __attribute__((aligned(16))) float lds[WAVES][MT][16][20];  // [row of the output][column], padded
+  const int lane = lane_id(), wave = wave_in_block(), frow = lane & 15, kq = lane >> 4;
+  const unsigned split = blockIdx.x / p.tiles;
+  const size_t col0 = (size_t)(blockIdx.x % p.tiles) * 16;
+  const size_t n = col0 + frow < p.N ? col0 + frow : p.N - 1;
+  const size_t steps = (p.K + STEP - 1) / STEP, per = (steps + p.splits - 1) / p.splits;
+  const size_t end = (split + 1) * per < steps ? (split + 1) * per : steps;
+  float4_t acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; i++) acc[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (size_t s = split * per + wave; s < end; s += WAVES) {
+    uint4_t b[UNROLL], a[MT][UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++) {
+      const size_t k = s * STEP + 32 * u + 8 * kq;
+      const int count = k < p.K ? (int)(p.K - k < 8 ? p.K - k : 8) : 0;
+      b[u] = load_chunk_of<DT, WHOLE>(p.B, n * p.ldb + k, count);
+#pragma unroll
+      for (int i = 0; i < MT; i++) a[i][u] = load_chunk_of<DT, WHOLE, false>(p.A, (16 * i + frow) * p.lda + k, (size_t)(16 * i + frow) < p.M ? count : 0);
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; u++)
+#pragma unroll
+      for (int i = 0; i < MT; i++) acc[i] = mfma_16x16x32_chunks<BF16>(b[u], a[i][u], acc[i]);  // lane: row (lane & 15), columns 4 (lane >> 4) ...
+  }
+#pragma unroll
+  for (int i = 0; i < MT; i++) *reinterpret_cast<float4_t *>(&lds[wave][i][frow][4 * kq]) = acc[i];
+  __syncthreads();
+  // 2 * 16 * MT chunks of 8 columns
+  for (int q = (int)threadIdx.x; q < 32 * MT; q += 64 * WAVES) {
+    const int r = q / 2, c = (q % 2) * 8;
+    const size_t row = r, col = col0 + c;
+    const int count = col < p.N ? (int)(p.N - col < 8 ? p.N - col : 8) : 0;
+    if (row >= p.M || count == 0) continue;
+    float v[8] = {}, bias[8] = {};
+#pragma unroll
+    for (int w = 0; w < WAVES; w++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[e] += lds[w][r / 16][r % 16][c + e];
+    if (p.shares) {
+      store_floats<8, true>(p.shares, ((size_t)split * p.M + row) * p.share_ld + col, 8, v);
+    } else {
+      if (p.bias) unpack_chunk<DT>(load_chunk_of<DT, WHOLE, false>(p.bias, col, count), bias);
+      fused_gemm_finish<DT, WHOLE>(p, row, col, count, v, bias);
+    }
+  }
+}
+
+// `rows` x `width` elements of 16 bits to rows of `to_ld` elements, 16-byte aligned (for operands whose rows are not)
+struct PackRowsParams {
+  const uint16_t *from;
+  uint16_t *to;
+  size_t rows, width, from_ld, to_ld;
+};
+__global__ __launch_bounds__(256) inline void pack_rows_kernel(PackRowsParams p) {
+  const size_t chunks = (p.width + 7) / 8, at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= p.rows * chunks) return;
+  const size_t row = at / chunks, col = at % chunks * 8;
+  const uint4_t c = load_chunk_of<kF16, false>(p.from, row * p.from_ld + col, p.width - col < 8 ? (int)(p.width - col) : 8);
+  *reinterpret_cast<uint4_t *>(p.to + row * p.to_ld + col) = c;  // to_ld: a multiple of 8, so what lies beyond the width is padding
+}
+
+// 64 x 64 tiles turned through LDS.  GRAD: what is turned is dZ = dD * act'(Z), written as it stands as well (dz, which may be
+// null), with the column sums of each 64-row strip before rounding (partial, may be null).
+struct TransposeParams {
+  const void *from, *Z;  // dD and Z with GRAD
+  void *to, *dz;
+  float *partial;        // [row strip][columns]
+  size_t rows, columns, from_ld, z_ld, to_ld, dz_ld;
+  unsigned column_tiles;
+  int act;
+};
+template <int DT, bool GRAD>
+__global__ __launch_bounds__(256) void transpose_kernel(TransposeParams p) {
+  constexpr int LD = 66;  // 16-bit elements per LDS row: 33 words, so a column of 16-bit pairs falls into different banks
+  __shared__ __attribute__((aligned(16))) uint16_t lds[64 * LD];
+  __shared__ float sums[GRAD ? 32 * 64 : 1];
+  const size_t row0 = (size_t)(blockIdx.x / p.column_tiles) * 64, col0 = (size_t)(blockIdx.x % p.column_tiles) * 64;
+  const int tid = (int)threadIdx.x, tr = tid / 8, tc = (tid % 8) * 8;  // 32 rows of 8 chunks a round
+  float s[8] = {};
+#pragma unroll
+  for (int h = 0; h < 2; h++) {
+    const int r = h * 32 + tr;
+    const size_t row = row0 + r, col = col0 + tc;
+    const int count = row < p.rows && col < p.columns ? (p.columns - col < 8 ? (int)(p.columns - col) : 8) : 0;
+    uint4_t c = load_chunk_of<DT, false>(p.from, count ? row * p.from_ld + col : 0, count);
+    if constexpr (GRAD) {
+      float d[8], z[8];
+      unpack_chunk<DT>(c, d);
+      if (p.Z) {
+        unpack_chunk<DT>(load_chunk_of<DT, false>(p.Z, count ? row * p.z_ld + col : 0, count), z);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          float value, slope;
+          activation_slope<false>(p.act, z[e], &value, &slope);
+          d[e] = e < count ? d[e] * slope : 0.0f;
+        }
+        c = pack_chunk<DT>(d);
+      }
+      if (p.dz) store_chunk_of<DT, false>(p.dz, count ? row * p.dz_ld + col : 0, count, d);
+#pragma unroll
+      for (int e = 0; e < 8; e++) s[e] += d[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) *reinterpret_cast<uint32_t *>(&lds[r * LD + tc + 2 * e]) = c[e];
+  }
+  if constexpr (GRAD) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) sums[tr * 64 + tc + e] = s[e];
+  }
+  __syncthreads();
+  if constexpr (GRAD) {
+    if (p.partial && tid < 64 && col0 + tid < p.columns) {
+      float t = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 32; r++) t += sums[r * 64 + tid];
+      p.partial[row0 / 64 * p.columns + col0 + tid] = t;
+    }
+  }
+  if (!p.to) return;
+#pragma unroll
+  for (int h = 0; h < 2; h++) {  // row tr (+ 32) of the transpose: 8 chunks of 8 of the tile's rows
+    const int r = h * 32 + tr;
+    const size_t row = col0 + r, col = row0 + tc;
+    if (row >= p.columns || col >= p.rows) continue;
+    uint4_t c;
+#pragma unroll
+    for (int e = 0; e < 4; e++) c[e] = (unsigned)lds[(tc + 2 * e) * LD + r] | (unsigned)lds[(tc + 2 * e + 1) * LD + r] << 16;
+    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(p.to) + row * p.to_ld + col) = c;  // to_ld: a multiple of 8
+  }
+}
+
+}  // namespace tcu

@@ -1,0 +1,298 @@
+// Argument checks, workspace layout and kernel selection of the fused product's entry points.
+#pragma once
+
+#include <utility>
+
+#include "checks.hpp"
+#include "column_sum.hpp"
+#include "fused_gemm.hpp"
+#include "launch.hpp"
+
+namespace tcu {
+
+constexpr size_t kGemmFewRows = 64;               // up to this many rows the product is bound by reading B
+constexpr size_t kGemmMaxInner = (size_t)1 << 22; // a tile's rows of an operand lie within 32-bit byte offsets: 256 * 2^22 * 2 < 2^32
+
+inline size_t up_to(size_t n, size_t step) { return (n + step - 1) / step * step; }
+// bytes of a part of a workspace
+inline size_t part_bytes(size_t bytes) { return up_to(bytes, 256); }
+
+// How one product M x N over K runs, and what it takes of the workspace.
+struct GemmPlan {
+  bool few_rows = false;
+  int few_tiles = 1;           // few rows: 16-row tiles
+  bool big = false;            // 256 x 256 tiles, else 128 x 128
+  size_t tiles = 0, splits = 1;
+  size_t share_ld = 0, share_bytes = 0;
+};
+inline GemmPlan plan_gemm(size_t M, size_t N, size_t K) {
+  GemmPlan g;
+  g.share_ld = up_to(N, 8);
+  if (M <= kGemmFewRows) {
+    g.few_rows = true;
+    g.few_tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    g.tiles = (N + 15) / 16;
+    // a block per compute unit: below that the waves of one compute unit cannot keep its share of the memory's bandwidth in flight
+    const size_t steps = K / 1024;
+    while (g.tiles * g.splits < 256 && g.splits * 2 <= steps) g.splits *= 2;
+  } else {
+    const size_t t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128);
+    g.big = t256 >= 128;
+    g.tiles = g.big ? t256 : t128;
+    const size_t steps = K / 64;
+    if (!g.big)
+      while (g.tiles * g.splits * 2 <= 512 && g.splits * 2 * 4 <= steps) g.splits *= 2;
+  }
+  if (g.splits > 1) g.share_bytes = part_bytes(g.splits * M * g.share_ld * 4);
+  return g;
+}
+
+// One product on operands that are ready for it.
+template <int DT, bool WHOLE>
+inline void launch_gemm(const GemmPlan &g, FusedGemmParams p, float *shares, bool whole_inner, void *stream) {
+  p.splits = (unsigned)g.splits;
+  p.tiles = (unsigned)g.tiles;
+  p.share_ld = g.share_ld;
+  p.shares = g.splits > 1 ? shares : nullptr;
+  const unsigned grid = (unsigned)(g.tiles * g.splits);
+  if (g.few_rows) {
+#define TCU_FEW(MT, UNROLL) \
+  (WHOLE && whole_inner ? launch(fused_gemm_few_rows_kernel<DT, WHOLE, MT, 8, UNROLL>, grid, 512u, stream, p) : launch(fused_gemm_few_rows_kernel<DT, false, MT, 8, UNROLL>, grid, 512u, stream, p))
+    if (g.few_tiles == 1) TCU_FEW(1, 4);
+    else if (g.few_tiles == 2) TCU_FEW(2, 4);
+    else TCU_FEW(4, 2);
+#undef TCU_FEW
+  } else if (g.big) {
+    launch(fused_gemm_tile_kernel<DT, WHOLE, 8>, grid, 256u, stream, p);
+  } else {
+    launch(fused_gemm_tile_kernel<DT, WHOLE, 4>, grid, 256u, stream, p);
+  }
+  if (g.splits > 1) launch(fused_gemm_join_kernel<DT, WHOLE>, (unsigned)((p.M * (g.share_ld / 8) + 255) / 256), 256u, stream, p);
+}
+inline void run_gemm(int dtype, bool whole, const GemmPlan &g, const FusedGemmParams &p, float *shares, bool whole_inner, void *stream) {
+  if (dtype == TCU_F16) {
+    if (whole) launch_gemm<kF16, true>(g, p, shares, whole_inner, stream);
+    else launch_gemm<kF16, false>(g, p, shares, whole_inner, stream);
+  } else {
+    if (whole) launch_gemm<kBF16, true>(g, p, shares, whole_inner, stream);
+    else launch_gemm<kBF16, false>(g, p, shares, whole_inner, stream);
+  }
+}
+
+// rows of 16 bits that the transfers of the tile kernel can take as they are
+inline bool rows_ready(const void *p, size_t ld) { return aligned_to(p, 16) && ld % 8 == 0 && ld <= kGemmMaxInner; }
+
+inline int check_gemm_shape(const std::string &w, const tcu_fused_gemm_shape *s) {
+  if (!s) return report_failure(TCU_ERR_INVALID_ARG, w + ": null shape");
+  if (s->dtype != TCU_F16 && s->dtype != TCU_BF16) return report_failure(TCU_ERR_INVALID_ARG, w + ": dtype must be TCU_F16 or TCU_BF16");
+  if (!known_activation(s->activation)) return report_failure(TCU_ERR_INVALID_ARG, w + ": unknown activation");
+  const size_t most = (size_t)1 << 31;
+  if (s->M >= most || s->N >= most || s->K > kGemmMaxInner) return report_failure(TCU_ERR_UNSUPPORTED, w + ": M or N from 2^31 on, or K above 2^22");
+  return TCU_OK;
+}
+// grids are counted in 32 bits: the smallest tiles any of the kernels may use
+inline int check_gemm_grid(const std::string &w, size_t M, size_t N) {
+  size_t chunks = 0;
+  if (!product_fits(M, up_to(N, 8) / 8, &chunks) || chunks / 256 >= ((size_t)1 << 30)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": output too large");
+  return TCU_OK;
+}
+
+inline void pack_rows(const void *from, size_t from_ld, void *to, size_t to_ld, size_t rows, size_t width, void *stream) {
+  const PackRowsParams q{static_cast<const uint16_t *>(from), static_cast<uint16_t *>(to), rows, width, from_ld, to_ld};
+  launch(pack_rows_kernel, (unsigned)((rows * ((width + 7) / 8) + 255) / 256), 256u, stream, q);
+}
+
+inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, size_t lda, const void *B, size_t ldb, const void *bias, const void *C, size_t ldc, void *D, size_t ldd, void *Z, size_t ldz,
+                               void *workspace, size_t *workspace_bytes, void *stream) {
+  const std::string w("tcu_fused_gemm");
+  if (int rc = check_gemm_shape(w, s)) return rc;
+  if (int rc = check_gemm_grid(w, s->M, s->N)) return rc;
+  const size_t M = s->M, N = s->N, K = s->K;
+  const GemmPlan g = plan_gemm(M, N, K);
+  const bool pack_a = !g.few_rows && K && !rows_ready(A, M > 1 ? lda : 8), pack_b = !g.few_rows && K && !rows_ready(B, N > 1 ? ldb : 8);
+  const size_t ldk = up_to(K, 8), a_bytes = pack_a ? part_bytes(M * ldk * 2) : 0, b_bytes = pack_b ? part_bytes(N * ldk * 2) : 0;
+  const size_t bytes = g.share_bytes + a_bytes + b_bytes, need = bytes < 256 ? 256 : bytes;
+  if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
+  if (!workspace) {
+    *workspace_bytes = need;
+    return TCU_OK;
+  }
+  if (int rc = check_workspace(w, workspace, *workspace_bytes, need)) return rc;
+  if (M == 0 || N == 0) return TCU_OK;
+  const bool use_c = s->beta != 0.0f;
+  if (use_c && !C) return report_failure(TCU_ERR_INVALID_ARG, w + ": beta without d_C");
+  bool whole = N % 8 == 0, whole_inner = K % 8 == 0;
+  if (K)
+    if (int rc = check_matrix(w, "d_A", A, lda, M, K, s->dtype, &whole_inner)) return rc;
+  if (K)
+    if (int rc = check_matrix(w, "d_B", B, ldb, N, K, s->dtype, &whole_inner)) return rc;
+  if (int rc = check_matrix(w, "d_D", D, ldd, M, N, s->dtype, &whole)) return rc;
+  if (int rc = use_c ? check_matrix(w, "d_C", C, ldc, M, N, s->dtype, &whole) : TCU_OK) return rc;
+  if (int rc = Z ? check_matrix(w, "d_Z", Z, ldz, M, N, s->dtype, &whole) : TCU_OK) return rc;
+  if (int rc = check_vector(w, "d_bias", bias, 2, &whole)) return rc;
+  if (D == A || D == B || D == Z || (Z && (Z == A || Z == B || (use_c && Z == C)))) return report_failure(TCU_ERR_INVALID_ARG, w + ": an output in the place of an operand other tiles still read, or of another output");
+  char *at = static_cast<char *>(workspace) + g.share_bytes;
+  FusedGemmParams p{};
+  p.A = A;
+  p.lda = lda;
+  if (pack_a) {
+    pack_rows(A, lda, at, ldk, M, K, stream);
+    p.A = at;
+    p.lda = ldk;
+    at += a_bytes;
+  }
+  p.B = B;
+  p.ldb = ldb;
+  if (pack_b) {
+    pack_rows(B, ldb, at, ldk, N, K, stream);
+    p.B = at;
+    p.ldb = ldk;
+  }
+  p.bias = bias;
+  p.C = use_c ? C : nullptr;
+  p.ldc = ldc;
+  p.D = D;
+  p.ldd = ldd;
+  p.Z = Z;
+  p.ldz = ldz;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.beta = s->beta;
+  p.act = s->activation;
+  run_gemm(s->dtype, whole, g, p, static_cast<float *>(workspace), whole_inner, stream);
+  return TCU_OK;
+}
+
+// transpose (and, with Z or for its column sums, activation gradient) of rows x columns elements
+template <bool GRAD>
+inline void run_transpose(int dtype, TransposeParams q, void *stream) {
+  q.column_tiles = (unsigned)((q.columns + 63) / 64);
+  const unsigned grid = (unsigned)((q.rows + 63) / 64 * q.column_tiles);
+  if (dtype == TCU_F16 || !GRAD) launch(transpose_kernel<kF16, GRAD>, grid, 256u, stream, q);  // bits move as they are
+  else launch(transpose_kernel<kBF16, GRAD>, grid, 256u, stream, q);
+}
+
+inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const void *dD, size_t lddd, const void *A, size_t lda, const void *B, size_t ldb, const void *Z, size_t ldz, void *dA, size_t ldda,
+                                        void *dB, size_t lddb, float *dbias, void *workspace, size_t *workspace_bytes, void *stream) {
+  const std::string w("tcu_fused_gemm_backward");
+  if (int rc = check_gemm_shape(w, s)) return rc;
+  const size_t M = s->M, N = s->N, K = s->K;
+  if (M > kGemmMaxInner || N > kGemmMaxInner) return report_failure(TCU_ERR_UNSUPPORTED, w + ": M or N above 2^22");
+  for (auto mn : {std::make_pair(M, N), std::make_pair(M, K), std::make_pair(N, K)})
+    if (int rc = check_gemm_grid(w, mn.first, mn.second)) return rc;
+  const bool act = s->activation != TCU_ACT_NONE;
+  if (act && !Z) return report_failure(TCU_ERR_INVALID_ARG, w + ": the gradient of an activation needs d_Z");
+  const size_t ldm = up_to(M, 8), ldn = up_to(N, 8);
+  const GemmPlan ga = plan_gemm(M, K, N), gb = plan_gemm(N, K, M);
+  // the gradient of the activation's argument: dD itself where there is no activation and its rows are ready
+  const bool own_dz = dA && (act || !rows_ready(dD, M > 1 ? lddd : 8));
+  const size_t dz_bytes = own_dz ? part_bytes(M * ldn * 2) : 0, dzt_bytes = dB ? part_bytes(N * ldm * 2) : 0, at_bytes = dB ? part_bytes(K * ldm * 2) : 0, bt_bytes = dA ? part_bytes(K * ldn * 2) : 0;
+  const size_t strips = (M + 63) / 64, sums_bytes = dbias ? part_bytes(strips * N * 4) : 0;
+  const size_t share_bytes = (dA ? ga.share_bytes : 0) > (dB ? gb.share_bytes : 0) ? ga.share_bytes : (dB ? gb.share_bytes : 0);
+  const size_t bytes = share_bytes + dz_bytes + dzt_bytes + at_bytes + bt_bytes + sums_bytes, need = bytes < 256 ? 256 : bytes;
+  if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
+  if (!workspace) {
+    *workspace_bytes = need;
+    return TCU_OK;
+  }
+  if (int rc = check_workspace(w, workspace, *workspace_bytes, need)) return rc;
+  bool ignored = true, whole_a = K % 8 == 0, whole_b = K % 8 == 0;
+  if (M && N)
+    if (int rc = check_matrix(w, "d_dD", dD, lddd, M, N, s->dtype, &ignored)) return rc;
+  if (M && N && act)
+    if (int rc = check_matrix(w, "d_Z", Z, ldz, M, N, s->dtype, &ignored)) return rc;
+  if (dB && M && K)
+    if (int rc = check_matrix(w, "d_A", A, lda, M, K, s->dtype, &ignored)) return rc;
+  if (dA && N && K)
+    if (int rc = check_matrix(w, "d_B", B, ldb, N, K, s->dtype, &ignored)) return rc;
+  if (dA && M && K)
+    if (int rc = check_matrix(w, "d_dA", dA, ldda, M, K, s->dtype, &whole_a)) return rc;
+  if (dB && N && K)
+    if (int rc = check_matrix(w, "d_dB", dB, lddb, N, K, s->dtype, &whole_b)) return rc;
+  if (int rc = check_vector(w, "d_dbias", dbias, 4, &ignored)) return rc;
+  if ((dA && (dA == dD || dA == A || dA == B || dA == Z || dA == dB)) || (dB && (dB == dD || dB == A || dB == B || dB == Z)))
+    return report_failure(TCU_ERR_INVALID_ARG, w + ": a gradient in the place of an operand, or of another gradient");
+  char *at = static_cast<char *>(workspace) + share_bytes;
+  auto take = [&](size_t n) {
+    char *q = at;
+    at += n;
+    return static_cast<void *>(q);
+  };
+  void *dz = take(dz_bytes), *dzt = take(dzt_bytes), *a_t = take(at_bytes), *b_t = take(bt_bytes);
+  float *sums = static_cast<float *>(take(sums_bytes));
+  float *shares = static_cast<float *>(workspace);
+  if (M && N && (own_dz || dB || dbias)) {
+    TransposeParams q{};
+    q.from = dD;
+    q.from_ld = lddd;
+    q.Z = act ? Z : nullptr;
+    q.z_ld = ldz;
+    q.to = dB ? dzt : nullptr;
+    q.to_ld = ldm;
+    q.dz = own_dz ? dz : nullptr;
+    q.dz_ld = ldn;
+    q.partial = dbias ? sums : nullptr;
+    q.rows = M;
+    q.columns = N;
+    q.act = s->activation;
+    run_transpose<true>(s->dtype, q, stream);
+  }
+  if (dbias && N) {
+    ColumnSumParams q{};
+    q.partial = sums;
+    q.out[0] = dbias;
+    q.parts = strips;
+    q.columns = (unsigned)N;
+    q.vectors = 1;
+    launch(column_sum_kernel, (unsigned)((N + 63) / 64), 64u * kColumnSumWaves, stream, q);
+  }
+  FusedGemmParams p{};
+  p.act = TCU_ACT_NONE;
+  p.N = K;
+  if (dA && M && K) {
+    if (N) {
+      TransposeParams q{};
+      q.from = B;
+      q.from_ld = ldb;
+      q.to = b_t;
+      q.to_ld = ldn;
+      q.rows = N;
+      q.columns = K;
+      run_transpose<false>(s->dtype, q, stream);
+    }
+    p.A = own_dz ? dz : dD;
+    p.lda = own_dz ? ldn : lddd;
+    p.B = b_t;
+    p.ldb = ldn;
+    p.D = dA;
+    p.ldd = ldda;
+    p.M = M;
+    p.K = N;
+    run_gemm(s->dtype, whole_a, ga, p, shares, N % 8 == 0, stream);
+  }
+  if (dB && N && K) {
+    if (M) {
+      TransposeParams q{};
+      q.from = A;
+      q.from_ld = lda;
+      q.to = a_t;
+      q.to_ld = ldm;
+      q.rows = M;
+      q.columns = K;
+      run_transpose<false>(s->dtype, q, stream);
+    }
+    p.A = dzt;
+    p.lda = ldm;
+    p.B = a_t;
+    p.ldb = ldm;
+    p.D = dB;
+    p.ldd = lddb;
+    p.M = N;
+    p.K = M;
+    run_gemm(s->dtype, whole_b, gb, p, shares, M % 8 == 0, stream);
+  }
+  return TCU_OK;
+}
+
+}  // namespace tcu

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "checks.hpp"
+#include "column_sum.hpp"
 #include "fused_norm.hpp"
 #include "launch.hpp"
 

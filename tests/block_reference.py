@@ -198,3 +198,33 @@ def norm_backward(kind, order, name, dout, z, gate, weight, bias, scale, eps, x,
         dz, edz = scale * dz, np.abs(scale) * (edz + 2 * EPS32 * np.abs(dz))
     got["dx"], err["dx"] = dz, edz
     return got, err
+
+
+# ---- product ----------------------------------------------------------------------------------------------------
+
+
+def product(A, B, bias, name, C, beta):
+    """(D, Z, bound on D, on Z) of D = act(A B^T + bias) + beta C; B as N rows of K.  A sum of K products in any order is off by at
+    most 2 K 2^-24 times the sum of their magnitudes (two roundings an addition: the matrix unit's own and the accumulator's)."""
+    k = A.shape[1]
+    z = A @ B.T + bias
+    ez = (2 * k + 8) * EPS32 * (np.abs(A) @ np.abs(B).T) + 2 * EPS32 * (np.abs(z) + np.abs(bias))
+    f, _, c = act(name, z)
+    d = f + (beta * C if C is not None else 0.0)
+    steepest = 1.2  # no activation's slope is above it
+    ed = steepest * ez + (c + 2) * EPS32 * np.abs(f) + 2 * EPS32 * (np.abs(d) + (np.abs(beta * C) if C is not None else 0.0))
+    return d, z, ed, ez
+
+
+def product_backward(dD, A, B, Z, name, dtype):
+    """dict of gradients and of bounds; dZ is rounded to `dtype` in front of the products."""
+    _, slope, c = act(name, Z) if Z is not None else (None, np.ones_like(dD), np.zeros_like(dD))
+    mag = 1.0 + np.abs(Z) if Z is not None and name != "relu" else np.abs(slope)
+    dz = dD * slope
+    e = (3 * c + 8) * EPS32 * np.abs(dD) * mag if Z is not None else np.zeros_like(dD)
+    er = e + U[dtype] * (np.abs(dz) + e) + TINY[dtype] if Z is not None else e
+    m, n = dD.shape
+    got = {"dA": dz @ B, "dB": dz.T @ A, "dbias": dz.sum(0)}
+    err = {"dA": er @ np.abs(B) + (2 * n + 8) * EPS32 * ((np.abs(dz) + er) @ np.abs(B)), "dB": er.T @ np.abs(A) + (2 * m + 8) * EPS32 * ((np.abs(dz) + er).T @ np.abs(A)),
+           "dbias": e.sum(0) + (m + 8) * EPS32 * np.abs(dz).sum(0)}
+    return got, err

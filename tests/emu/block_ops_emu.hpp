@@ -26,5 +26,32 @@ inline uint16_t bf16_bits(float v) {
 }
 inline unsigned pack_bf16x2(float lo, float hi) { return (unsigned)bf16_bits(lo) | ((unsigned)bf16_bits(hi) << 16); }
 
+template <bool BF16>
+inline float4_t mfma_16x16x32_chunks(uint4_t a, uint4_t b, float4_t c) {
+  auto &w = my_wave();
+  const int lane = lane_id();
+  memcpy(&w.slot[lane][0], &a, 16);
+  memcpy(&w.slot[lane][4], &b, 16);
+  emu::wave_sync();
+  auto value = [](const uint32_t *words, int e) {
+    const uint16_t h = (uint16_t)(words[e / 2] >> (16 * (e % 2)));
+    if (BF16) return __uint_as_float((unsigned)h << 16);
+    half_t v;
+    memcpy(&v, &h, 2);
+    return (float)v;
+  };
+  float4_t d = c;
+  const int n = lane & 15;
+  for (int i = 0; i < 4; i++) {
+    const int m = 4 * (lane >> 4) + i;
+    float acc = 0.0f;
+    for (int kb = 0; kb < 4; kb++)
+      for (int e = 0; e < 8; e++) acc += value(&w.slot[16 * kb + m][0], e) * value(&w.slot[16 * kb + n][4], e);
+    d[i] += acc;
+  }
+  emu::wave_sync();
+  return d;
+}
+
 }  // namespace tcu
 #endif  // TCU_BLOCK_OPS_HPP

@@ -536,3 +536,158 @@ def test_fused_norm_refusals(emu):
     assert back(dw=p + 2) == 1 and "d_dweight" in err()
     need = sz(0)
     assert back(ws=None, have=need, dw=p) == 0 and need.value == 256
+
+
+# ---- fused product ----------------------------------------------------------------------------------------------
+
+
+class GemmShape(ctypes.Structure):
+    _fields_ = [("dtype", ci), ("activation", ci), ("M", sz), ("N", sz), ("K", sz), ("beta", cf)]
+
+
+def gemm_emu(emu):
+    shape, psz, m = ctypes.POINTER(GemmShape), ctypes.POINTER(sz), [vp, sz]
+    emu.emu_fused_gemm.argtypes = [shape, *m * 2, vp, *m * 3, vp, psz]
+    emu.emu_fused_gemm_backward.argtypes = [shape, *m * 6, vp, vp, psz]
+    emu.emu_fused_gemm_tiles.argtypes = [ci, ctypes.c_uint, ci, ci, sz, sz, sz, cf, *m * 2, vp, *m * 3, vp]
+    return emu
+
+
+def gemm_operands(rng, dtype, M, N, K, with_bias, with_c):
+    f = lambda v: ref.to_f64(ref.to_bits(v, dtype), dtype)
+    A, B = f(rng.standard_normal((M, K))), f(rng.standard_normal((N, K)) / max(K, 1) ** 0.5)
+    return A, B, f(rng.standard_normal(N)) if with_bias else None, f(rng.standard_normal((M, N))) if with_c else None
+
+
+# M, N, K, gap of the operands' rows, activation, bias, C, Z
+GEMMS = [
+    (1, 1, 1, 0, "none", False, False, False),
+    (1, 40, 0, 0, "silu", True, True, True),
+    (3, 17, 100, 0, "gelu", True, True, False),
+    (5, 64, 1032, 8, "none", True, True, False),
+    (16, 33, 2100, 0, "relu", False, False, True),
+    (20, 24, 72, 1, "sigmoid", True, False, True),
+    (64, 16, 4160, 0, "silu", True, True, True),
+    (65, 136, 64, 0, "silu", True, True, True),
+    (70, 130, 200, 8, "gelu", True, False, True),
+    (129, 40, 37, 0, "none", False, True, False),
+    (66, 9, 1100, 3, "sigmoid", True, True, False),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("case", GEMMS, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}-{c[4]}")
+def test_fused_gemm(emu, dtype, case):
+    M, N, K, gap, name, with_bias, with_c, with_z = case
+    emu = gemm_emu(emu)
+    rng = np.random.default_rng(M * 7 + N)
+    A, B, bias, C = gemm_operands(rng, dtype, M, N, K, with_bias, with_c)
+    mA, mB = Matrix(A, dtype, K + gap) if K else None, Matrix(B, dtype, K + 2 * gap) if K else None
+    mD, mZ = Matrix(np.zeros((M, N)), dtype, N + gap), Matrix(np.zeros((M, N)), dtype) if with_z else None
+    mC = Matrix(C, dtype, N + gap) if with_c else None
+    vb = vector(bias, dtype) if with_bias else None
+    beta = 0.5 if with_c else 0.0
+    s = GemmShape(DTYPES[dtype], ACTS[name], M, N, K, beta)
+    run = lambda out: (lambda call: (lambda kept, ws, have: call(ws, ctypes.byref(have)))(*workspace_for(call)))(
+        lambda ws, need: emu.emu_fused_gemm(ctypes.byref(s), *operand(mA), *operand(mB), vb.ctypes.data if with_bias else None, *operand(mC), *operand(out), *operand(mZ), ws, need))
+    assert run(mD) == 0, emu.emu_last_error()
+    d, z, ed, ez = ref.product(A, B, bias if with_bias else np.zeros(N), name, C, beta)
+    ref.check(mD.get(), d, ed, dtype, "D")
+    assert mD.untouched_between()
+    if with_z:
+        ref.check(mZ.get(), z, ez, dtype, "Z")
+    if with_c:
+        assert run(mC) == 0
+        assert (mC.get() == mD.get()).all() and mC.untouched_between()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("w8,splits,M,N,K", [(4, 1, 130, 250, 136), (4, 3, 140, 100, 330), (8, 1, 300, 257, 208), (8, 2, 256, 40, 61), (8, 1, 33, 300, 448), (4, 5, 100, 30, 128)])
+def test_fused_gemm_tiles(emu, dtype, w8, splits, M, N, K):
+    emu = gemm_emu(emu)
+    rng = np.random.default_rng(M)
+    A, B, bias, C = gemm_operands(rng, dtype, M, N, K, True, True)
+    ld = (K + 7) // 8 * 8
+    mA, mB, mC, mD, mZ = Matrix(A, dtype, ld), Matrix(B, dtype, ld + 8), Matrix(C, dtype), Matrix(C, dtype, N + 3), Matrix(C, dtype)
+    vb = vector(bias, dtype)
+    shares = floats(np.full(splits * M * ((N + 7) // 8 * 8), np.nan))
+    emu.emu_fused_gemm_tiles(w8, splits, DTYPES[dtype], ACTS["silu"], M, N, K, 0.5, *operand(mA), *operand(mB), vb.ctypes.data, *operand(mC), *operand(mD), *operand(mZ), shares.ctypes.data)
+    d, z, ed, ez = ref.product(A, B, bias, "silu", C, 0.5)
+    ref.check(mD.get(), d, ed, dtype, "D")
+    ref.check(mZ.get(), z, ez, dtype, "Z")
+    assert mD.untouched_between()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,gap,name", [(1, 1, 1, 0, "silu"), (70, 100, 72, 0, "silu"), (130, 8, 65, 1, "gelu"), (9, 67, 130, 0, "none"), (100, 16, 24, 3, "none"), (40, 80, 16, 8, "sigmoid"), (0, 5, 9, 0, "relu"), (66, 70, 68, 0, "relu")])
+def test_fused_gemm_gradient(emu, dtype, M, N, K, gap, name):
+    emu = gemm_emu(emu)
+    rng = np.random.default_rng(M + N)
+    f = lambda v: ref.to_f64(ref.to_bits(v, dtype), dtype)
+    A, B, _, _ = gemm_operands(rng, dtype, M, N, K, False, False)
+    dD, Z = f(rng.standard_normal((M, N))), f(rng.standard_normal((M, N))) if name != "none" else None
+    mA, mB, mD, mZ = Matrix(A, dtype, K + gap), Matrix(B, dtype, K + gap), Matrix(dD, dtype, N + gap), Matrix(Z, dtype) if name != "none" else None
+    dA, dB, db = Matrix(np.full((M, K), 5.0), dtype), Matrix(np.full((N, K), 5.0), dtype), floats(np.full(N, 9.0))
+    s = GemmShape(DTYPES[dtype], ACTS[name], M, N, K, 0.0)
+    got, err = ref.product_backward(dD, A, B, Z, name, dtype)
+    for wanted in ("AB+", "A", "B", "+"):
+        call = lambda ws, need: emu.emu_fused_gemm_backward(ctypes.byref(s), *operand(mD), *operand(mA), *operand(mB), *operand(mZ), *(operand(dA) if "A" in wanted else NULL), *(operand(dB) if "B" in wanted else NULL),
+                                                            db.ctypes.data if "+" in wanted else None, ws, need)
+        dA.put(np.full((M, K), 5.0))
+        dB.put(np.full((N, K), 5.0))
+        kept, ws, have = workspace_for(call)
+        assert call(ws, ctypes.byref(have)) == 0, emu.emu_last_error()
+        if "A" in wanted:
+            ref.check(dA.get(), got["dA"], err["dA"], dtype, "dA")
+        if "B" in wanted:
+            ref.check(dB.get(), got["dB"], err["dB"], dtype, "dB")
+        if "+" in wanted:
+            ref.check(db[:N], got["dbias"], err["dbias"], "f32", "dbias")
+
+
+def test_product_gradient_against_differences():
+    rng = np.random.default_rng(4)
+    for name in ACTS:
+        A, B, bias, dD = rng.standard_normal((3, 4)), rng.standard_normal((5, 4)), rng.standard_normal(5), rng.standard_normal((3, 5))
+        loss = lambda A, B, bias: float((ref.product(A, B, bias, name, None, 0.0)[0] * dD).sum())
+        got, _ = ref.product_backward(dD, A, B, A @ B.T + bias, name, "f32")
+        args = [A, B, bias]
+        for k, key in enumerate(("dA", "dB", "dbias")):
+            for at in itertools.product(*(range(n) for n in args[k].shape)):
+                lo, hi = [v.copy() for v in args], [v.copy() for v in args]
+                lo[k][at] -= 1e-5
+                hi[k][at] += 1e-5
+                assert abs((loss(*hi) - loss(*lo)) / 2e-5 - got[key][at]) < 1e-7, (name, key)
+
+
+def test_fused_gemm_refusals(emu):
+    emu = gemm_emu(emu)
+    buf = aligned(1 << 16, np.uint8, 0)
+    p = buf.ctypes.data
+    ws0 = p // 256 * 256 + 32768
+    err = lambda: emu.emu_last_error().decode()
+    big = sz(1 << 40)
+    m = lambda k: (p + 1024 * k, 8)
+    ok = dict(dtype=0, activation=0, M=2, N=8, K=8, beta=0.0)
+
+    def fwd(A=m(0), B=m(1), bias=None, C=NULL, D=m(2), Z=NULL, ws=ws0, have=big, **k):
+        return emu.emu_fused_gemm(ctypes.byref(GemmShape(**{**ok, **k})), *A, *B, bias, *C, *D, *Z, ws, ctypes.byref(have) if have else None)
+
+    assert emu.emu_fused_gemm(None, *NULL, *NULL, None, *NULL, *NULL, *NULL, None, None) == 1 and "null shape" in err()
+    assert fwd(dtype=2) == 1 and "dtype" in err()
+    assert fwd(activation=9) == 1 and "activation" in err()
+    assert fwd(K=(1 << 22) + 1) == 2 and fwd(M=1 << 31) == 2 and fwd(M=1 << 30, N=1 << 30) == 2
+    assert fwd(have=None) == 1 and fwd(have=sz(16)) == 4 and fwd(ws=ws0 + 8) == 1
+    assert fwd(beta=1.0) == 1 and "beta without d_C" in err()
+    assert fwd(A=(None, 8)) == 1 and "d_A" in err()
+    assert fwd(B=(p, 7)) == 1 and "overlap" in err()
+    assert fwd(D=(p + 1, 8)) == 1 and "aligned" in err()
+    assert fwd(D=m(0)) == 1 and fwd(D=m(1)) == 1 and fwd(Z=m(2)) == 1 and fwd(Z=m(1)) == 1 and "in the place" in err()
+    assert fwd(C=m(3), Z=m(3), beta=1.0) == 1
+    assert fwd(bias=p + 1) == 1 and "d_bias" in err()
+    assert fwd(M=0, A=NULL, D=NULL) == 0
+    back = lambda dA=m(4), dB=m(5), Z=NULL, db=None, **k: emu.emu_fused_gemm_backward(ctypes.byref(GemmShape(**{**ok, **k})), *m(0), *m(1), *m(2), *Z, *dA, *dB, db, ws0, ctypes.byref(big))
+    assert back(activation=3) == 1 and "needs d_Z" in err()
+    assert back(M=(1 << 22) + 1) == 2
+    assert back(dA=m(0)) == 1 and back(dA=m(5)) == 1 and back(dB=m(1)) == 1 and "in the place" in err()
+    assert back(db=p + 2) == 1 and "d_dbias" in err()
