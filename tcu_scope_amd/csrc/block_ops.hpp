@@ -1,5 +1,5 @@
 // What the recurrent-block operators (gated scan, fused norm, fused matrix product) use beyond wave_ops.hpp: element
-// types behind a 16-byte chunk, the transcendental instructions, cross-lane reads by lane number.
+// types behind a 16-byte chunk, the transcendental instructions, lane exchanges.
 //
 // A chunk is 16 bytes of one row: 8 elements of 16 bits or 4 of 32.  Everything is computed in fp32; the one rounding to
 // 16 bits is the conversion of a result to the type its tensor has (to nearest even).
@@ -15,8 +15,26 @@ TCU_DEVICE float hw_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 TCU_DEVICE float hw_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 TCU_DEVICE float hw_rsqrt(float x) { return __builtin_amdgcn_rsqf(x); }
 
-// value of `x` in lane `l` (may differ from lane to lane)
-TCU_DEVICE float read_lane_of(float x, int l) { return __int_as_float(__builtin_amdgcn_ds_bpermute(l << 2, __float_as_int(x))); }
+// With lo = hi = x: lo becomes x of the lane without bit D in its number, hi x of the lane with it (D = 16 or 32)
+template <int D>
+TCU_DEVICE void swap_halves(unsigned &lo, unsigned &hi) {
+  if constexpr (D == 16) permlane16_swap(lo, hi);
+  else permlane32_swap(lo, hi);
+}
+
+// 16 bytes at a 32-bit offset from a base that is the same for the whole wave (which then stays in scalar registers).
+// WHOLE: 16-byte aligned; otherwise at any element's address.
+typedef unsigned any_chunk_t __attribute__((ext_vector_type(4), aligned(2)));
+template <bool WHOLE>
+TCU_DEVICE uint4_t load_at(const char *base, unsigned offset) {
+  if constexpr (WHOLE) return __builtin_nontemporal_load(reinterpret_cast<const uint4_t *>(base + offset));
+  return *reinterpret_cast<const any_chunk_t *>(base + offset);
+}
+template <bool WHOLE>
+TCU_DEVICE void store_at(char *base, unsigned offset, uint4_t v) {
+  if constexpr (WHOLE) __builtin_nontemporal_store(v, reinterpret_cast<uint4_t *>(base + offset));
+  else *reinterpret_cast<any_chunk_t *>(base + offset) = v;
+}
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 TCU_DEVICE unsigned pack_bf16x2(float lo, float hi) {

@@ -64,7 +64,6 @@ TCU_DEVICE uint4_t pack_chunk(const float (&v)[Elem<DT>::V]) {
 // The chunk at element `at` of p, of which `count` elements exist (count <= 0: none; the others read as 0).
 // WHOLE: count is at most 0 or at least V, and p + at is 16-byte aligned.  Otherwise a whole chunk is still one access
 // (the hardware takes 16-byte accesses at any element's address), and a part of one is read element by element.
-typedef unsigned any_chunk_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef float any_floats_t __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int DT, bool WHOLE, bool NT = true>

@@ -17,19 +17,22 @@
 // array), channels are contiguous.  Both directions run in one order of "places" 0, 1, ...: place p is row p forwards and
 // row rows-1-p backwards.
 //
-// One pass over the data: a block takes a tile of TILE_ROWS places x TILE_CHANNELS channels into registers (a thread has
-// RPT consecutive places of one 16-byte chunk of channels), works out the (A, B) of each thread's places, the carry into
-// each thread from those in LDS, and finishes from registers.  The bound is HBM traffic (2 streams in, 1 out; backwards
-// 3 or 4 in, 2 out); exponential and reciprocal are quarter-rate instructions, so a and b are worked out once and kept.
+// One pass over the data: a block takes a tile of TILE_ROWS places x TILE_CHANNELS channels into registers.  A thread has
+// RPT consecutive places of one 16-byte chunk of channels and works out their (a, b) once (exponential and reciprocal are
+// quarter-rate instructions) and the (A, B) of all of them; the groups of a wave combine theirs by lane exchanges, the waves
+// in LDS; from the state in front of the tile every thread finishes from registers.  The bound is HBM traffic (2 streams in,
+// 1 out; backwards 3 or 4 in, 2 out).
 //
-// Tiles that follow each other along the sequences hand the state on through descriptors in the workspace, two 64-bit
-// words per channel, each a tag with a value, so that a word is whole whenever it is seen and needs no fence.  A tile
-// publishes either its aggregate (A, B), as soon as it has read its input, or the state behind it; which of the two is
-// settled by its place alone: the state where a sequence begins inside the tile (nothing from in front is needed) and at
-// every kGroupTiles-th tile; so a tile waits for its group's aggregates, which wait for nothing, and for one state, and
-// combines them in one fixed order: the same input gives the same bits every time, and the chain of waits is a
-// kGroupTiles-th of the tiles.  Tiles are handed out by a ticket, so the one that is waited for has always been started;
-// a wait is bounded and leaves NaN in what depended on it.
+// Tiles that follow each other along the sequences hand the state on through entries in the workspace, one 64-bit word per
+// channel, whole whenever it is seen, so that no fence is needed: an aggregate (A, B), or a state.  Every tile publishes its
+// own aggregate, or, where a sequence begins inside it, the state behind it; every 8th tile the same for the 8 tiles it closes,
+// which wait for nothing but each other; every 64th tile the state behind it, which waits for the state 64 tiles before.  A
+// tile's carry is that state with at most 7 entries of 8 tiles and 7 entries of one tile applied in their order.  What is
+// published and in which order it is combined depends on places alone, never on timing: the same input gives the same bits
+// every time.  The chain of waits is a 64th of the tiles long (every 8th tile handing a state on, with 512 tiles along a
+// sequence: 65536 x 2048 fp16, 390 us; waits left out 264 us).
+// Tiles are handed out by a ticket, so the one that is waited for has always been started; a wait is bounded and leaves NaN
+// in what depended on it.
 #pragma once
 
 #include "elements.hpp"
@@ -37,7 +40,7 @@
 namespace tcu {
 
 constexpr int kGateDecay = 0, kGateLog = 1, kGateSigmoid = 2;  // tcu_gate
-constexpr unsigned kScanGroupTiles = 8;
+constexpr unsigned kScanGroup = 8;  // tiles that share an entry, and entries under one state
 
 struct GatedScanParams {
   const void *x, *g, *h, *dh;  // x: also the input of the sigmoid gate's gradient; h: backwards only
@@ -48,17 +51,33 @@ struct GatedScanParams {
   const int *row_sequence;     // sequence of each row, -1 outside all; null: sequence_rows rows each
   size_t x_stride, g_stride, h_stride, dh_stride, out_stride, out_g_stride;  // elements from row to row
   unsigned rows, sequence_rows, channels, strips, chunks;
+  bool near_rows;                  // 64 rows of any matrix lie within 4 GiB
   bool zero_outside;               // rows of no sequence: their outputs become 0, or are left as they are
   unsigned *ticket;                // null: one chunk of places, the block index is the tile
-  unsigned long long *descriptors; // [chunk][strip][channel of the tile][2]
+  unsigned long long *entries;     // [chunks + chunks / 8 + chunks / 64][strip][channel of the tile]
   unsigned poll_limit, mute_tile;  // mute_tile: tests only, tile mute_tile - 1 publishes nothing
   unsigned *expired;
 };
 
-constexpr unsigned kDescAggregate = 1, kDescState = 2;
-TCU_DEVICE unsigned long long tagged(unsigned tag, float v) { return ((unsigned long long)tag << 32) | __float_as_uint(v); }
-TCU_DEVICE unsigned tag_of(unsigned long long w) { return (unsigned)(w >> 32); }
-TCU_DEVICE float value_of(unsigned long long w) { return __uint_as_float((unsigned)w); }
+// An entry: (A, B) as two fp32 words, or a state with kIsState in the place of A; kNoEntry before it is published.  Both marks
+// are NaNs that no A carries: a NaN is published as the one the hardware makes.
+constexpr unsigned kIsState = 0xfffffffeu, kQuietNaN = 0x7fc00000u;
+constexpr unsigned long long kNoEntry = ~0ull;
+TCU_DEVICE unsigned published_bits(float v) { return v != v ? kQuietNaN : __float_as_uint(v); }
+TCU_DEVICE unsigned long long entry_of(bool is_state, float A, float B) { return ((unsigned long long)published_bits(B) << 32) | (is_state ? kIsState : published_bits(A)); }
+
+// (A, B), then an entry's step: a state replaces what came before it
+struct ScanStep {
+  float A, B;
+  bool is_state;
+};
+TCU_DEVICE void apply_entry(ScanStep &s, unsigned long long w) {
+  const bool state = (unsigned)w == kIsState;
+  const float A = __uint_as_float((unsigned)w), B = __uint_as_float((unsigned)(w >> 32));
+  s.B = state ? B : __builtin_fmaf(A, s.B, B);
+  s.A = state ? 0.0f : A * s.A;
+  s.is_state = s.is_state || state;
+}
 
 template <int DT, int GATE>
 TCU_DEVICE void gate_of(float g, float *a, float *keep) {  // keep = 1 - a (sigmoid only)
@@ -68,76 +87,124 @@ TCU_DEVICE void gate_of(float g, float *a, float *keep) {  // keep = 1 - a (sigm
   if constexpr (GATE == kGateSigmoid) sigmoid_pair<DT == kF32>(g, a, keep);
 }
 
-// The carry into this tile for channel `c` of it; the tile's own aggregate is (A, B).  One thread per channel.
-//   own_state: a sequence begins in the tile, so B is the state behind it whatever came in front
+// Reads those of the first `count` entries that have not been seen published yet; true if all have.
+TCU_DEVICE bool read_entries(const unsigned long long *first, size_t stride, unsigned count, unsigned long long (&w)[kScanGroup]) {
+#pragma unroll
+  for (unsigned j = 0; j < kScanGroup; j++)
+    if (j < count && w[j] == kNoEntry) w[j] = atomic_load_u64(first + j * stride);
+  bool all = true;
+#pragma unroll
+  for (unsigned j = 0; j < kScanGroup; j++) all = all && !(j < count && w[j] == kNoEntry);
+  return all;
+}
+
+// The carry into this tile for channel `c` of it; the tile's own step is `own`.  One thread per channel.
 //   needs: the tile's first place continues a sequence
-TCU_DEVICE float exchange_carry(const GatedScanParams &p, unsigned chunk, unsigned strip, int tile_channels, int c, float A, float B, bool own_state, bool needs) {
-  const size_t stride = (size_t)p.strips * tile_channels * 2;  // words from chunk to chunk
-  unsigned long long *mine = p.descriptors + ((size_t)chunk * p.strips + strip) * tile_channels * 2 + 2 * c;
+TCU_DEVICE float exchange_carry(const GatedScanParams &p, unsigned chunk, unsigned strip, int tile_channels, int c, const ScanStep &own, bool needs) {
+  constexpr unsigned G = kScanGroup;
+  const size_t stride = (size_t)p.strips * tile_channels;  // from chunk to chunk
+  unsigned long long *tiles = p.entries + (size_t)strip * tile_channels + c;
+  unsigned long long *groups = tiles + (size_t)p.chunks * stride, *states = groups + (size_t)(p.chunks / G) * stride;
+  const unsigned group = chunk / G, in_group = chunk % G, super = group / G, in_super = group % G;
+  const bool closes_group = in_group == G - 1, closes_super = closes_group && in_super == G - 1;
   const bool muted = p.mute_tile != 0 && chunk * p.strips + strip == p.mute_tile - 1;
-  const bool closes_group = chunk % kScanGroupTiles == kScanGroupTiles - 1;
-  if (own_state && !muted) {
-    atomic_store_u64(mine, tagged(kDescState, B));
-  } else if (!closes_group && !muted) {
-    atomic_store_u64(mine, tagged(kDescAggregate, A));
-    atomic_store_u64(mine + 1, tagged(kDescAggregate, B));
+  if (!closes_group && !muted) atomic_store_u64(tiles + chunk * stride, entry_of(own.is_state, own.A, own.B));
+  if (!needs && !closes_group) return 0.0f;
+  // everything this tile may have to know is asked for at once (one wait on memory instead of three)
+  const unsigned long long *tile0 = tiles + (size_t)group * G * stride, *group0 = groups + (size_t)super * G * stride, *state0 = states + (size_t)(super > 0 ? super - 1 : 0) * stride;
+  const unsigned tile_count = !own.is_state || needs ? in_group : 0u, group_count = needs ? in_super : 0u, state_count = needs && super > 0 ? 1u : 0u;
+  unsigned long long w[G], v[G], u[G];
+#pragma unroll
+  for (unsigned j = 0; j < G; j++) w[j] = v[j] = u[j] = kNoEntry;
+  bool have_tiles = read_entries(tile0, stride, tile_count, w), have_states = read_entries(state0, stride, state_count, u), have_groups = read_entries(group0, stride, group_count, v);
+  unsigned polls = 0;
+  for (; !have_tiles && polls < p.poll_limit; polls++) {
+    spin_pause();
+    have_tiles = read_entries(tile0, stride, tile_count, w);
+  }
+  ScanStep front{1.0f, 0.0f, false};  // the group's tiles in front of this one
+#pragma unroll
+  for (unsigned j = 0; j < G; j++)
+    if (j < tile_count) apply_entry(front, w[j]);
+  const float bad = __builtin_nanf("");
+  if (closes_group && !closes_super && !muted) {
+    const float B = own.is_state ? own.B : __builtin_fmaf(own.A, front.B, own.B);
+    const bool known = have_tiles || own.is_state;
+    atomic_store_u64(groups + (size_t)group * stride, entry_of(!known || own.is_state || front.is_state, own.A * front.A, known ? B : bad));
   }
   float carry = 0.0f;
   if (needs) {
-    // the group's tiles in front of this one, and the one that closed the group before
-    const unsigned in_group = chunk % kScanGroupTiles;
-    const unsigned count = in_group + (chunk >= kScanGroupTiles ? 1u : 0u);  // >= 1: the first tile of all begins a sequence
-    const unsigned long long *first = mine - (size_t)count * stride;
-    unsigned long long w0[kScanGroupTiles], w1[kScanGroupTiles];
-#pragma unroll
-    for (unsigned j = 0; j < kScanGroupTiles; j++) w0[j] = w1[j] = 0;
-    unsigned polls = 0;
-    bool waiting = true, gave_up = false;
-    while (waiting) {
-      waiting = false;
-#pragma unroll
-      for (unsigned j = 0; j < kScanGroupTiles; j++) {
-        if (j < count) {
-          if (tag_of(w0[j]) == 0) w0[j] = atomic_load_u64(first + j * stride);
-          if (tag_of(w1[j]) == 0 && tag_of(w0[j]) != kDescState) w1[j] = atomic_load_u64(first + j * stride + 1);
-        }
-      }
-#pragma unroll
-      for (unsigned j = 0; j < kScanGroupTiles; j++)
-        if (j < count && (tag_of(w0[j]) == 0 || (tag_of(w0[j]) == kDescAggregate && tag_of(w1[j]) == 0))) waiting = true;
-      if (waiting && polls++ >= p.poll_limit) {
-        gave_up = true;
-        break;
-      }
-      if (waiting) spin_pause();
+    const bool behind = have_tiles && !front.is_state;  // what lies in front of the group matters
+    for (; behind && !(have_states && have_groups) && polls < p.poll_limit; polls++) {
+      spin_pause();
+      have_states = read_entries(state0, stride, state_count, u);
+      have_groups = read_entries(group0, stride, group_count, v);
     }
+    ScanStep s{0.0f, state_count ? __uint_as_float((unsigned)(u[0] >> 32)) : 0.0f, true};
 #pragma unroll
-    for (unsigned j = 0; j < kScanGroupTiles; j++)
-      if (j < count) carry = tag_of(w0[j]) == kDescState ? value_of(w0[j]) : __builtin_fmaf(value_of(w0[j]), carry, value_of(w1[j]));
-    if (gave_up) {
-      carry = __builtin_nanf("");
+    for (unsigned j = 0; j < G; j++)
+      if (j < group_count) apply_entry(s, v[j]);
+    carry = front.is_state ? front.B : __builtin_fmaf(front.A, s.B, front.B);
+    if (!have_tiles || (behind && !(have_states && have_groups))) {
+      carry = bad;
       if (c == 0 && p.expired) atomic_add_u32(p.expired, 1u);
     }
   }
-  if (!own_state && closes_group && !muted) atomic_store_u64(mine, tagged(kDescState, __builtin_fmaf(A, carry, B)));
+  if (closes_super && !muted) atomic_store_u64(states + (size_t)super * stride, entry_of(true, 0.0f, own.is_state ? own.B : __builtin_fmaf(own.A, carry, own.B)));
   return carry;
+}
+
+// Combines the steps of the wave's groups of TCL lanes: on return (A, B, reset) is the step of all of them, and
+// (FA, FB, front_reset) that of the groups in front of the lane's own.  A lane exchange leaves the half in front in one
+// register and the half behind in the other, in every lane.  RESETS = false: no sequence begins in any of them.
+template <int TCL, int V, bool RESETS>
+TCU_DEVICE void combine_groups(float (&A)[V], float (&B)[V], unsigned &reset, float (&FA)[V], float (&FB)[V], unsigned &front_reset) {
+#pragma unroll
+  for (int e = 0; e < V; e++) {
+    FA[e] = 1.0f;
+    FB[e] = 0.0f;
+  }
+  front_reset = 0;
+  static_for<2>([&](auto step) {
+    constexpr int D = TCL << decltype(step)::value;
+    static_assert(D == 16 || D == 32, "groups of 16 lanes");
+    const bool upper = (lane_id() & D) != 0;
+    unsigned lo_reset = reset, hi_reset = reset;
+    if constexpr (RESETS) swap_halves<D>(lo_reset, hi_reset);
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      unsigned la = __float_as_uint(A[e]), ha = la, lb = __float_as_uint(B[e]), hb = lb;
+      swap_halves<D>(la, ha);
+      swap_halves<D>(lb, hb);
+      const float lA = __uint_as_float(la), hA = __uint_as_float(ha), lB = __uint_as_float(lb), hB = __uint_as_float(hb);
+      const float nB = RESETS && front_reset ? FB[e] : __builtin_fmaf(FA[e], lB, FB[e]), nA = RESETS && front_reset ? 0.0f : FA[e] * lA;
+      FB[e] = upper ? nB : FB[e];  // what lies in front of the group now begins with the other half
+      FA[e] = upper ? nA : FA[e];
+      B[e] = RESETS && hi_reset ? hB : __builtin_fmaf(hA, lB, hB);
+      A[e] = RESETS && hi_reset ? 0.0f : hA * lA;
+    }
+    if constexpr (RESETS) {
+      if (upper) front_reset |= lo_reset;
+      reset = lo_reset | hi_reset;
+    }
+  });
 }
 
 // TCL lanes share a row of the tile (TCL * V channels); blocks of THREADS threads, RPT places per thread.
 template <int DT, int GATE, bool BACK, bool ALIGNED, int TCL, int RPT, int THREADS>
 __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) {
-  constexpr int V = Elem<DT>::V, TC = TCL * V, GROUPS = THREADS / TCL, TILE_ROWS = GROUPS * RPT;
+  constexpr int V = Elem<DT>::V, TC = TCL * V, GROUPS = THREADS / TCL, TILE_ROWS = GROUPS * RPT, WAVES = THREADS / 64;
   static_assert(TC <= THREADS, "one thread per channel carries the state through the tile");
-  __shared__ __attribute__((aligned(16))) float lds_a[GROUPS * TC];
-  __shared__ __attribute__((aligned(16))) float lds_b[GROUPS * TC];
-  __shared__ unsigned lds_reset[GROUPS];  // bit 0: a sequence begins in the group, bit 1: it does so at the group's first place
+  __shared__ __attribute__((aligned(16))) float lds_a[WAVES * TC];  // a wave's step, then the state in front of the wave
+  __shared__ __attribute__((aligned(16))) float lds_b[WAVES * TC];
+  __shared__ unsigned lds_reset[WAVES];  // bit 0: a sequence begins in the wave's places, bit 1: the first of them continues none
   __shared__ unsigned lds_tile;
   const int tid = (int)threadIdx.x, lane = tid % TCL, group = tid / TCL;
   unsigned tile = blockIdx.x;
   if (p.ticket) {  // the same for every block of the launch
     if (tid == 0) lds_tile = atomic_add_u32(p.ticket, 1u);
     __syncthreads();
-    tile = lds_tile;
+    tile = wave_uniform(lds_tile);
   }
   const unsigned chunk = tile / p.strips, strip = tile % p.strips;
   const unsigned place0 = chunk * TILE_ROWS + group * RPT;
@@ -145,6 +212,7 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
   const int count = (int)p.channels - (int)channel;  // channels of this chunk that exist (<= 0: none)
 
   // what each of the thread's places is: inside a sequence, the first or the last one of it in place order
+  constexpr unsigned kAll = (1u << RPT) - 1u;
   unsigned inside = 0, begins = 0, ends = 0;
   auto row_of = [&](unsigned place) { return BACK ? p.rows - 1 - place : place; };
   if (p.row_sequence) {
@@ -165,14 +233,18 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
     }
   } else {
     unsigned at = place0 % p.sequence_rows;  // the rows are whole sequences, so this holds in either direction
+    if (at > 0 && at + RPT < p.sequence_rows) {
+      inside = place0 < p.rows ? kAll : 0u;
+    } else {
 #pragma unroll
-    for (int i = 0; i < RPT; i++) {
-      if (place0 + i < p.rows) {
-        inside |= 1u << i;
-        if (at == 0) begins |= 1u << i;
-        if (at == p.sequence_rows - 1) ends |= 1u << i;
+      for (int i = 0; i < RPT; i++) {
+        if (place0 + i < p.rows) {
+          inside |= 1u << i;
+          if (at == 0) begins |= 1u << i;
+          if (at == p.sequence_rows - 1) ends |= 1u << i;
+        }
+        at = at == p.sequence_rows - 1 ? 0 : at + 1;
       }
-      at = at == p.sequence_rows - 1 ? 0 : at + 1;
     }
   }
   auto sequence_at = [&](int i) {
@@ -180,97 +252,195 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
     return p.row_sequence ? (unsigned)p.row_sequence[row] : row / p.sequence_rows;
   };
 
-  // all loads first
-  uint4_t cx[RPT], cg[RPT], ch[BACK ? RPT : 1], cd[BACK ? RPT : 1];
-#pragma unroll
-  for (int i = 0; i < RPT; i++) {
-    const int n = (inside >> i) & 1u ? count : 0;
-    const size_t row = n > 0 ? row_of(place0 + i) : 0;
-    cg[i] = load_chunk_of<DT, ALIGNED>(p.g, row * p.g_stride + channel, n);
-    if constexpr (!BACK || GATE == kGateSigmoid) cx[i] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + channel, n);
-    if constexpr (BACK) {
-      cd[i] = load_chunk_of<DT, ALIGNED>(p.dh, row * p.dh_stride + channel, n);
-      const int nh = (ends >> i) & 1u ? 0 : n;  // the row in front of a sequence's first one is another sequence's
-      ch[i] = load_chunk_of<DT, ALIGNED>(p.h, (nh > 0 ? row - 1 : 0) * p.h_stride + channel, nh);
-    }
-  }
-  // a, b of every place (b: what the place adds to the state; where a sequence begins, with its seed) and the aggregate
-  float a[RPT][V], b[RPT][V], A[V], B[V];
+  // Most waves have places in the middle of one sequence only.  For them nothing has to be looked at place by place (the
+  // general form takes 53 instruction slots per element, this one 26, and the kernel is bound by them as soon as it is not
+  // by memory), and a lane's addresses are one 32-bit offset from a base that the wave's rows share.
+  const int wave = wave_in_block();
+  constexpr int WAVE_GROUPS = 64 / TCL;
+  const bool plain = p.near_rows && (ALIGNED || strip * TC + TC <= p.channels) && ballot(inside != kAll || (begins | ends) != 0) == 0;
+  const unsigned wave_place = wave_uniform(chunk * TILE_ROWS + wave * (WAVE_GROUPS * RPT));
+  const unsigned wave_row = BACK ? p.rows - wave_place - WAVE_GROUPS * RPT : wave_place;  // the lowest row of a plain wave
+  const unsigned lane_row = (unsigned)(BACK ? WAVE_GROUPS - 1 - group % WAVE_GROUPS : group % WAVE_GROUPS) * RPT;
+  const unsigned strip_at = wave_uniform(strip * TC);
+  const unsigned lane_channel = count > 0 ? (unsigned)(lane * V) : 0u;  // a lane without channels reads the strip's first ones
+  constexpr size_t E = sizeof(typename Elem<DT>::word_t);
+  // place i of the thread lies in row wave_row + lane_row + step_row(i)
+  auto step_row = [](int i) { return BACK ? RPT - 1 - i : i; };
+  auto plain_load = [&](const void *q, size_t stride, int row) {
+    const char *base = static_cast<const char *>(q) + (((ptrdiff_t)wave_row + row) * (ptrdiff_t)stride + strip_at) * (ptrdiff_t)E;
+    return load_at<ALIGNED>(base, (lane_row * (unsigned)stride + lane_channel) * (unsigned)E);
+  };
+  auto plain_store = [&](void *q, size_t stride, int row, const float (&v)[V]) {
+    char *base = static_cast<char *>(q) + (((ptrdiff_t)wave_row + row) * (ptrdiff_t)stride + strip_at) * (ptrdiff_t)E;
+    if (count > 0) store_at<ALIGNED>(base, (lane_row * (unsigned)stride + lane_channel) * (unsigned)E, pack_chunk<DT>(v));
+  };
+
+  constexpr bool KEEP = GATE == kGateSigmoid;
+  uint4_t cx[BACK && KEEP ? RPT : 1], ch[BACK ? RPT : 1];  // what the gradient needs again at the end
+  float a[RPT][V], b[RPT][V], A[V], B[V];                  // b: what the place adds to the state; where a sequence begins, with its seed
+  float keep[BACK && KEEP ? RPT : 1][V];
 #pragma unroll
   for (int e = 0; e < V; e++) {
     A[e] = 1.0f;
     B[e] = 0.0f;
   }
-#pragma unroll
-  for (int i = 0; i < RPT; i++) {
-    const bool in = (inside >> i) & 1u, first = (begins >> i) & 1u;
-    float g[V], x[V], seed[V];
-    unpack_chunk<DT>(cg[i], g);
-    unpack_chunk<DT>(BACK ? cd[BACK ? i : 0] : cx[i], x);
-    if (first && p.seed) {
-      load_floats<V, ALIGNED>(p.seed, (size_t)sequence_at(i) * p.channels + channel, count, seed);
+  auto element = [&](int i, int e, float g, float x) {  // x: the input, or dh
+    float k;
+    gate_of<DT, GATE>(g, &a[i][e], &k);
+    if constexpr (BACK) {
+      b[i][e] = x;  // delta without the carry; the state is u = a delta
+      if constexpr (KEEP) keep[i][e] = k;
     } else {
+      b[i][e] = KEEP ? k * x : x;
+    }
+  };
+  if (plain) {
+    uint4_t cg[RPT], cin[RPT];
 #pragma unroll
-      for (int e = 0; e < V; e++) seed[e] = 0.0f;
+    for (int i = 0; i < RPT; i++) {
+      cg[i] = plain_load(p.g, p.g_stride, step_row(i));
+      cin[i] = BACK ? plain_load(p.dh, p.dh_stride, step_row(i)) : plain_load(p.x, p.x_stride, step_row(i));
+    }
+    if constexpr (BACK) {
+#pragma unroll
+      for (int i = 0; i < RPT; i++) {
+        ch[i] = plain_load(p.h, p.h_stride, step_row(i) - 1);  // the row in front belongs to the same sequence
+        if constexpr (KEEP) cx[i] = plain_load(p.x, p.x_stride, step_row(i));
+      }
     }
 #pragma unroll
-    for (int e = 0; e < V; e++) {
-      float keep;
-      gate_of<DT, GATE>(g[e], &a[i][e], &keep);
+    for (int i = 0; i < RPT; i++) {
+      float g[V], x[V];
+      unpack_chunk<DT>(cg[i], g);
+      unpack_chunk<DT>(cin[i], x);
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        element(i, e, g[e], x[e]);
+        B[e] = BACK ? a[i][e] * (b[i][e] + B[e]) : __builtin_fmaf(a[i][e], B[e], b[i][e]);
+        A[e] *= a[i][e];
+      }
+    }
+  } else {
+    uint4_t cg[RPT], cin[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+      const int n = (inside >> i) & 1u ? count : 0;
+      const size_t row = n > 0 ? row_of(place0 + i) : 0;
+      cg[i] = load_chunk_of<DT, ALIGNED>(p.g, row * p.g_stride + channel, n);
+      if constexpr (!BACK) cin[i] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + channel, n);
       if constexpr (BACK) {
-        b[i][e] = first ? x[e] + seed[e] : x[e];  // delta without the carry; the state is u = a delta
-        if (in) {
-          B[e] = a[i][e] * (first ? b[i][e] : b[i][e] + B[e]);
-          A[e] = first ? 0.0f : a[i][e] * A[e];
-        }
+        cin[i] = load_chunk_of<DT, ALIGNED>(p.dh, row * p.dh_stride + channel, n);
+        if constexpr (KEEP) cx[i] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + channel, n);
+        const int nh = (ends >> i) & 1u ? 0 : n;  // the row in front of a sequence's first one is another sequence's
+        ch[i] = load_chunk_of<DT, ALIGNED>(p.h, (nh > 0 ? row - 1 : 0) * p.h_stride + channel, nh);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+      const bool in = (inside >> i) & 1u, first = (begins >> i) & 1u;
+      float g[V], x[V], seed[V];
+      unpack_chunk<DT>(cg[i], g);
+      unpack_chunk<DT>(cin[i], x);
+      if (first && p.seed) {
+        load_floats<V, ALIGNED>(p.seed, (size_t)sequence_at(i) * p.channels + channel, count, seed);
       } else {
-        b[i][e] = GATE == kGateSigmoid ? keep * x[e] : x[e];
-        if (first) b[i][e] = __builtin_fmaf(a[i][e], seed[e], b[i][e]);
-        if (in) {
-          B[e] = first ? b[i][e] : __builtin_fmaf(a[i][e], B[e], b[i][e]);
-          A[e] = first ? 0.0f : a[i][e] * A[e];
+#pragma unroll
+        for (int e = 0; e < V; e++) seed[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        element(i, e, g[e], x[e]);
+        if constexpr (BACK) {
+          if (first) b[i][e] += seed[e];
+          if (in) B[e] = a[i][e] * (first ? b[i][e] : b[i][e] + B[e]);
+        } else {
+          if (first) b[i][e] = __builtin_fmaf(a[i][e], seed[e], b[i][e]);
+          if (in) B[e] = first ? b[i][e] : __builtin_fmaf(a[i][e], B[e], b[i][e]);
         }
+        if (in) A[e] = first ? 0.0f : a[i][e] * A[e];
       }
     }
   }
+  unsigned reset = begins ? 1u : 0u, front_reset;
+  float FA[V], FB[V];
+  if (plain) combine_groups<TCL, V, false>(A, B, reset, FA, FB, front_reset);
+  else combine_groups<TCL, V, true>(A, B, reset, FA, FB, front_reset);
+  if (lane_id() < TCL) {
 #pragma unroll
-  for (int i = 0; i < V / 4; i++) {
-    *reinterpret_cast<float4_t *>(&lds_a[group * TC + lane * V + 4 * i]) = float4_t{A[4 * i], A[4 * i + 1], A[4 * i + 2], A[4 * i + 3]};
-    *reinterpret_cast<float4_t *>(&lds_b[group * TC + lane * V + 4 * i]) = float4_t{B[4 * i], B[4 * i + 1], B[4 * i + 2], B[4 * i + 3]};
+    for (int i = 0; i < V / 4; i++) {
+      *reinterpret_cast<float4_t *>(&lds_a[wave * TC + lane * V + 4 * i]) = float4_t{A[4 * i], A[4 * i + 1], A[4 * i + 2], A[4 * i + 3]};
+      *reinterpret_cast<float4_t *>(&lds_b[wave * TC + lane * V + 4 * i]) = float4_t{B[4 * i], B[4 * i + 1], B[4 * i + 2], B[4 * i + 3]};
+    }
+    // behind a place outside every sequence another one begins: nothing is carried over it
+    if (lane == 0) lds_reset[wave] = reset | ((begins & 1u) || !(inside & 1u) ? 2u : 0u);
   }
-  // a place outside every sequence ends what came before it, too: what follows it begins a sequence
-  const unsigned outside = ~inside & ((1u << RPT) - 1u);
-  if (lane == 0) lds_reset[group] = (begins ? 1u : 0u) | ((begins & 1u) || (outside & 1u) ? 2u : 0u);
   __syncthreads();
   if (tid < TC) {
-    const bool exists = strip * TC + tid < p.channels;
-    float TA = 1.0f, TB = 0.0f;
-    bool own_state = false;
+    float ga[WAVES], gb[WAVES];
+    unsigned gr[WAVES];
+    ScanStep own{1.0f, 0.0f, false};
 #pragma unroll
-    for (int j = 0; j < GROUPS; j++) {
-      const bool reset = lds_reset[j] & 1u;
-      const float ga = lds_a[j * TC + tid], gb = lds_b[j * TC + tid];
-      TB = reset ? gb : __builtin_fmaf(ga, TB, gb);
-      TA = reset ? 0.0f : ga * TA;
-      own_state = own_state || reset;
+    for (int j = 0; j < WAVES; j++) {
+      ga[j] = lds_a[j * TC + tid];
+      gb[j] = lds_b[j * TC + tid];
+      gr[j] = lds_reset[j];
+    }
+#pragma unroll
+    for (int j = 0; j < WAVES; j++) {
+      own.B = gr[j] & 1u ? gb[j] : __builtin_fmaf(ga[j], own.B, gb[j]);
+      own.A = gr[j] & 1u ? 0.0f : ga[j] * own.A;
+      own.is_state = own.is_state || (gr[j] & 1u);
     }
     float state = 0.0f;
-    if (p.ticket && exists) state = exchange_carry(p, chunk, strip, TC, tid, TA, TB, own_state, (lds_reset[0] & 2u) == 0);
+    if (p.ticket && strip * TC + tid < p.channels) state = exchange_carry(p, chunk, strip, TC, tid, own, (gr[0] & 2u) == 0);
 #pragma unroll
-    for (int j = 0; j < GROUPS; j++) {
-      const bool reset = lds_reset[j] & 1u;
-      const float ga = lds_a[j * TC + tid], gb = lds_b[j * TC + tid];
-      lds_a[j * TC + tid] = state;  // from here on: the state in front of the group
-      state = reset ? gb : __builtin_fmaf(ga, state, gb);
+    for (int j = 0; j < WAVES; j++) {
+      lds_a[j * TC + tid] = state;
+      state = gr[j] & 1u ? gb[j] : __builtin_fmaf(ga[j], state, gb[j]);
     }
   }
   __syncthreads();
   float state[V];
 #pragma unroll
   for (int i = 0; i < V / 4; i++) {
-    const float4_t s = *reinterpret_cast<const float4_t *>(&lds_a[group * TC + lane * V + 4 * i]);
+    const float4_t s = *reinterpret_cast<const float4_t *>(&lds_a[wave * TC + lane * V + 4 * i]);
 #pragma unroll
     for (int e = 0; e < 4; e++) state[4 * i + e] = s[e];
+  }
+#pragma unroll
+  for (int e = 0; e < V; e++) state[e] = front_reset ? FB[e] : __builtin_fmaf(FA[e], state[e], FB[e]);
+  auto gradients = [&](int i, int e, float delta, float h, float x, float *dx, float *dg) {
+    if constexpr (KEEP) {
+      *dx = keep[i][e] * delta;
+      *dg = *dx * ((h - x) * a[i][e]);
+    } else {
+      *dx = delta;
+      *dg = delta * h;
+      if constexpr (GATE == kGateLog) *dg *= a[i][e];
+    }
+  };
+  if (plain) {
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+      if constexpr (BACK) {
+        float h[V], x[V], dx[V], dg[V];
+        unpack_chunk<DT>(ch[i], h);
+        if constexpr (KEEP) unpack_chunk<DT>(cx[i], x);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const float delta = b[i][e] + state[e];
+          state[e] = a[i][e] * delta;
+          gradients(i, e, delta, h[e], KEEP ? x[e] : 0.0f, &dx[e], &dg[e]);
+        }
+        plain_store(p.out, p.out_stride, step_row(i), dx);
+        plain_store(p.out_g, p.out_g_stride, step_row(i), dg);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++) state[e] = __builtin_fmaf(a[i][e], state[e], b[i][e]);
+        plain_store(p.out, p.out_stride, step_row(i), state);
+      }
+    }
+    return;
   }
 #pragma unroll
   for (int i = 0; i < RPT; i++) {
@@ -281,26 +451,13 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
       float h[V], x[V], dx[V], dg[V];
       unpack_chunk<DT>(ch[i], h);
       if (end && p.h0) load_floats<V, ALIGNED>(p.h0, (size_t)sequence_at(i) * p.channels + channel, count, h);
-      if constexpr (GATE == kGateSigmoid) unpack_chunk<DT>(cx[i], x);
+      if constexpr (KEEP) unpack_chunk<DT>(cx[i], x);
 #pragma unroll
       for (int e = 0; e < V; e++) {
         const float delta = first ? b[i][e] : b[i][e] + state[e];
         if (in) state[e] = a[i][e] * delta;
-        dx[e] = delta;
-        dg[e] = delta * h[e];
-        if constexpr (GATE == kGateLog) dg[e] *= a[i][e];
-        if constexpr (GATE == kGateSigmoid) {
-          float g[V];
-          unpack_chunk<DT>(cg[i], g);
-          float s, keep;
-          sigmoid_pair<DT == kF32>(g[e], &s, &keep);
-          dx[e] = keep * delta;
-          dg[e] = delta * (h[e] - x[e]) * (s * keep);
-        }
-      }
-      if (!in) {
-#pragma unroll
-        for (int e = 0; e < V; e++) dx[e] = dg[e] = 0.0f;
+        gradients(i, e, delta, h[e], KEEP ? x[e] : 0.0f, &dx[e], &dg[e]);
+        if (!in) dx[e] = dg[e] = 0.0f;
       }
       store_chunk_of<DT, ALIGNED>(p.out, row * p.out_stride + channel, n, dx);
       store_chunk_of<DT, ALIGNED>(p.out_g, row * p.out_g_stride + channel, n, dg);
@@ -313,11 +470,11 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
   }
 }
 
-// Ahead of the scan: clears the ticket and the descriptors, finds every row's sequence from the offsets (rows of no
+// Ahead of the scan: clears the ticket and the entries, finds every row's sequence from the offsets (rows of no
 // sequence get -1), and hands the seed of each empty sequence on as the state behind it.
 struct GatedScanSetup {
   unsigned *head;          // 64 words: ticket, expired waits
-  uint4_t *clear;          // descriptors
+  uint4_t *clear;          // entries
   size_t clear_chunks;     // 16-byte chunks of them
   const void *offsets;     // sequences + 1 of them, or null (then all sequences are empty, or none is)
   int offset_bits;
@@ -331,7 +488,7 @@ TCU_DEVICE long long offset_at(const GatedScanSetup &s, unsigned j) { return s.o
 __global__ __launch_bounds__(256) inline void gated_scan_setup_kernel(GatedScanSetup s) {
   const size_t me = (size_t)blockIdx.x * blockDim.x + threadIdx.x, all = (size_t)gridDim.x * blockDim.x;
   if (me < 64) s.head[me] = 0u;
-  for (size_t i = me; i < s.clear_chunks; i += all) s.clear[i] = uint4_t{0u, 0u, 0u, 0u};
+  for (size_t i = me; i < s.clear_chunks; i += all) s.clear[i] = uint4_t{~0u, ~0u, ~0u, ~0u};  // kNoEntry
   for (size_t r = me; s.offsets && r < s.rows; r += all) {
     unsigned lo = 0, hi = s.sequences;  // the last sequence that begins at or in front of the row is in [lo - 1, hi - 1]
     while (lo < hi) {

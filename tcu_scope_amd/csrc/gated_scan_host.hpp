@@ -7,18 +7,23 @@
 
 namespace tcu {
 
-// Tiles: 16 lanes (256 bytes of a row) x 16 groups.  Places per thread: the (a, b) of every place stay in registers.
-constexpr int kScanLanes = 16, kScanThreads = 256, kScanPlaces = 8, kScanBackPlaces = 4;
-constexpr unsigned kScanTileRows = kScanThreads / kScanLanes * kScanPlaces, kScanBackTileRows = kScanThreads / kScanLanes * kScanBackPlaces;
+// Tiles: 16 lanes (256 bytes of a row) x 16 or 32 groups of so many places per thread, whose (a, b) stay in registers (two
+// waves per SIMD).  Places: 8 | 4 forwards 65536 x 2048 fp16 187 | 228 us, 4 | 2 | 8 backwards 32768 x 2048 bf16 164 | 223 | 227.
+// Blocks of 512 threads where there are few tiles, i.e. where the waits for each other count: 8191 x 1000 bf16 packed 22.5 ->
+// 19.1 us, backwards 4099 x 769 fp32 30.2 -> 23.7; from about 1024 tiles on 256 threads are as fast or faster (backwards
+// 32768 x 2048 bf16 164 | 178).
+constexpr int kScanLanes = 16, kScanPlaces = 8, kScanBackPlaces = 4;
+constexpr size_t kScanManyTiles = 1024;
 inline unsigned scan_tile_channels(int dtype) { return (unsigned)(kScanLanes * 16 / element_bytes(dtype)); }
 
 struct GatedScanPlan {
   size_t rows = 0, strips = 0, chunks = 0;
-  size_t rows_at = 0, desc_at = 0, desc_bytes = 0, bytes = 0;  // workspace: 64 words, the rows' sequences, the descriptors
-  bool chained = false;                                        // several chunks of places: ticket and descriptors
+  size_t rows_at = 0, entries_at = 0, entries_bytes = 0, bytes = 0;  // workspace: 64 words, the rows' sequences, the entries
+  int threads = 256;
+  bool chained = false;                                        // several chunks of places: ticket and entries
 };
 
-inline int plan_gated_scan(const char *what, const tcu_gated_scan_shape *s, unsigned tile_rows, GatedScanPlan *plan) {
+inline int plan_gated_scan(const char *what, const tcu_gated_scan_shape *s, int places, GatedScanPlan *plan) {
   const std::string w(what);
   if (!s) return report_failure(TCU_ERR_INVALID_ARG, w + ": null shape");
   if (!known_dtype(s->dtype)) return report_failure(TCU_ERR_INVALID_ARG, w + ": dtype must be TCU_F16, TCU_BF16 or TCU_F32");
@@ -37,23 +42,27 @@ inline int plan_gated_scan(const char *what, const tcu_gated_scan_shape *s, unsi
   if (plan->rows > ((size_t)1 << 31) - 4096) return report_failure(TCU_ERR_UNSUPPORTED, w + ": more than 2^31 - 4096 rows");
   const unsigned tc = scan_tile_channels(s->dtype);
   plan->strips = (s->channels + tc - 1) / tc;
-  plan->chunks = (plan->rows + tile_rows - 1) / tile_rows;
+  auto chunks = [&](int threads) { return (plan->rows + threads / kScanLanes * places - 1) / (threads / kScanLanes * places); };
+  if (plan->strips * chunks(256) < kScanManyTiles) plan->threads = 512;
+  plan->chunks = chunks(plan->threads);
   if (plan->strips * plan->chunks >= ((size_t)1 << 31)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": 2^31 tiles or more");
   plan->chained = plan->chunks > 1;
   plan->rows_at = 256;
-  plan->desc_at = plan->rows_at + (s->d_offsets ? (plan->rows * 4 + 255) / 256 * 256 : 0);
-  plan->desc_bytes = plan->chained ? plan->strips * plan->chunks * tc * 16 : 0;
-  plan->bytes = plan->desc_at + plan->desc_bytes;
+  plan->entries_at = plan->rows_at + (s->d_offsets ? (plan->rows * 4 + 255) / 256 * 256 : 0);
+  plan->entries_bytes = plan->chained ? plan->strips * (plan->chunks + plan->chunks / kScanGroup + plan->chunks / (kScanGroup * kScanGroup)) * tc * 8 : 0;
+  plan->bytes = plan->entries_at + plan->entries_bytes;
   return TCU_OK;
 }
 
 template <int DT, int GATE, bool BACK, bool ALIGNED>
-inline void launch_gated_scan_kernel(unsigned grid, void *stream, const GatedScanParams &p) {
-  launch(gated_scan_kernel<DT, GATE, BACK, ALIGNED, kScanLanes, BACK ? kScanBackPlaces : kScanPlaces, kScanThreads>, grid, (unsigned)kScanThreads, stream, p);
+inline void launch_gated_scan_kernel(unsigned grid, int threads, void *stream, const GatedScanParams &p) {
+  constexpr int PLACES = BACK ? kScanBackPlaces : kScanPlaces;
+  if (threads == 512) launch(gated_scan_kernel<DT, GATE, BACK, ALIGNED, kScanLanes, PLACES, 512>, grid, 512u, stream, p);
+  else launch(gated_scan_kernel<DT, GATE, BACK, ALIGNED, kScanLanes, PLACES, 256>, grid, 256u, stream, p);
 }
 template <int DT, bool BACK>
-inline void launch_gated_scan_typed(int gate, bool aligned, unsigned grid, void *stream, const GatedScanParams &p) {
-#define TCU_SCAN_GATE(G_) aligned ? launch_gated_scan_kernel<DT, G_, BACK, true>(grid, stream, p) : launch_gated_scan_kernel<DT, G_, BACK, false>(grid, stream, p)
+inline void launch_gated_scan_typed(int gate, bool aligned, unsigned grid, int threads, void *stream, const GatedScanParams &p) {
+#define TCU_SCAN_GATE(G_) aligned ? launch_gated_scan_kernel<DT, G_, BACK, true>(grid, threads, stream, p) : launch_gated_scan_kernel<DT, G_, BACK, false>(grid, threads, stream, p)
   if (gate == TCU_GATE_DECAY) TCU_SCAN_GATE(kGateDecay);
   else if (gate == TCU_GATE_LOG) TCU_SCAN_GATE(kGateLog);
   else TCU_SCAN_GATE(kGateSigmoid);
@@ -69,19 +78,21 @@ inline int run_gated_scan(const tcu_gated_scan_shape *s, const GatedScanPlan &pl
   p.sequence_rows = (unsigned)s->sequence_length;
   p.channels = (unsigned)s->channels;
   p.zero_outside = s->zero_outside != 0;
+  p.near_rows = true;
+  for (size_t stride : {p.x_stride, p.g_stride, p.h_stride, p.dh_stride, p.out_stride, p.out_g_stride}) p.near_rows = p.near_rows && stride < ((size_t)1 << 23);
   p.strips = (unsigned)plan.strips;
   p.chunks = (unsigned)plan.chunks;
   p.ticket = plan.chained ? head : nullptr;
   p.expired = head + 1;
-  p.descriptors = reinterpret_cast<unsigned long long *>(base + plan.desc_at);
+  p.entries = reinterpret_cast<unsigned long long *>(base + plan.entries_at);
   p.poll_limit = shared_poll_limit();
   p.mute_tile = shared_mute_partition();
   p.row_sequence = s->d_offsets ? reinterpret_cast<const int *>(base + plan.rows_at) : nullptr;
   if (plan.chained || s->d_offsets || (plan.rows == 0 && p.last)) {
     GatedScanSetup q{};
     q.head = head;
-    q.clear = reinterpret_cast<uint4_t *>(base + plan.desc_at);
-    q.clear_chunks = plan.desc_bytes / 16;
+    q.clear = reinterpret_cast<uint4_t *>(base + plan.entries_at);
+    q.clear_chunks = plan.entries_bytes / 16;
     q.offsets = s->d_offsets;
     q.offset_bits = s->offset_bits;
     q.sequences = (unsigned)s->num_sequences;
@@ -90,7 +101,7 @@ inline int run_gated_scan(const tcu_gated_scan_shape *s, const GatedScanPlan &pl
     q.row_sequence = reinterpret_cast<int *>(base + plan.rows_at);
     q.seed = p.seed;
     q.last = p.last;
-    size_t work = q.clear_chunks / 4 > plan.rows ? q.clear_chunks / 4 : plan.rows;
+    size_t work = q.clear_chunks > plan.rows ? q.clear_chunks : plan.rows;
     if (q.last && (q.offsets || plan.rows == 0) && (size_t)q.sequences * 256 > work) work = (size_t)q.sequences * 256;
     size_t blocks = (work + 255) / 256;
     blocks = blocks < 1 ? 1 : (blocks > 2048 ? 2048 : blocks);
@@ -98,9 +109,9 @@ inline int run_gated_scan(const tcu_gated_scan_shape *s, const GatedScanPlan &pl
   }
   if (plan.rows == 0) return TCU_OK;
   const unsigned grid = (unsigned)(plan.strips * plan.chunks);
-  if (s->dtype == TCU_F16) launch_gated_scan_typed<kF16, BACK>(s->gate, aligned, grid, stream, p);
-  else if (s->dtype == TCU_BF16) launch_gated_scan_typed<kBF16, BACK>(s->gate, aligned, grid, stream, p);
-  else launch_gated_scan_typed<kF32, BACK>(s->gate, aligned, grid, stream, p);
+  if (s->dtype == TCU_F16) launch_gated_scan_typed<kF16, BACK>(s->gate, aligned, grid, plan.threads, stream, p);
+  else if (s->dtype == TCU_BF16) launch_gated_scan_typed<kBF16, BACK>(s->gate, aligned, grid, plan.threads, stream, p);
+  else launch_gated_scan_typed<kF32, BACK>(s->gate, aligned, grid, plan.threads, stream, p);
   return TCU_OK;
 }
 
@@ -109,7 +120,7 @@ inline int gated_scan_dispatch(const tcu_gated_scan_shape *s, const void *x, siz
   const char *what = "tcu_gated_scan";
   const std::string w(what);
   GatedScanPlan plan;
-  if (int rc = plan_gated_scan(what, s, kScanTileRows, &plan)) return rc;
+  if (int rc = plan_gated_scan(what, s, kScanPlaces, &plan)) return rc;
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
   if (!workspace) {
     *workspace_bytes = plan.bytes;
@@ -142,7 +153,7 @@ inline int gated_scan_backward_dispatch(const tcu_gated_scan_shape *s, const voi
   const char *what = "tcu_gated_scan_backward";
   const std::string w(what);
   GatedScanPlan plan;
-  if (int rc = plan_gated_scan(what, s, kScanBackTileRows, &plan)) return rc;
+  if (int rc = plan_gated_scan(what, s, kScanBackPlaces, &plan)) return rc;
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
   if (!workspace) {
     *workspace_bytes = plan.bytes;
@@ -195,7 +206,7 @@ inline int gated_scan_step_dispatch(int dtype, int gate, size_t channels, size_t
   s.num_sequences = 1;
   s.sequence_length = s.num_rows = rows;
   GatedScanPlan plan;
-  if (int rc = plan_gated_scan(what, &s, kScanTileRows, &plan)) return rc;
+  if (int rc = plan_gated_scan(what, &s, kScanPlaces, &plan)) return rc;
   if (rows == 0) return TCU_OK;
   if (num_slots == 0 || num_slots >= ((size_t)1 << 31)) return report_failure(TCU_ERR_INVALID_ARG, w + ": num_slots must be 1 ... 2^31 - 1");
   if (!slots && num_slots < rows) return report_failure(TCU_ERR_INVALID_ARG, w + ": fewer slots than rows, and no d_slots to say which");

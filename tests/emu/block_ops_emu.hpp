@@ -11,13 +11,21 @@ namespace tcu {
 inline float hw_exp2(float x) { return exp2f(x); }
 inline float hw_rcp(float x) { return 1.0f / x; }
 inline float hw_rsqrt(float x) { return 1.0f / sqrtf(x); }
-inline float read_lane_of(float x, int l) {
-  auto &w = my_wave();
-  w.slot[lane_id()][0] = __float_as_uint(x);
-  emu::wave_sync();
-  const unsigned r = w.slot[l & 63][0];
-  emu::wave_sync();
-  return __uint_as_float(r);
+template <int D>
+inline void swap_halves(unsigned &lo, unsigned &hi) {
+  if (D == 16) permlane16_swap(lo, hi);
+  else permlane32_swap(lo, hi);
+}
+typedef unsigned any_chunk_t __attribute__((ext_vector_type(4), aligned(2)));
+template <bool WHOLE>
+inline uint4_t load_at(const char *base, unsigned offset) {
+  if (WHOLE) return *reinterpret_cast<const uint4_t *>(base + offset);
+  return *reinterpret_cast<const any_chunk_t *>(base + offset);
+}
+template <bool WHOLE>
+inline void store_at(char *base, unsigned offset, uint4_t v) {
+  if (WHOLE) *reinterpret_cast<uint4_t *>(base + offset) = v;
+  else *reinterpret_cast<any_chunk_t *>(base + offset) = v;
 }
 inline uint16_t bf16_bits(float v) {
   unsigned u = __float_as_uint(v);

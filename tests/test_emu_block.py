@@ -258,7 +258,7 @@ def test_gate_extremes(emu):
 
 def test_waits_that_expire_leave_nan(emu):
     """A tile that publishes nothing (test switch) and a poll limit of 3: everything that depended on it is NaN up to the end of the sequence, nothing else is."""
-    rows, channels = 2600, 8  # 128 places a tile: tiles 0 ... 20, one strip
+    rows, channels = 2600, 8
     offsets = [0, 2000, 2600]
     rng = np.random.default_rng(9)
     x, g, h0 = scan_case(rng, "f16", "sigmoid", offsets, rows, channels)
@@ -271,10 +271,41 @@ def test_waits_that_expire_leave_nan(emu):
         assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0
     finally:
         emu.emu_waits(1 << 20, 0)
-    got, tile = mh.get(), 128
+    got, tile = mh.get(), 256  # places of a tile
     ok = np.r_[0:5 * tile, 2000:rows]
     ref.check(got[ok], want[ok], e[ok], "f16", "what did not wait")
     assert np.isnan(got[5 * tile:2000]).all() and np.isnan(last.reshape(2, channels)[0]).all() and np.isfinite(last.reshape(2, channels)[1]).all()
+
+
+def test_states_handed_on_over_many_tiles(emu):
+    """More than 64 tiles along one sequence (entries of one tile, of eight, and states), forwards and backwards; then a mute tile
+    in the middle of a group, one that closes eight and one that closes 64: NaN behind it, and nothing else."""
+    rows, channels = 9000, 8  # tiles of 128 places backwards
+    offsets = [0, rows]
+    rng = np.random.default_rng(11)
+    x, g, h0 = scan_case(rng, "f32", "decay", offsets, rows, channels)
+    g = np.clip(np.abs(g), 0.99, 0.9999).astype(np.float32).astype(np.float64)  # a state that lasts
+    hs, dh = x[::-1].copy(), x * 0.5
+    m = {k: Matrix(v, "f32") for k, v in dict(g=g, h=hs, dh=dh, dx=x, dg=x).items()}
+    s, keep = shape_of("f32", "decay", rows, channels, None, 32, 1)
+    f0, d0 = floats(h0), floats(h0)
+    call = lambda ws, need: emu.emu_gated_scan_backward(ctypes.byref(s), *operand(m["dh"]), None, 0, *operand(m["g"]), *operand(m["h"]), f0.ctypes.data, None, *operand(m["dx"]), *operand(m["dg"]), d0.ctypes.data, ws, need)
+    kept, ws, have = workspace_for(call)
+    assert call(ws, ctypes.byref(have)) == 0
+    (dx, dg, dh0), (ex, eg, e0) = ref.scan_backward("decay", x, g, hs, dh, offsets, h0, np.zeros(h0.shape))
+    ref.check(m["dx"].get(), dx, ex, "f32", "dx")
+    ref.check(m["dg"].get(), dg, eg, "f32", "dg")
+    ref.check(d0.reshape(h0.shape), dh0, e0, "f32", "dh0")
+    for mute in (3, 15, 63):
+        emu.emu_waits(2, mute + 1)
+        try:
+            assert call(ws, ctypes.byref(have)) == 0
+        finally:
+            emu.emu_waits(1 << 20, 0)
+        first_bad = rows - (mute + 1) * 128  # places run backwards; the mute tile itself knows its carry
+        got = m["dx"].get()
+        ref.check(got[first_bad:], dx[first_bad:], ex[first_bad:], "f32", "what did not wait")
+        assert np.isnan(got[:first_bad]).all() and np.isnan(d0).all()
 
 
 @pytest.mark.parametrize("dtype", list(DTYPES))
