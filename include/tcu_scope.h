@@ -339,7 +339,7 @@ typedef struct {
   int order;      /* tcu_norm_order */
   int activation; /* tcu_activation of the gate; TCU_ACT_NONE without one */
   size_t rows;    /* below 2^31 */
-  size_t dim;     /* 1 ... 32768 */
+  size_t dim;     /* 1 ... 16384 */
   float eps, scale;
 } tcu_fused_norm_shape;
 

@@ -182,10 +182,16 @@ def _check(rc):
         raise TcuError(rc, lib().tcu_last_error().decode())
 
 
-def _torch():
-    import torch
+_torch_module = None
 
-    return torch
+
+def _torch():
+    global _torch_module
+    if _torch_module is None:
+        import torch
+
+        _torch_module = torch
+    return _torch_module
 
 
 def _stream(stream):
@@ -447,24 +453,34 @@ def _dtype_code(t, name):
     return code
 
 
+_enum_values = {}
+
+
 def _enum(kind, value):
-    """A member of the enumeration `kind` from a member, a number or a name in any case."""
-    if isinstance(value, str):
-        try:
-            return int(kind[value.upper()])
-        except KeyError:
-            raise ValueError(f"{value!r} is none of {', '.join(m.name.lower() for m in kind)}") from None
-    return int(kind(value))
+    """The number of a member of the enumeration `kind`, given the member, its number or its name in any case."""
+    known = _enum_values.get((kind, value))
+    if known is None:
+        if isinstance(value, str):
+            if value.upper() not in kind.__members__:
+                raise ValueError(f"{value!r} is none of {', '.join(m.name.lower() for m in kind)}")
+            known = int(kind[value.upper()])
+        else:
+            known = int(kind(value))
+        _enum_values[(kind, value)] = known
+    return known
 
 
 def _matrix(t, name, like=None):
     """(pointer, rows, row stride) of a tensor whose leading dimensions can be read as one: rows of contiguous elements at an even distance."""
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape != like.shape):
-        raise ValueError(f"{name} must have the shape, type and device of the other operands ({tuple(like.shape)}, {like.dtype}, {like.device}); got {tuple(t.shape)}, {t.dtype}, {t.device}")
-    sizes, strides = t.shape, t.stride()
+    sizes = t.shape
+    if like is not None and (t.dtype != like.dtype or t.device != like.device or sizes != like.shape):
+        raise ValueError(f"{name} must have the shape, type and device of the other operands ({tuple(like.shape)}, {like.dtype}, {like.device}); got {tuple(sizes)}, {t.dtype}, {t.device}")
     if len(sizes) < 2:
         raise ValueError(f"{name} must have at least two dimensions")
     width = sizes[-1]
+    if t.is_contiguous():
+        return t.data_ptr(), sizes[0] if len(sizes) == 2 else sizes[:-1].numel(), width
+    strides = t.stride()
     if width > 1 and strides[-1] != 1:
         raise ValueError(f"{name} must be contiguous along its last dimension")
     rows, stride, ok = 1, None, True
@@ -481,10 +497,9 @@ def _matrix(t, name, like=None):
 
 
 def _vector_f32(t, name, shape, device):
-    torch = _torch()
     if t is None:
         return None
-    if t.dtype != torch.float32 or t.device != device or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype != _torch().float32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor of shape {tuple(shape)} on {device}")
     return t.data_ptr()
 
@@ -498,20 +513,43 @@ def _launch_on(device, stream, body):
         with torch.cuda.stream(stream):
             return body(stream.cuda_stream)
     if torch.cuda.current_device() == device.index:
-        return body(torch.cuda.current_stream().cuda_stream)
+        return body(_current_raw_stream(device.index))
     with torch.cuda.device(device):
-        return body(torch.cuda.current_stream().cuda_stream)
+        return body(_current_raw_stream(device.index))
 
 
-def _workspace_of(fn, args, workspace, device):
-    """(pointer, size) of a workspace for the call: the caller's, or a new one of the size the call asks for."""
-    if workspace is None:
-        need = ctypes.c_size_t(0)
-        _check(fn(*args, None, ctypes.byref(need), None))
-        workspace = _torch().empty(need.value, dtype=_torch().uint8, device=device)
-    elif workspace.device != device or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be a contiguous tensor on {device}")
-    return workspace, ctypes.c_size_t(workspace.numel() * workspace.element_size())
+def _current_raw_stream(index):
+    torch = _torch()
+    quick = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without the object around it: 4 us less
+    return quick(index) if quick is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+# Workspace sizes by entry point and sizes of the operands, so that the size is asked for once and not at every call.
+_workspace_sizes = {}
+
+
+def _call_with_workspace(fn, args, sizes, workspace, device, raw):
+    """fn(*args, workspace, its size, stream) with the caller's workspace, or a new one of the size the call needs."""
+    if workspace is not None:
+        if workspace.device != device or not workspace.is_contiguous():
+            raise ValueError(f"workspace must be a contiguous tensor on {device}")
+        have = ctypes.c_size_t(workspace.numel() * workspace.element_size())
+        _check(fn(*args, workspace.data_ptr(), ctypes.byref(have), raw))
+        return
+    torch = _torch()
+    key = (fn.__name__, *sizes)
+    have = ctypes.c_size_t(_workspace_sizes.get(key, 0))
+    if have.value:
+        ws = torch.empty(have.value, dtype=torch.uint8, device=device)
+        rc = fn(*args, ws.data_ptr(), ctypes.byref(have), raw)
+        if rc != 4:  # the size also goes by the operands' alignment: another one may need more
+            return _check(rc)
+    _check(fn(*args, None, ctypes.byref(have), None))
+    if len(_workspace_sizes) >= 1024:
+        _workspace_sizes.clear()
+    _workspace_sizes[key] = have.value
+    ws = torch.empty(have.value, dtype=torch.uint8, device=device)
+    _check(fn(*args, ws.data_ptr(), ctypes.byref(have), raw))
 
 
 def _scan_shape(x, gate, offsets, h0, name="x"):
@@ -555,8 +593,7 @@ def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=
         last = torch.empty(states, dtype=torch.float32, device=x.device) if h_last is None else h_last
         ph, _, sh = _matrix(h, "out", x)
         args = (ctypes.byref(s), px, sx, pg, sg, ph, sh, p0, _vector_f32(last, "h_last", states, x.device))
-        ws, have = _workspace_of(lib().tcu_gated_scan, args, workspace, x.device)
-        _check(lib().tcu_gated_scan(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        _call_with_workspace(lib().tcu_gated_scan, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, x.device, raw)
         return h, last
 
     return _launch_on(x.device, stream, body)
@@ -588,8 +625,7 @@ def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, o
         pox, _, sox = _matrix(out_x, "dx", g)
         pog, _, sog = _matrix(out_g, "dg", g)
         args = (ctypes.byref(s), pd, sd, px, sx, pg, sg, ph, sh, p0, pl, pox, sox, pog, sog, dh0.data_ptr())
-        ws, have = _workspace_of(lib().tcu_gated_scan_backward, args, workspace, g.device)
-        _check(lib().tcu_gated_scan_backward(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        _call_with_workspace(lib().tcu_gated_scan_backward, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, g.device, raw)
         return out_x, out_g, dh0
 
     return _launch_on(g.device, stream, body)
@@ -701,8 +737,7 @@ def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, c
                 got[name] = column()
         args = (ctypes.byref(s), pd, sd, *pz, *pg, *vectors, *px, *ps, *(v for n in ("dx", "dgate", "dresidual") for v in ((got[n].data_ptr(), s.dim) if n in got else (None, 0))),
                 *(got[n].data_ptr() if n in got else None for n in ("dweight", "dbias", "dscale")))
-        ws, have = _workspace_of(lib().tcu_fused_norm_backward, args, workspace, dout.device)
-        _check(lib().tcu_fused_norm_backward(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        _call_with_workspace(lib().tcu_fused_norm_backward, args, (s.dtype, s.rows, s.dim, weight is None, bias is None, channel_scale is None), workspace, dout.device, raw)
         return got
 
     return _launch_on(dout.device, stream, body)
@@ -739,8 +774,7 @@ def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, o
         D = new() if out is None else out
         Z = new() if preactivation is None and return_preactivation else preactivation
         args = (ctypes.byref(s), pa, lda, *pb, pbias, *pc, *_operand(D, "out", M, N, A), *_operand(Z, "preactivation", M, N, A))
-        ws, have = _workspace_of(lib().tcu_fused_gemm, args, workspace, A.device)
-        _check(lib().tcu_fused_gemm(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        _call_with_workspace(lib().tcu_fused_gemm, args, (M, N, K), workspace, A.device, raw)
         return D if Z is None else (D, Z)
 
     return _launch_on(A.device, stream, body)
@@ -767,8 +801,7 @@ def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_grad
         if bias_gradient:
             got["dbias"] = torch.empty(N, dtype=torch.float32, device=A.device)
         args = (ctypes.byref(s), *pd, pa, lda, *pb, *pz, *(v for n in ("dA", "dB") for v in ((got[n].data_ptr(), K) if n in got else (None, 0))), got["dbias"].data_ptr() if bias_gradient else None)
-        ws, have = _workspace_of(lib().tcu_fused_gemm_backward, args, workspace, A.device)
-        _check(lib().tcu_fused_gemm_backward(*args, ws.data_ptr(), ctypes.byref(have), raw))
+        _call_with_workspace(lib().tcu_fused_gemm_backward, args, (M, N, K, s.activation == 0, input_gradient, weight_gradient, bias_gradient), workspace, A.device, raw)
         return got
 
     return _launch_on(A.device, stream, body)

@@ -48,6 +48,35 @@ TCU_DEVICE void unpack_chunk(const uint4_t &c, float (&v)[Elem<DT>::V]) {
     }
   }
 }
+// values 4 q ... 4 q + 3 of a chunk, and four values packed into their place (operators with many operands work on a chunk four
+// values at a time, which keeps their operands' fp32 forms from filling the registers)
+template <int DT>
+TCU_DEVICE void unpack_four(const uint4_t &c, int q, float (&v)[4]) {
+  if constexpr (DT == kF32) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const unsigned w = c[i];
+      v[i] = __uint_as_float(w);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const unsigned w = c[2 * q + i];
+      v[2 * i] = Elem<DT>::load((uint16_t)(w & 0xffffu));
+      v[2 * i + 1] = Elem<DT>::load((uint16_t)(w >> 16));
+    }
+  }
+}
+template <int DT>
+TCU_DEVICE void pack_four(uint4_t &c, int q, const float (&v)[4]) {
+  if constexpr (DT == kF32) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) c[i] = __float_as_uint(v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++) c[2 * q + i] = Elem<DT>::pack(v[2 * i], v[2 * i + 1]);
+  }
+}
 template <int DT>
 TCU_DEVICE uint4_t pack_chunk(const float (&v)[Elem<DT>::V]) {
   uint4_t c;
@@ -90,19 +119,28 @@ TCU_DEVICE uint4_t load_chunk_of(const void *p, size_t at, int count) {
   return c;
 }
 template <int DT, bool WHOLE, bool NT = true>
-TCU_DEVICE void store_chunk_of(void *p, size_t at, int count, const float (&v)[Elem<DT>::V]) {
+TCU_DEVICE void store_packed(void *p, size_t at, int count, const uint4_t &c) {
   constexpr int V = Elem<DT>::V;
   typename Elem<DT>::word_t *q = static_cast<typename Elem<DT>::word_t *>(p) + at;
   if (WHOLE ? count > 0 : count >= V) {
-    const uint4_t c = pack_chunk<DT>(v);
     if constexpr (WHOLE && NT) __builtin_nontemporal_store(c, reinterpret_cast<uint4_t *>(q));
     if constexpr (WHOLE && !NT) *reinterpret_cast<uint4_t *>(q) = c;
     if constexpr (!WHOLE) *reinterpret_cast<any_chunk_t *>(q) = c;
   } else if constexpr (!WHOLE) {
 #pragma unroll
-    for (int e = 0; e < V; e++)
-      if (e < count) q[e] = Elem<DT>::round(v[e]);
+    for (int e = 0; e < V; e++) {
+      if (e < count) {
+        if constexpr (DT == kF32)
+          q[e] = c[e];
+        else
+          q[e] = (uint16_t)(c[e / 2] >> (16 * (e % 2)));
+      }
+    }
   }
+}
+template <int DT, bool WHOLE, bool NT = true>
+TCU_DEVICE void store_chunk_of(void *p, size_t at, int count, const float (&v)[Elem<DT>::V]) {
+  if (count > 0) store_packed<DT, WHOLE, NT>(p, at, count, pack_chunk<DT>(v));
 }
 
 // V fp32 values at element `at` of a fp32 vector, the same conventions
@@ -169,39 +207,61 @@ TCU_DEVICE void sigmoid_pair(float x, float *s, float *one_minus) {
 
 // Activations (tcu_activation) and their slopes.
 constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSigmoid = 4;
-// act(z); the gelu is its tanh form, z (1 + tanh u) / 2 = z sigmoid(2 u) with u = sqrt(2/pi) (z + 0.044715 z^3)
-template <bool EXACT>
-TCU_DEVICE float activation(int act, float z) {
-  constexpr float kTwoA = 1.59576912160573071176f, kB = 0.044715f;  // 2 sqrt(2/pi)
-  if (act == kActNone) return z;
-  if (act == kActRelu) return z < 0.0f ? 0.0f : z;  // a NaN stays one
-  float s, r;
-  sigmoid_pair<EXACT>(act == kActGelu ? kTwoA * z * __builtin_fmaf(kB * z, z, 1.0f) : z, &s, &r);
-  return act == kActSigmoid ? s : z * s;
-}
-// act(z) and act'(z)
-template <bool EXACT>
-TCU_DEVICE void activation_slope(int act, float z, float *value, float *slope) {
-  constexpr float kTwoA = 1.59576912160573071176f, kB = 0.044715f;
-  if (act == kActNone) {
-    *value = z;
-    *slope = 1.0f;
-    return;
-  }
+// The gelu is its tanh form, z (1 + tanh u) / 2 = z sigmoid(2 u) with u = sqrt(2/pi) (z + 0.044715 z^3); so every activation but
+// relu is z sigmoid(v) or sigmoid(v).  `act` is the same for all lanes: one branch for a whole array of values.
+constexpr float kGeluTwoA = 1.59576912160573071176f, kGeluB = 0.044715f;  // 2 sqrt(2/pi)
+
+// z[] = act(z[])
+template <bool EXACT, int N>
+TCU_DEVICE void activate(int act, float (&z)[N]) {
+  if (act == kActNone) return;
   if (act == kActRelu) {
-    *value = z < 0.0f ? 0.0f : z;
-    *slope = z > 0.0f ? 1.0f : 0.0f;
-    return;
+#pragma unroll
+    for (int e = 0; e < N; e++) z[e] = z[e] < 0.0f ? 0.0f : z[e];  // a NaN stays one
+  } else if (act == kActSigmoid) {
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      float s, r;
+      sigmoid_pair<EXACT>(z[e], &s, &r);
+      z[e] = s;
+    }
+  } else {
+    const float cubic = act == kActGelu ? kGeluTwoA * kGeluB : 0.0f, linear = act == kActGelu ? kGeluTwoA : 1.0f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      float s, r;
+      sigmoid_pair<EXACT>(z[e] * __builtin_fmaf(cubic * z[e], z[e], linear), &s, &r);
+      z[e] *= s;
+    }
   }
-  float s, r;  // sigmoid of the argument and 1 - sigmoid
-  sigmoid_pair<EXACT>(act == kActGelu ? kTwoA * z * __builtin_fmaf(kB * z, z, 1.0f) : z, &s, &r);
-  if (act == kActSigmoid) {
-    *value = s;
-    *slope = s * r;
+}
+// value[] = act(z[]), slope[] = act'(z[])
+template <bool EXACT, int N>
+TCU_DEVICE void activate_slope(int act, const float (&z)[N], float (&value)[N], float (&slope)[N]) {
+  if (act == kActNone || act == kActRelu) {
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      value[e] = act == kActRelu && z[e] < 0.0f ? 0.0f : z[e];
+      slope[e] = act == kActRelu && !(z[e] > 0.0f) ? 0.0f : 1.0f;
+    }
+  } else if (act == kActSigmoid) {
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      float s, r;
+      sigmoid_pair<EXACT>(z[e], &s, &r);
+      value[e] = s;
+      slope[e] = s * r;
+    }
   } else {  // z s(v): s + z s (1 - s) v'
-    *value = z * s;
-    const float dv = act == kActGelu ? kTwoA * __builtin_fmaf(3.0f * kB * z, z, 1.0f) : 1.0f;
-    *slope = __builtin_fmaf(z * dv * r, s, s);
+    const float cubic = act == kActGelu ? kGeluTwoA * kGeluB : 0.0f, linear = act == kActGelu ? kGeluTwoA : 1.0f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      float s, r;
+      const float cz = cubic * z[e];
+      sigmoid_pair<EXACT>(z[e] * __builtin_fmaf(cz, z[e], linear), &s, &r);
+      value[e] = z[e] * s;
+      slope[e] = __builtin_fmaf(value[e] * r, __builtin_fmaf(3.0f * cz, z[e], linear), s);
+    }
   }
 }
 

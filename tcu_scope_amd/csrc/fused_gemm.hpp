@@ -40,8 +40,7 @@ TCU_DEVICE void fused_gemm_finish(const FusedGemmParams &p, size_t row, size_t c
 #pragma unroll
   for (int e = 0; e < 8; e++) v[e] += bias[e];
   if (p.Z) store_chunk_of<DT, WHOLE>(p.Z, row * p.ldz + col, count, v);
-#pragma unroll
-  for (int e = 0; e < 8; e++) v[e] = activation<false>(p.act, v[e]);
+  activate<false>(p.act, v);
   if (p.C) {
     float c[8];
     unpack_chunk<DT>(load_chunk_of<DT, WHOLE>(p.C, row * p.ldc + col, count), c);
@@ -350,12 +349,10 @@ __global__ __launch_bounds__(256) void transpose_kernel(TransposeParams p) {
       unpack_chunk<DT>(c, d);
       if (p.Z) {
         unpack_chunk<DT>(load_chunk_of<DT, false>(p.Z, count ? row * p.z_ld + col : 0, count), z);
+        float value[8], slope[8];
+        activate_slope<false>(p.act, z, value, slope);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-          float value, slope;
-          activation_slope<false>(p.act, z[e], &value, &slope);
-          d[e] = e < count ? d[e] * slope : 0.0f;
-        }
+        for (int e = 0; e < 8; e++) d[e] = e < count ? d[e] * slope[e] : 0.0f;
         c = pack_chunk<DT>(d);
       }
       if (p.dz) store_chunk_of<DT, false>(p.dz, count ? row * p.dz_ld + col : 0, count, d);

@@ -135,8 +135,9 @@ __global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_kernel(FusedNormP
     if (p.gate) {
       float g[V];
       unpack_chunk<DT>(cg[k], g);
+      activate<EXACT>(p.act, g);
 #pragma unroll
-      for (int e = 0; e < V; e++) y[e] *= activation<EXACT>(p.act, g[e]);
+      for (int e = 0; e < V; e++) y[e] *= g[e];
     }
     if (p.order == kOrderNormAdd) {
       float s[V], r[V];
@@ -163,7 +164,11 @@ struct FusedNormBackParams {
   bool want_weight, want_bias, want_scale;
 };
 
-template <int DT, bool ALIGNED, int WAVES, int CHUNKS, int BLOCK_WAVES>
+// GATE, STREAM: there is a gate; there is a dstream or x is read (each costs registers; not ALIGNED: there may be).
+// LEAN: for rows so long that the rest would not fit the registers (a spill here costs several times the kernel): the next row
+// is not fetched ahead, only z stays in registers between the statistics and the gradients, and the other operands are read a
+// second time, from the cache.
+template <int DT, bool ALIGNED, bool GATE, bool STREAM, bool LEAN, int WAVES, int CHUNKS, int BLOCK_WAVES>
 __global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_backward_kernel(FusedNormBackParams p) {
   constexpr int V = Elem<DT>::V;
   constexpr bool EXACT = DT == kF32;
@@ -184,17 +189,99 @@ __global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_backward_kernel(F
 #pragma unroll
     for (int e = 0; e < V; e++) sw[k][e] = sb[k][e] = ss[k][e] = 0.0f;
 
-  int parity = 0;
-  for (size_t row = part; row < p.rows; row += parts) {
-    float z[CHUNKS][V], d[CHUNKS][V];  // z, centred; dout, then dy
-    uint4_t cg[CHUNKS], cs[CHUNKS], cx[CHUNKS];
+  // the vectors stay in registers as they are stored (LEAN: in the cache)
+  constexpr int HELD = LEAN ? 1 : CHUNKS;
+  uint4_t vw[HELD], vb[HELD], vc[HELD];
+  if constexpr (!LEAN) {
 #pragma unroll
     for (int k = 0; k < CHUNKS; k++) {
-      unpack_chunk<DT>(load_chunk_of<DT, ALIGNED>(p.z, row * p.z_stride + column(k), exists(k)), z[k]);
-      unpack_chunk<DT>(load_chunk_of<DT, ALIGNED>(p.dout, row * p.dout_stride + column(k), exists(k)), d[k]);
-      if (p.gate) cg[k] = load_chunk_of<DT, ALIGNED>(p.gate, row * p.gate_stride + column(k), exists(k));
-      if (p.dstream) cs[k] = load_chunk_of<DT, ALIGNED>(p.dstream, row * p.dstream_stride + column(k), exists(k));
-      if (p.want_scale && add_norm) cx[k] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + column(k), exists(k));
+      vw[k] = vb[k] = vc[k] = uint4_t{0u, 0u, 0u, 0u};
+      if (p.weight) vw[k] = load_chunk_of<DT, ALIGNED, false>(p.weight, column(k), exists(k));
+      if (p.bias) vb[k] = load_chunk_of<DT, ALIGNED, false>(p.bias, column(k), exists(k));
+      if (p.channel_scale) vc[k] = load_chunk_of<DT, ALIGNED, false>(p.channel_scale, column(k), exists(k));
+    }
+  }
+  auto held = [&](const void *there, const uint4_t &kept, int k) {
+    if constexpr (LEAN) return there ? load_chunk_of<DT, ALIGNED, false>(there, column(k), exists(k)) : uint4_t{0u, 0u, 0u, 0u};
+    return kept;
+  };
+  auto four_of = [](const void *there, const uint4_t &c, int q, float missing, float(&v)[4]) {
+    if (there) {
+      unpack_four<DT>(c, q, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = missing;
+    }
+  };
+  uint4_t nz[CHUNKS], nd[HELD], ng[HELD], ns[HELD], nx[HELD];
+  const bool read_x = p.want_scale && add_norm, gated = GATE && (ALIGNED || p.gate);
+  auto load_z = [&](size_t row, int k) { return load_chunk_of<DT, ALIGNED>(p.z, row * p.z_stride + column(k), exists(k)); };
+  auto load_d = [&](size_t row, int k) { return load_chunk_of<DT, ALIGNED, !LEAN>(p.dout, row * p.dout_stride + column(k), exists(k)); };
+  auto load_g = [&](size_t row, int k) { return load_chunk_of<DT, ALIGNED, !LEAN>(p.gate, row * p.gate_stride + column(k), exists(k)); };
+  auto load_rest = [&](size_t row, int k, int at) {
+    if (STREAM && p.dstream) ns[at] = load_chunk_of<DT, ALIGNED>(p.dstream, row * p.dstream_stride + column(k), exists(k));
+    if (STREAM && read_x) nx[at] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + column(k), exists(k));
+  };
+  auto load_row = [&](size_t row) {
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+      nz[k] = load_z(row, k);
+      if constexpr (!LEAN) {
+        nd[k] = load_d(row, k);
+        if (gated) ng[k] = load_g(row, k);
+        load_rest(row, k, k);
+      }
+    }
+  };
+  // the next row's operands are on their way while a row is worked on
+  if (!LEAN && part < p.rows) load_row(part);
+
+  int parity = 0;
+  for (size_t row = part; row < p.rows; row += parts) {
+    float z[CHUNKS][V];  // centred
+    float f[HELD][V], slope[HELD][V];  // act(gate) and act'(gate)
+    uint4_t cd[HELD], cs[HELD], cx[HELD];
+    auto gate_factors = [&](const uint4_t &gate, int q, float(&value)[4], float(&slopes)[4]) {
+      if (gated) {
+        float g[4];
+        unpack_four<DT>(gate, q, g);
+        activate_slope<EXACT>(p.act, g, value, slopes);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          value[e] = 1.0f;
+          slopes[e] = 0.0f;
+        }
+      }
+    };
+    if constexpr (LEAN) load_row(row);
+#pragma unroll
+    for (int k = 0; k < CHUNKS; k++) {
+      unpack_chunk<DT>(nz[k], z[k]);
+      if constexpr (!LEAN) {
+        cd[k] = nd[k];
+#pragma unroll
+        for (int q = 0; q < V / 4; q++) {
+          float v[4], t[4];
+          gate_factors(ng[k], q, v, t);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            f[k][4 * q + e] = v[e];
+            slope[k][4 * q + e] = t[e];
+          }
+        }
+        if (STREAM && p.dstream) cs[k] = ns[k];
+        if (STREAM && read_x) cx[k] = nx[k];
+      }
+    }
+    if constexpr (!LEAN) {
+      if (row + parts < p.rows) load_row(row + parts);
+#pragma unroll
+      for (int k = 0; k < CHUNKS; k++) {
+        keep_packed(vw[k]);
+        keep_packed(vb[k]);
+        keep_packed(vc[k]);
+      }
     }
     float mean = 0.0f;
     if (p.norm == kNormLayer) {
@@ -207,33 +294,50 @@ __global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_backward_kernel(F
       parity ^= 1;
       mean = s[0] * inv;
     }
-    // sums of z^2, dn z and dn over the row (z centred); columns beyond the row have d = 0
+    // the factors of values 4 q ... of chunk k, and the gradient with respect to act(gate) y there
+    constexpr int H = LEAN ? 0 : 1;
+    auto upstream = [&](int k, int q, const uint4_t &scale, float(&v)[4], float(&t)[4], float(&d)[4], float(&up)[4], float(&c)[4]) {
+      if constexpr (LEAN) {
+        gate_factors(ng[0], q, v, t);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          v[e] = f[H * k][4 * q + e];
+          t[e] = slope[H * k][4 * q + e];
+        }
+      }
+      unpack_four<DT>(cd[H * k], q, d);
+      four_of(p.channel_scale, scale, q, 1.0f, c);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        c[e] *= p.scale;
+        up[e] = add_norm ? d[e] : c[e] * d[e];
+      }
+    };
+    // sums of z^2, dn z and dn over the row (z centred)
     float s[3] = {0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < CHUNKS; k++) {
-      float w[V], f[V], c[V];
-      load_vector<DT, ALIGNED>(p.weight, column(k), exists(k), 1.0f, w);
-#pragma unroll
-      for (int e = 0; e < V; e++) f[e] = 1.0f;
-      if (p.gate) {
-        float g[V];
-        unpack_chunk<DT>(cg[k], g);
-#pragma unroll
-        for (int e = 0; e < V; e++) f[e] = activation<EXACT>(p.act, g[e]);
+      if constexpr (LEAN) {
+        cd[0] = load_d(row, k);
+        if (gated) ng[0] = load_g(row, k);
       }
-      if (!add_norm) {
-        load_vector<DT, ALIGNED>(p.channel_scale, column(k), exists(k), 1.0f, c);
+      const uint4_t cw = held(p.weight, vw[H * k], k), cc = held(p.channel_scale, vc[H * k], k);
 #pragma unroll
-        for (int e = 0; e < V; e++) f[e] *= p.scale * c[e];
-      }
+      for (int q = 0; q < V / 4; q++) {
+        float w[4], v[4], t[4], d[4], up[4], c[4];
+        four_of(p.weight, cw, q, 1.0f, w);
+        upstream(k, q, cc, v, t, d, up, c);
 #pragma unroll
-      for (int e = 0; e < V; e++) {
-        z[k][e] -= mean;
-        if (e < exists(k)) {
-          const float dn = d[k][e] * f[e] * w[e];
-          s[0] = __builtin_fmaf(z[k][e], z[k][e], s[0]);
-          s[1] = __builtin_fmaf(dn, z[k][e], s[1]);
-          s[2] += dn;
+        for (int e = 0; e < 4; e++) {
+          float &zc = z[k][4 * q + e];
+          zc -= mean;
+          if (4 * q + e < exists(k)) {
+            const float dn = up[e] * v[e] * w[e];
+            s[0] = __builtin_fmaf(zc, zc, s[0]);
+            s[1] = __builtin_fmaf(dn, zc, s[1]);
+            s[2] += dn;
+          }
         }
       }
     }
@@ -243,41 +347,48 @@ __global__ __launch_bounds__(64 * BLOCK_WAVES) void fused_norm_backward_kernel(F
     const float mean_dnn = s[1] * rho * inv, mean_dn = p.norm == kNormLayer ? s[2] * inv : 0.0f;
 #pragma unroll
     for (int k = 0; k < CHUNKS; k++) {
-      float w[V], b[V], c[V], dx[V], dg[V];
-      load_vector<DT, ALIGNED>(p.weight, column(k), exists(k), 1.0f, w);
-      load_vector<DT, ALIGNED>(p.bias, column(k), exists(k), 0.0f, b);
-      load_vector<DT, ALIGNED>(p.channel_scale, column(k), exists(k), 1.0f, c);
-      float g[V], extra[V], x[V];
+      if constexpr (LEAN) {
+        cd[0] = load_d(row, k);
+        if (gated) ng[0] = load_g(row, k);
+        load_rest(row, k, 0);
+        if (STREAM && p.dstream) cs[0] = ns[0];
+        if (STREAM && read_x) cx[0] = nx[0];
+      }
+      const uint4_t cw = held(p.weight, vw[H * k], k), cb = held(p.bias, vb[H * k], k), cc = held(p.channel_scale, vc[H * k], k);
+      uint4_t odx, odg, odr;
 #pragma unroll
-      for (int e = 0; e < V; e++) g[e] = extra[e] = x[e] = 0.0f;
-      if (p.gate) unpack_chunk<DT>(cg[k], g);
-      if (p.dstream) unpack_chunk<DT>(cs[k], extra);
-      if (p.want_scale && add_norm) unpack_chunk<DT>(cx[k], x);
+      for (int q = 0; q < V / 4; q++) {
+        float w[4], b[4], v[4], t[4], d[4], up[4], c[4], extra[4], x[4], dx[4], dg[4];
+        four_of(p.weight, cw, q, 1.0f, w);
+        four_of(p.bias, cb, q, 0.0f, b);
+        upstream(k, q, cc, v, t, d, up, c);
+        four_of(STREAM ? p.dstream : nullptr, cs[H * k], q, 0.0f, extra);
+        four_of(STREAM && read_x ? p.x : nullptr, cx[H * k], q, 0.0f, x);
 #pragma unroll
-      for (int e = 0; e < V; e++) {
-        const float n = z[k][e] * rho, y = __builtin_fmaf(n, w[e], b[e]), sc = p.scale * c[e];
-        float f = 1.0f, slope = 0.0f;
-        if (p.gate) activation_slope<EXACT>(p.act, g[e], &f, &slope);
-        const float up = add_norm ? d[k][e] : sc * d[k][e];  // gradient with respect to act(gate) y
-        const float dy = up * f;
-        dg[e] = up * y * slope;
-        sw[k][e] = __builtin_fmaf(dy, n, sw[k][e]);
-        sb[k][e] += dy;
-        if (!add_norm) ss[k][e] = __builtin_fmaf(d[k][e], f * y, ss[k][e]);
-        float dz = rho * (__builtin_fmaf(-n, mean_dnn, dy * w[e]) - mean_dn);
-        if (add_norm) {
-          dz += extra[e];
-          ss[k][e] = __builtin_fmaf(dz, x[e], ss[k][e]);
+        for (int e = 0; e < 4; e++) {
+          const int i = 4 * q + e;
+          const float n = z[k][i] * rho, y = __builtin_fmaf(n, w[e], b[e]), dy = up[e] * v[e];
+          dg[e] = up[e] * y * t[e];
+          sw[k][i] = __builtin_fmaf(dy, n, sw[k][i]);
+          sb[k][i] += dy;
+          if (!add_norm) ss[k][i] = __builtin_fmaf(d[e], v[e] * y, ss[k][i]);
+          dx[e] = rho * (__builtin_fmaf(-n, mean_dnn, dy * w[e]) - mean_dn);
+          if (add_norm) {
+            dx[e] += extra[e];
+            if constexpr (STREAM) ss[k][i] = __builtin_fmaf(dx[e], x[e], ss[k][i]);
+          }
         }
-        dx[e] = dz;
-      }
-      if (p.dresidual) store_chunk_of<DT, ALIGNED>(p.dresidual, row * p.dresidual_stride + column(k), exists(k), dx);
-      if (add_norm) {
+        pack_four<DT>(odr, q, dx);
+        if (add_norm) {
 #pragma unroll
-        for (int e = 0; e < V; e++) dx[e] *= p.scale * c[e];
+          for (int e = 0; e < 4; e++) dx[e] *= c[e];
+        }
+        pack_four<DT>(odx, q, dx);
+        if constexpr (GATE) pack_four<DT>(odg, q, dg);
       }
-      store_chunk_of<DT, ALIGNED>(p.dx, row * p.dx_stride + column(k), exists(k), dx);
-      if (p.dgate) store_chunk_of<DT, ALIGNED>(p.dgate, row * p.dgate_stride + column(k), exists(k), dg);
+      if (p.dresidual) store_packed<DT, ALIGNED>(p.dresidual, row * p.dresidual_stride + column(k), exists(k), odr);
+      store_packed<DT, ALIGNED>(p.dx, row * p.dx_stride + column(k), exists(k), odx);
+      if (GATE && p.dgate) store_packed<DT, ALIGNED>(p.dgate, row * p.dgate_stride + column(k), exists(k), odg);
     }
   }
   const int vectors = (int)p.want_weight + (int)p.want_bias + (int)p.want_scale;

@@ -8,9 +8,12 @@
 
 namespace tcu {
 
-constexpr size_t kNormMaxDim = 32768;   // 16 waves x 64 lanes x 8 chunks of 4 fp32 (x 4 chunks of 8 16-bit values)
-constexpr size_t kNormFewRows = 2048;   // below this many rows four waves share a row that one could hold
-constexpr size_t kNormBackBlocks = 512; // blocks of the gradient's kernel, i.e. partial sums per column
+constexpr size_t kNormMaxDim = 16384;    // beyond it a block cannot hold a row and its columns' sums in registers
+// Waves that share a row in the gradient's kernel, by the chunks per lane that one wave would need.
+inline int norm_back_waves(size_t chunks) { return chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8; }
+// Its blocks, i.e. partial sums per column: as many as bring 8 waves to every compute unit (8192 x 4096 bf16 gated, 8 waves
+// a row: 256 blocks 77 us + 4.7 for the sums, 512 blocks 85 + 7.5; 32768 x 1024: 227 us with half the waves).
+constexpr size_t kNormBackWaves = 256 * 8;
 
 inline int check_norm_shape(const std::string &w, const tcu_fused_norm_shape *s) {
   if (!s) return report_failure(TCU_ERR_INVALID_ARG, w + ": null shape");
@@ -19,33 +22,26 @@ inline int check_norm_shape(const std::string &w, const tcu_fused_norm_shape *s)
   if (s->order != TCU_ORDER_ADD_NORM && s->order != TCU_ORDER_NORM_ADD) return report_failure(TCU_ERR_INVALID_ARG, w + ": unknown order");
   if (!known_activation(s->activation)) return report_failure(TCU_ERR_INVALID_ARG, w + ": unknown activation");
   if (s->dim == 0) return report_failure(TCU_ERR_INVALID_ARG, w + ": dim is 0");
-  if (s->dim > kNormMaxDim) return report_failure(TCU_ERR_UNSUPPORTED, w + ": dim is above 32768");
+  if (s->dim > kNormMaxDim) return report_failure(TCU_ERR_UNSUPPORTED, w + ": dim is above 16384");
   if (s->rows >= ((size_t)1 << 31)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": 2^31 rows or more");
   return TCU_OK;
 }
 
-// launches KERNEL<DT, ALIGNED, WAVES, CHUNKS, BLOCK_WAVES> with `blocks` blocks
-#define TCU_NORM_LAUNCH(KERNEL, DT, ALIGNED, WAVES, CHUNKS, BLOCK_WAVES, blocks) launch(KERNEL<DT, ALIGNED, WAVES, CHUNKS, BLOCK_WAVES>, (unsigned)(blocks), 64u * (BLOCK_WAVES), stream, p)
-
+// Waves that share a row, and chunks per lane: four waves as soon as the row has more than two chunks per lane of one (16384 x
+// 4096 bf16 with residual: 4 waves 89.8 us, 1 wave with 8 chunks per lane 92.7; and the shorter way through a row counts where
+// there are few).
 template <int DT, bool ALIGNED>
 inline void launch_fused_norm(const FusedNormParams &p, void *stream) {
   const size_t ct = (p.dim + 64 * Elem<DT>::V - 1) / (64 * Elem<DT>::V);  // chunks per lane if one wave takes the row
   const size_t rows = p.rows, quads = (rows + 3) / 4;
-#define TCU_NORM(W, C, BW, blocks) TCU_NORM_LAUNCH(fused_norm_kernel, DT, ALIGNED, W, C, BW, blocks)
-  if (ct == 1 || (ct <= 8 && rows >= kNormFewRows)) {
-    if (ct == 1) TCU_NORM(1, 1, 4, quads);
-    else if (ALIGNED && ct == 2) TCU_NORM(1, ALIGNED ? 2 : 8, 4, quads);
-    else if (ALIGNED && ct <= 4) TCU_NORM(1, ALIGNED ? 4 : 8, 4, quads);
-    else TCU_NORM(1, 8, 4, quads);
-  } else if (ct <= 32) {
-    if (ALIGNED && ct <= 4) TCU_NORM(4, ALIGNED ? 1 : 8, 4, rows);
-    else if (ALIGNED && ct <= 8) TCU_NORM(4, ALIGNED ? 2 : 8, 4, rows);
-    else if (ALIGNED && ct <= 16) TCU_NORM(4, ALIGNED ? 4 : 8, 4, rows);
-    else TCU_NORM(4, 8, 4, rows);
-  } else {
-    if (ct <= 64) TCU_NORM(16, 4, 16, rows);
-    else TCU_NORM(16, DT == kF32 ? 8 : 4, 16, rows);  // 16-bit types end at ct = 64
-  }
+#define TCU_NORM(W, C, BW, blocks) launch(fused_norm_kernel<DT, ALIGNED, W, C, BW>, (unsigned)(blocks), 64u * (BW), stream, p)
+  if (ALIGNED && ct == 1) TCU_NORM(1, ALIGNED ? 1 : 2, 4, quads);
+  else if (ct <= 2) TCU_NORM(1, 2, 4, quads);
+  else if (ALIGNED && ct <= 4) TCU_NORM(4, ALIGNED ? 1 : 2, 4, rows);
+  else if (ct <= 8) TCU_NORM(4, 2, 4, rows);
+  else if (ALIGNED && ct <= 16) TCU_NORM(4, 4, 4, rows);
+  else if (ct <= 32) TCU_NORM(8, 4, 8, rows);
+  else TCU_NORM(16, 4, 16, rows);
 #undef TCU_NORM
 }
 
@@ -84,31 +80,41 @@ struct NormBackPlan {
 };
 inline NormBackPlan plan_norm_backward(const tcu_fused_norm_shape *s, size_t vectors) {
   NormBackPlan plan;
-  const size_t per_wave = 64 * 16 / element_bytes(s->dtype);
-  const bool wave_rows = s->dim <= per_wave;  // a wave takes a row, a block four of them
-  const size_t wanted = wave_rows ? (s->rows + 3) / 4 : s->rows;
-  plan.blocks = wanted < kNormBackBlocks ? wanted : kNormBackBlocks;
-  plan.parts = wave_rows ? plan.blocks * 4 : plan.blocks;
+  const size_t per_wave = 64 * 16 / element_bytes(s->dtype), waves = norm_back_waves((s->dim + per_wave - 1) / per_wave);
+  const size_t rows_per_block = waves == 1 ? 4 : 1, block_waves = waves == 1 ? 4 : waves;
+  const size_t wanted = (s->rows + rows_per_block - 1) / rows_per_block, most = kNormBackWaves / block_waves;
+  plan.blocks = wanted < most ? wanted : most;
+  plan.parts = plan.blocks * rows_per_block;
   plan.vectors = vectors;
   const size_t bytes = plan.parts * vectors * s->dim * 4;
   plan.bytes = bytes < 256 ? 256 : bytes;
   return plan;
 }
 
-template <int DT, bool ALIGNED>
+// A lane has one chunk of the row up to 8 waves: the column sums, the row, the next row and the gate's factors are then all in
+// registers.  Longer rows take the lean form.
+template <int DT, bool ALIGNED, bool GATE, bool STREAM>
 inline void launch_fused_norm_backward(const FusedNormBackParams &p, size_t blocks, void *stream) {
   const size_t ct = (p.dim + 64 * Elem<DT>::V - 1) / (64 * Elem<DT>::V);
-#define TCU_NORM(W, C, BW) TCU_NORM_LAUNCH(fused_norm_backward_kernel, DT, ALIGNED, W, C, BW, blocks)
-  if (ct == 1) TCU_NORM(1, 1, 4);
-  else if (ALIGNED && ct <= 4) TCU_NORM(4, ALIGNED ? 1 : 4, 4);
-  else if (ALIGNED && ct <= 8) TCU_NORM(4, ALIGNED ? 2 : 4, 4);
-  else if (ct <= 16) TCU_NORM(4, 4, 4);
-  else if (ALIGNED && ct <= 32) TCU_NORM(ALIGNED ? 8 : 16, 4, ALIGNED ? 8 : 16);
-  else if (ct <= 64) TCU_NORM(16, 4, 16);
-  else TCU_NORM(16, DT == kF32 ? 8 : 4, 16);
+#define TCU_NORM(LEAN, W, C, BW) launch(fused_norm_backward_kernel<DT, ALIGNED, GATE, STREAM, LEAN, W, C, BW>, (unsigned)blocks, 64u * (BW), stream, p)
+  if (ct <= 1) TCU_NORM(false, 1, 1, 4);
+  else if (ct <= 2) TCU_NORM(false, 2, 1, 2);
+  else if (ct <= 4) TCU_NORM(false, 4, 1, 4);
+  else if (ct <= 8) TCU_NORM(false, 8, 1, 8);
+  else if (ct <= 16) TCU_NORM(true, 8, 2, 8);
+  else if (ct <= 32) TCU_NORM(true, 8, 4, 8);
+  else TCU_NORM(true, 8, DT == kF32 ? 8 : 4, 8);  // 16-bit types end at ct = 32
 #undef TCU_NORM
 }
-#undef TCU_NORM_LAUNCH
+template <int DT>
+inline void launch_fused_norm_backward_typed(bool aligned, const FusedNormBackParams &p, size_t blocks, void *stream) {
+  const bool streams = p.dstream != nullptr || (p.want_scale && p.order == kOrderAddNorm);
+  if (!aligned) launch_fused_norm_backward<DT, false, true, true>(p, blocks, stream);
+  else if (p.gate && streams) launch_fused_norm_backward<DT, true, true, true>(p, blocks, stream);
+  else if (p.gate) launch_fused_norm_backward<DT, true, true, false>(p, blocks, stream);
+  else if (streams) launch_fused_norm_backward<DT, true, false, true>(p, blocks, stream);
+  else launch_fused_norm_backward<DT, true, false, false>(p, blocks, stream);
+}
 
 inline int fused_norm_backward_dispatch(const tcu_fused_norm_shape *s, const void *dout, size_t dout_stride, const void *z, size_t z_stride, const void *gate, size_t gate_stride, const void *weight,
                                         const void *bias, const void *channel_scale, const void *x, size_t x_stride, const void *dresidual_out, size_t dresidual_out_stride, void *dx, size_t dx_stride,
@@ -181,7 +187,7 @@ inline int fused_norm_backward_dispatch(const tcu_fused_norm_shape *s, const voi
     p.want_weight = dweight != nullptr;
     p.want_bias = dbias != nullptr;
     p.want_scale = dchannel_scale != nullptr;
-#define TCU_NORM_TYPE(DT) (aligned ? launch_fused_norm_backward<DT, true>(p, plan.blocks, stream) : launch_fused_norm_backward<DT, false>(p, plan.blocks, stream))
+#define TCU_NORM_TYPE(DT) launch_fused_norm_backward_typed<DT>(aligned, p, plan.blocks, stream)
     if (s->dtype == TCU_F16) TCU_NORM_TYPE(kF16);
     else if (s->dtype == TCU_BF16) TCU_NORM_TYPE(kBF16);
     else TCU_NORM_TYPE(kF32);

@@ -425,7 +425,7 @@ NORMS = [
     (3, 2049, 0, 0, "rms", "norm_add", "relu", True, True, True, True, 1.0),
     (2, 4104, 0, 0, "rms", "norm_add", None, True, True, False, False, 0.25),
     (1, 8200, 0, 0, "layer", "norm_add", "silu", True, True, True, True, 1.0),
-    (1, 20000, 0, 0, "rms", "add_norm", "silu", True, True, False, True, 1.0),
+    (1, 16384, 0, 0, "rms", "add_norm", "silu", True, True, False, True, 1.0),
 ]
 
 
@@ -546,7 +546,7 @@ def test_fused_norm_refusals(emu):
     assert fwd(order=2) == 1 and "order" in err()
     assert fwd(activation=5) == 1 and "activation" in err()
     assert fwd(activation=3) == 1 and "without a gate" in err()
-    assert fwd(dim=0) == 1 and fwd(dim=32769) == 2 and fwd(rows=1 << 31) == 2
+    assert fwd(dim=0) == 1 and fwd(dim=16385) == 2 and fwd(rows=1 << 31) == 2
     assert fwd(scale=2.0) == 1 and "without a residual" in err()
     assert fwd(cs=p) == 1 and "without a residual" in err()
     assert fwd(z=m(2)) == 1 and "residual_out" in err()

@@ -27,8 +27,8 @@ CASES = [
     (2100, 2048, None, "layer", "norm_add", "gelu", False, True, True, False, 2.0),
     (2050, 4001, None, "rms", "add_norm", "silu", True, False, False, False, 1.0),
     (40, 8200, None, "layer", "norm_add", "relu", True, True, True, True, 1.0),
-    (9, 32768, None, "rms", "add_norm", "silu", True, True, True, True, 1.0),
-    (5, 20001, None, "layer", "add_norm", "silu", True, True, True, True, 1.0),
+    (9, 16384, None, "rms", "add_norm", "silu", True, True, True, True, 1.0),
+    (5, 16001, None, "layer", "add_norm", "silu", True, True, True, True, 1.0),
 ]
 
 
@@ -130,7 +130,7 @@ def test_refusals(tcu):
         (lambda: tcu.fused_norm(x, scale=2.0), tcu.TcuError, "without a residual"),
         (lambda: tcu.fused_norm(x, residual_out=x), ValueError, "residual_out"),
         (lambda: tcu.fused_norm(x, norm="group"), ValueError, "rms"),
-        (lambda: tcu.fused_norm(torch.zeros(1, 32769, device="cuda")), tcu.TcuError, "32768"),
+        (lambda: tcu.fused_norm(torch.zeros(1, 16385, device="cuda")), tcu.TcuError, "16384"),
         (lambda: tcu.fused_norm_backward(x, x, channel_scale=v), ValueError, "needs x"),
         (lambda: tcu.fused_norm_backward(x, x, order="norm_add", dresidual_out=x), tcu.TcuError, "d_dout itself"),
     ]:
