@@ -361,7 +361,7 @@ int tcu_fused_norm_backward(const tcu_fused_norm_shape *shape, const void *d_dou
 typedef struct {
   int dtype;      /* TCU_F16 or TCU_BF16 */
   int activation; /* tcu_activation */
-  size_t M, N, K; /* K up to 2^22 */
+  size_t M, N, K; /* M below 2^31, N and the leading dimensions of outputs up to 2^28, K up to 2^22 */
   float beta;
 } tcu_fused_gemm_shape;
 

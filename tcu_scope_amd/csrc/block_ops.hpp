@@ -39,6 +39,13 @@ TCU_DEVICE void store_at(char *base, unsigned offset, uint4_t v) {
 // Hides from the compiler that `c` is what it was: what is unpacked from it is then not kept across a loop in twice the registers.
 TCU_DEVICE void keep_packed(uint4_t &c) { asm volatile("" : "+v"(c)); }
 
+// four zeros that the compiler does not know to be zeros
+TCU_DEVICE float4_t opaque_zero() {
+  float4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+  asm volatile("" : "+v"(z));
+  return z;
+}
+
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 TCU_DEVICE unsigned pack_bf16x2(float lo, float hi) {
   bf16x2_t v = {(__bf16)lo, (__bf16)hi};

@@ -211,6 +211,10 @@ constexpr int kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3, kActSigmoi
 // relu is z sigmoid(v) or sigmoid(v).  `act` is the same for all lanes: one branch for a whole array of values.
 constexpr float kGeluTwoA = 1.59576912160573071176f, kGeluB = 0.044715f;  // 2 sqrt(2/pi)
 
+// 1 / (1 + e^-x) alone: where e^-x overflows the reciprocal is 0, as it should be
+template <bool EXACT>
+TCU_DEVICE float sigmoid_of(float x) { return hw_rcp(1.0f + exp_of<EXACT>(-x)); }
+
 // z[] = act(z[])
 template <bool EXACT, int N>
 TCU_DEVICE void activate(int act, float (&z)[N]) {
@@ -220,19 +224,13 @@ TCU_DEVICE void activate(int act, float (&z)[N]) {
     for (int e = 0; e < N; e++) z[e] = z[e] < 0.0f ? 0.0f : z[e];  // a NaN stays one
   } else if (act == kActSigmoid) {
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      float s, r;
-      sigmoid_pair<EXACT>(z[e], &s, &r);
-      z[e] = s;
-    }
-  } else {
-    const float cubic = act == kActGelu ? kGeluTwoA * kGeluB : 0.0f, linear = act == kActGelu ? kGeluTwoA : 1.0f;
+    for (int e = 0; e < N; e++) z[e] = sigmoid_of<EXACT>(z[e]);
+  } else if (act == kActSilu) {
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      float s, r;
-      sigmoid_pair<EXACT>(z[e] * __builtin_fmaf(cubic * z[e], z[e], linear), &s, &r);
-      z[e] *= s;
-    }
+    for (int e = 0; e < N; e++) z[e] *= sigmoid_of<EXACT>(z[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; e++) z[e] *= sigmoid_of<EXACT>(z[e] * __builtin_fmaf(kGeluTwoA * kGeluB * z[e], z[e], kGeluTwoA));
   }
 }
 // value[] = act(z[]), slope[] = act'(z[])

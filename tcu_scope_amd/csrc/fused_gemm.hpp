@@ -34,35 +34,39 @@ struct FusedGemmParams {
   unsigned splits, tiles;  // blocks: splits * tiles, the splits of K outermost
 };
 
-// z = sum + bias, d = act(z) + beta c for the chunk at (row, col), of which `count` columns exist
+// z = sum + bias, d = act(z) + beta c for the 8 columns at (row + lane_row, col + lane_col), of which `count` exist; row and col are
+// the same for the whole wave, so that a lane's address is a scalar base and one offset per matrix.
 template <int DT, bool WHOLE>
-TCU_DEVICE void fused_gemm_finish(const FusedGemmParams &p, size_t row, size_t col, int count, float (&v)[8], const float (&bias)[8]) {
+TCU_DEVICE void fused_gemm_finish(const FusedGemmParams &p, size_t row, size_t col, unsigned lane_row, unsigned lane_col, int count, float (&v)[8], const float (&bias)[8]) {
+  auto base = [&](const void *q, size_t ld) { return static_cast<const uint16_t *>(q) + row * ld + col; };
+  auto offset = [&](size_t ld) { return lane_row * (unsigned)ld + lane_col; };
 #pragma unroll
   for (int e = 0; e < 8; e++) v[e] += bias[e];
-  if (p.Z) store_chunk_of<DT, WHOLE>(p.Z, row * p.ldz + col, count, v);
+  if (p.Z) store_chunk_of<DT, WHOLE>(const_cast<uint16_t *>(base(p.Z, p.ldz)), offset(p.ldz), count, v);
   activate<false>(p.act, v);
   if (p.C) {
     float c[8];
-    unpack_chunk<DT>(load_chunk_of<DT, WHOLE>(p.C, row * p.ldc + col, count), c);
+    unpack_chunk<DT>(load_chunk_of<DT, WHOLE>(base(p.C, p.ldc), offset(p.ldc), count), c);
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = __builtin_fmaf(p.beta, c[e], v[e]);
   }
-  store_chunk_of<DT, WHOLE>(p.D, row * p.ldd + col, count, v);
+  store_chunk_of<DT, WHOLE>(const_cast<uint16_t *>(base(p.D, p.ldd)), offset(p.ldd), count, v);
 }
 
-// One block tile (W8 = 8: 256 x 256, W8 = 4: 128 x 128; waves of 16 W8 x 16 W8).  Rows of A and B begin on 16 bytes; a tile's
-// rows of either lie within 4 GiB.  The product is formed transposed (B fragment first), so a lane owns row (lane & 15)
+// One block tile (W8 = 8: 256 x 256, 6: 192 x 192, 4: 128 x 128; waves of 16 W8 x 16 W8).  Rows of A and B begin on 16 bytes; a tile's
+// rows of either lie within 4 GiB.  A 192 x 192 tile has room for three buffers of B as well: the tiles of step s + 3 go out
+// behind the barrier of step s, into its buffers, and have two steps to arrive.  The product is formed transposed (B fragment first), so a lane owns row (lane & 15)
 // and four adjacent columns of every 16 x 16 tile.
-template <int DT, bool WHOLE, int W8>
+template <int DT, bool WHOLE, int W8, bool TAIL>
 TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t tile_n, size_t step0, size_t steps, bool tail, float *share) {
-  constexpr int BK = 64, ROWH = BK, CPR = 8, RPT = 8, RS = 1, SUB = 2, NA = 3, NB = 2;
+  constexpr int BK = 64, ROWH = BK, CPR = 8, RPT = 8, RS = 1, SUB = 2, NA = 3, NB = W8 == 6 ? 3 : 2;
   constexpr int TILE = 32 * W8, WT = 16 * W8;
   constexpr int NM = W8 * W8;
   constexpr int OPH = TILE * ROWH;
   constexpr int TPW = TILE / RPT / 4;
   constexpr int TEVERY = NM / 2 / TPW;
   constexpr bool BF16 = DT == kBF16;
-  static_assert(W8 == 8 || W8 == 4, "fragment reads and transfers must fit a substep");
+  static_assert((W8 == 8 || W8 == 6 || W8 == 4) && 4 * W8 <= NM && (NM / 2) % TPW == 0, "fragment reads and transfers must fit a substep");
   __shared__ __attribute__((aligned(1024))) half_t lds_a[NA][OPH];
   __shared__ __attribute__((aligned(1024))) half_t lds_b[NB][OPH];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -75,7 +79,11 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
 #pragma unroll
   for (int i = 0; i < W8; i++)
 #pragma unroll
-    for (int j = 0; j < W8; j++) acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < W8; j++) {
+      // (of 192 x 192 tiles the compiler keeps known zeros apart from the loop's values, and copies those every step)
+      if constexpr (W8 == 6 && !TAIL) acc[i][j] = opaque_zero();
+      else acc[i][j] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
   const int frow = lane & 15, kq = lane >> 4, fsw = (frow >> RS) & (CPR - 1);
   const int fa0 = (wm * WT + frow) * ROWH, fb0 = (wn * WT + frow) * ROWH;
@@ -84,84 +92,12 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
   for (int kk = 0; kk < SUB; kk++) ko[kk] = ((4 * kk + kq) ^ fsw) * 8;
   auto fragment = [](const half_t *q) { return *reinterpret_cast<const uint4_t *>(q); };
 
-  if (steps) {  // the same for the whole block
-    uint32_t off_a[TPW], off_b[TPW];
-#pragma unroll
-    for (int t = 0; t < TPW; t++) {
-      const unsigned row = (unsigned)((wave * TPW + t) * RPT + lane / CPR);
-      const unsigned chunk = (unsigned)(lane % CPR) ^ ((row >> RS) & (CPR - 1));
-      const unsigned ra = row < last_a ? row : last_a, rb = row < last_b ? row : last_b;
-      off_a[t] = (uint32_t)((ra * p.lda + chunk * 8) * 2);
-      off_b[t] = (uint32_t)((rb * p.ldb + chunk * 8) * 2);
-    }
-    constexpr lds_addr_t STAGE = OPH * 2, TBYTES = 1024, STEPB = BK * 2;
-    const char *ga = A + step0 * STEPB, *gb = B + step0 * STEPB;
-    const lds_addr_t ta = wave_uniform(lds_address_of(&lds_a[0][0]) + wave * TPW * TBYTES);
-    const lds_addr_t tb = wave_uniform(lds_address_of(&lds_b[0][0]) + wave * TPW * TBYTES);
-    // steps past the end: a harmless re-read of the last step into a free buffer
-    auto issue_a = [&](size_t step, int buf, int t) { load_chunk_to_lds(ga + (step < steps ? step : steps - 1) * STEPB, off_a[t], ta + buf * STAGE + t * TBYTES); };
-    auto issue_b = [&](size_t step, int buf, int t) { load_chunk_to_lds(gb + (step < steps ? step : steps - 1) * STEPB, off_b[t], tb + buf * STAGE + t * TBYTES); };
-    // in flight at the first barrier: A0 B0 | A1 B1 (the wave's counter returns in issue order)
-#pragma unroll
-    for (int t = 0; t < TPW; t++) issue_a(0, 0, t);
-#pragma unroll
-    for (int t = 0; t < TPW; t++) issue_b(0, 0, t);
-#pragma unroll
-    for (int t = 0; t < TPW; t++) issue_a(1, 1, t);
-#pragma unroll
-    for (int t = 0; t < TPW; t++) issue_b(1, 1, t);
-    wait_vector_loads<2 * TPW>();
-    block_barrier_lds_only();
-    uint4_t fa[2][W8], fb[2][W8];
-#pragma unroll
-    for (int i = 0; i < W8; i++) {
-      fa[0][i] = fragment(&lds_a[0][fa0 + i * 16 * ROWH + ko[0]]);
-      fb[0][i] = fragment(&lds_b[0][fb0 + i * 16 * ROWH + ko[0]]);
-    }
-    int ca = 0, cb = 0;  // s % NA, s % NB
-    for (size_t s = 0; s < steps; s++) {
-      const int na = ca + 1 == NA ? 0 : ca + 1, nb = cb ^ 1;
-      const int fill_a = ca == 0 ? NA - 1 : ca - 1;  // A buffer of step s - 1 = of step s + 2
-      // substep 0: MFMA t works on tile (t / W8, t % W8); the fragments of substep 1 are read under it, the A tile of
-      // step s + 2 goes out under its second half
-#pragma unroll
-      for (int t = 0; t < NM; t++) {
-        if (t < 4 * W8 && t % 2 == 0) {
-          const int k = t / 2;
-          if (k == 0) fa[1][0] = fragment(&lds_a[ca][fa0 + ko[1]]);
-          else if (k <= W8) fb[1][k - 1] = fragment(&lds_b[cb][fb0 + (k - 1) * 16 * ROWH + ko[1]]);
-          else fa[1][k - W8] = fragment(&lds_a[ca][fa0 + (k - W8) * 16 * ROWH + ko[1]]);
-        }
-        if (t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_a(s + 2, fill_a, (t - NM / 2) / TEVERY);
-        acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[0][t % W8], fa[0][t / W8], acc[t / W8][t % W8]);
-        sched_fence();
-      }
-      // substep 1: own transfers of step s + 1 done (the A tile of step s + 2 may still fly), barrier, fragments of step
-      // s + 1; the B tile of step s + 2 into the B buffer of step s
-      wait_vector_loads<TPW>();
-      block_barrier_lds_only();
-      sched_fence();
-#pragma unroll
-      for (int t = 0; t < NM; t++) {
-        if (t < 4 * W8 && t % 2 == 0) {
-          const int k = t / 2;
-          if (k == 0) fa[0][0] = fragment(&lds_a[na][fa0 + ko[0]]);
-          else if (k <= W8) fb[0][k - 1] = fragment(&lds_b[nb][fb0 + (k - 1) * 16 * ROWH + ko[0]]);
-          else fa[0][k - W8] = fragment(&lds_a[na][fa0 + (k - W8) * 16 * ROWH + ko[0]]);
-        }
-        if (t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_b(s + 2, cb, (t - NM / 2) / TEVERY);
-        acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[1][t % W8], fa[1][t / W8], acc[t / W8][t % W8]);
-        sched_fence();
-      }
-      ca = na;
-      cb = nb;
-    }
-    wait_vector_loads<0>();  // the re-reads past the last step must land before the buffers are used for anything else
-  }
-  if (tail) {  // the same for the whole block: the last K % 64, zero-filled, through registers into the first buffers
+  // What is left of K behind the last whole step, zero-filled, through registers into the first buffers.  It comes first, so that
+  // the accumulators run through the loop below and into the epilogue without a branch between them (with one, the compiler
+  // copies all of them every step: 4001 x 2056 x 4096 98 us instead of 75).
+  if (TAIL && tail) {  // the same for the whole block
     const size_t k0 = p.K / BK * BK;
     const int left = (int)(p.K - k0);
-    block_barrier_lds_only();
 #pragma unroll
     for (int t = 0; t < TILE * CPR / 256; t++) {
       const int row = (t * 256 + tid) / CPR, chunk = (t * 256 + tid) % CPR;
@@ -182,55 +118,143 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
 #pragma unroll
       for (int t = 0; t < NM; t++) acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[t % W8], fa[t / W8], acc[t / W8][t % W8]);
     }
+    __syncthreads();  // the buffers are free again
+  }
+  {
+    uint32_t off_a[TPW], off_b[TPW];
+#pragma unroll
+    for (int t = 0; t < TPW; t++) {
+      const unsigned row = (unsigned)((wave * TPW + t) * RPT + lane / CPR);
+      const unsigned chunk = (unsigned)(lane % CPR) ^ ((row >> RS) & (CPR - 1));
+      const unsigned ra = row < last_a ? row : last_a, rb = row < last_b ? row : last_b;
+      off_a[t] = (uint32_t)((ra * p.lda + chunk * 8) * 2);
+      off_b[t] = (uint32_t)((rb * p.ldb + chunk * 8) * 2);
+    }
+    constexpr lds_addr_t STAGE = OPH * 2, TBYTES = 1024, STEPB = BK * 2;
+    const char *ga = A + step0 * STEPB, *gb = B + step0 * STEPB;
+    const lds_addr_t ta = wave_uniform(lds_address_of(&lds_a[0][0]) + wave * TPW * TBYTES);
+    const lds_addr_t tb = wave_uniform(lds_address_of(&lds_b[0][0]) + wave * TPW * TBYTES);
+    // steps past the end: a harmless re-read of the last step into a free buffer
+    auto issue_a = [&](size_t step, int buf, int t) { load_chunk_to_lds(ga + (step < steps ? step : steps - 1) * STEPB, off_a[t], ta + buf * STAGE + t * TBYTES); };
+    auto issue_b = [&](size_t step, int buf, int t) { load_chunk_to_lds(gb + (step < steps ? step : steps - 1) * STEPB, off_b[t], tb + buf * STAGE + t * TBYTES); };
+    // in flight at the first barrier: A0 B0 | A1 B1 (| A2 B2) (the wave's counter returns in issue order)
+#pragma unroll
+    for (int d = 0; d < NB; d++) {
+#pragma unroll
+      for (int t = 0; t < TPW; t++) issue_a(d, d, t);
+#pragma unroll
+      for (int t = 0; t < TPW; t++) issue_b(d, d, t);
+    }
+    wait_vector_loads<2 * TPW * (NB - 1)>();
+    block_barrier_lds_only();
+    uint4_t fa[2][W8], fb[2][W8];
+#pragma unroll
+    for (int i = 0; i < W8; i++) {
+      fa[0][i] = fragment(&lds_a[0][fa0 + i * 16 * ROWH + ko[0]]);
+      fb[0][i] = fragment(&lds_b[0][fb0 + i * 16 * ROWH + ko[0]]);
+    }
+    int ca = 0, cb = 0;  // s % NA, s % NB
+    for (size_t s = 0; s < steps; s++) {
+      const int na = ca + 1 == NA ? 0 : ca + 1, nb = cb + 1 == NB ? 0 : cb + 1;
+      const int fill_a = ca == 0 ? NA - 1 : ca - 1;  // A buffer of step s - 1 = of step s + 2
+      // substep 0: MFMA t works on tile (t / W8, t % W8); the fragments of substep 1 are read under it, the A tile of
+      // step s + 2 goes out under its second half
+#pragma unroll
+      for (int t = 0; t < NM; t++) {
+        if (t < 4 * W8 && t % 2 == 0) {
+          const int k = t / 2;
+          if (k == 0) fa[1][0] = fragment(&lds_a[ca][fa0 + ko[1]]);
+          else if (k <= W8) fb[1][k - 1] = fragment(&lds_b[cb][fb0 + (k - 1) * 16 * ROWH + ko[1]]);
+          else fa[1][k - W8] = fragment(&lds_a[ca][fa0 + (k - W8) * 16 * ROWH + ko[1]]);
+        }
+        if (NB == 2 && t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_a(s + 2, fill_a, (t - NM / 2) / TEVERY);
+        acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[0][t % W8], fa[0][t / W8], acc[t / W8][t % W8]);
+        sched_fence();
+      }
+      // substep 1: own transfers of step s + 1 done (the A tile of step s + 2 may still fly), barrier, fragments of step
+      // s + 1; the B tile of step s + 2 into the B buffer of step s
+      wait_vector_loads<NB == 2 ? TPW : 2 * TPW>();
+      block_barrier_lds_only();
+      sched_fence();
+#pragma unroll
+      for (int t = 0; t < NM; t++) {
+        if (t < 4 * W8 && t % 2 == 0) {
+          const int k = t / 2;
+          if (k == 0) fa[0][0] = fragment(&lds_a[na][fa0 + ko[0]]);
+          else if (k <= W8) fb[0][k - 1] = fragment(&lds_b[nb][fb0 + (k - 1) * 16 * ROWH + ko[0]]);
+          else fa[0][k - W8] = fragment(&lds_a[na][fa0 + (k - W8) * 16 * ROWH + ko[0]]);
+        }
+        if (NB == 2 && t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_b(s + 2, cb, (t - NM / 2) / TEVERY);
+        if (NB == 3 && t % TEVERY == 0) {  // the buffers of step s are free behind the barrier
+          if (t < NM / 2) issue_a(s + 3, ca, t / TEVERY);
+          else issue_b(s + 3, cb, (t - NM / 2) / TEVERY);
+        }
+        acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[1][t % W8], fa[1][t / W8], acc[t / W8][t % W8]);
+        sched_fence();
+      }
+      ca = na;
+      cb = nb;
+    }
+    wait_vector_loads<0>();  // the re-reads past the last step must land before the buffers are used for anything else
   }
   // Epilogue: a row of W8 tiles (16 rows x 16 W8 columns) is turned through LDS, so that a lane finishes 8 adjacent columns of
   // a row and global memory sees whole rows of the wave's tile.
-  constexpr int SROW = 16 * W8 + 4, LPR = 2 * W8, RPA = 64 / LPR;  // floats per parked row, lanes per row, rows per access
+  constexpr int SROW = 16 * W8 + 4, LPR = 2 * W8;                    // floats per parked row, lanes per row
+  constexpr int RPA = 64 / LPR >= 8 ? 8 : 64 / LPR >= 4 ? 4 : 2;     // rows per access; 192 x 192 tiles leave 16 lanes idle
   static_assert(4 * 2 * 16 * SROW * sizeof(float) <= sizeof(lds_a), "parking area of four waves");
   block_barrier_lds_only();  // the other waves have read their last fragments
   float *park = reinterpret_cast<float *>(&lds_a[0][0]) + wave * (2 * 16 * SROW);
-  const int rr = lane / LPR, rc = (lane % LPR) * 8;
-  const size_t col = col0 + wn * WT + rc;
-  const int count = col < p.N ? (int)(p.N - col < 8 ? p.N - col : 8) : 0;
+  const bool active = RPA * LPR == 64 || lane < RPA * LPR;
+  const unsigned rr = active ? lane / LPR : 0, rc = (lane % LPR) * 8;
+  const size_t wave_row = row0 + wave_uniform(wm * WT), wave_col = col0 + wave_uniform(wn * WT);
+  const size_t col = wave_col + rc;
+  const int count = active && col < p.N ? (int)(p.N - col < 8 ? p.N - col : 8) : 0;
+  const bool inside = wave_row + WT <= p.M && wave_col + WT <= p.N;  // the same for the whole wave
   float bias[8] = {};
   if (p.bias && !share) unpack_chunk<DT>(load_chunk_of<DT, WHOLE, false>(p.bias, col, count), bias);
-#pragma unroll
-  for (int i = 0; i < W8; i++) {
+  static_for<W8>([&](auto index) {  // unrolled whatever its size: the accumulators are registers
+    constexpr int i = decltype(index)::value;
     float *buf = park + (i & 1) * (16 * SROW);
 #pragma unroll
     for (int j = 0; j < W8; j++) *reinterpret_cast<float4_t *>(buf + frow * SROW + 16 * j + 4 * kq) = acc[i][j];
     wave_lds_fence();
-#pragma unroll
-    for (int t = 0; t < 16 / RPA; t++) {
-      const int r = t * RPA + rr;
-      const size_t row = row0 + wm * WT + 16 * i + r;
-      if (row >= p.M) continue;
+    auto finish = [&](int t, int n) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 4) {
-        const float4_t q = *reinterpret_cast<const float4_t *>(buf + r * SROW + rc + e);
+        const float4_t q = *reinterpret_cast<const float4_t *>(buf + (t * RPA + rr) * SROW + rc + e);
         v[e] = q[0];
         v[e + 1] = q[1];
         v[e + 2] = q[2];
         v[e + 3] = q[3];
       }
       if (share)
-        store_floats<8, true>(share, row * p.share_ld + col, col < p.share_ld ? 8 : 0, v);  // share_ld: N up to a multiple of 8
+        store_floats<8, true>(share + (wave_row + 16 * i + t * RPA) * p.share_ld + wave_col, rr * (unsigned)p.share_ld + rc, n > 0 ? 8 : 0, v);  // share_ld: N up to a multiple of 8
       else
-        fused_gemm_finish<DT, WHOLE>(p, row, col, count, v, bias);
+        fused_gemm_finish<DT, WHOLE>(p, wave_row + 16 * i + t * RPA, wave_col, rr, rc, n, v, bias);
+    };
+    if (inside) {
+      if (active) {
+#pragma unroll
+        for (int t = 0; t < 16 / RPA; t++) finish(t, 8);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 16 / RPA; t++)
+        if (wave_row + 16 * i + t * RPA + rr < p.M) finish(t, count);
     }
-  }
+  });
 }
 
-template <int DT, bool WHOLE, int W8>
+// K is at least 64, and each split has a whole step at least.  TAIL: K is no multiple of 64.
+template <int DT, bool WHOLE, int W8, bool TAIL>
 __global__ __launch_bounds__(256, W8 == 4 ? 2 : 1) void fused_gemm_tile_kernel(FusedGemmParams p) {
   constexpr int TILE = 32 * W8;
   const unsigned split = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
   size_t tile_m, tile_n;
   gemm_tile_of_block((p.M + TILE - 1) / TILE, (p.N + TILE - 1) / TILE, tile, &tile_m, &tile_n);
-  const size_t full = p.K / 64, per = (full + p.splits - 1) / p.splits;
-  const size_t step0 = split * per < full ? split * per : full, end = step0 + per < full ? step0 + per : full;
-  fused_gemm_tile<DT, WHOLE, W8>(p, tile_m, tile_n, step0, end - step0, split + 1 == p.splits && p.K % 64 != 0, p.shares ? p.shares + (size_t)split * p.M * p.share_ld : nullptr);
+  const size_t full = p.K / 64, step0 = split * full / p.splits, end = (split + 1) * full / p.splits;
+  fused_gemm_tile<DT, WHOLE, W8, TAIL>(p, tile_m, tile_n, step0, end - step0, split + 1 == p.splits, p.shares ? p.shares + (size_t)split * p.M * p.share_ld : nullptr);
 }
 
 // The epilogue over the sum of the shares, one thread per 8 adjacent columns, the shares in order.
@@ -248,7 +272,7 @@ __global__ __launch_bounds__(256) void fused_gemm_join_kernel(FusedGemmParams p)
     for (int e = 0; e < 8; e++) v[e] += w[e];
   }
   if (p.bias) unpack_chunk<DT>(load_chunk_of<DT, WHOLE, false>(p.bias, col, count), bias);
-  fused_gemm_finish<DT, WHOLE>(p, row, col, count, v, bias);
+  fused_gemm_finish<DT, WHOLE>(p, row, col, 0u, 0u, count, v, bias);
 }
 
 // Up to 16 * MT rows: a block of WAVES waves takes 16 columns; wave w takes the K steps of 32 * UNROLL elements w, w + WAVES, ...
@@ -268,20 +292,34 @@ __global__ __launch_bounds__(64 * WAVES) void fused_gemm_few_rows_kernel(FusedGe
   float4_t acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; i++) acc[i] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (size_t s = split * per + wave; s < end; s += WAVES) {
-    uint4_t b[UNROLL], a[MT][UNROLL];
+  uint4_t b[2][UNROLL], a[2][MT][UNROLL];
+  auto load = [&](size_t s, int to) {
 #pragma unroll
     for (int u = 0; u < UNROLL; u++) {
       const size_t k = s * STEP + 32 * u + 8 * kq;
       const int count = k < p.K ? (int)(p.K - k < 8 ? p.K - k : 8) : 0;
-      b[u] = load_chunk_of<DT, WHOLE>(p.B, n * p.ldb + k, count);
+      b[to][u] = load_chunk_of<DT, WHOLE>(p.B, n * p.ldb + k, count);
 #pragma unroll
-      for (int i = 0; i < MT; i++) a[i][u] = load_chunk_of<DT, WHOLE, false>(p.A, (16 * i + frow) * p.lda + k, (size_t)(16 * i + frow) < p.M ? count : 0);
+      for (int i = 0; i < MT; i++) a[to][i][u] = load_chunk_of<DT, WHOLE, false>(p.A, (16 * i + frow) * p.lda + k, (size_t)(16 * i + frow) < p.M ? count : 0);
     }
+  };
+  auto multiply = [&](int from) {
 #pragma unroll
     for (int u = 0; u < UNROLL; u++)
 #pragma unroll
-      for (int i = 0; i < MT; i++) acc[i] = mfma_16x16x32_chunks<BF16>(b[u], a[i][u], acc[i]);  // lane: row (lane & 15), columns 4 (lane >> 4) ...
+      for (int i = 0; i < MT; i++) acc[i] = mfma_16x16x32_chunks<BF16>(b[from][u], a[from][i][u], acc[i]);  // lane: row (lane & 15), columns 4 (lane >> 4) ...
+  };
+  // The wave's steps are numbered 0 ... count - 1 and begin at another one in every block: with all blocks at the same place
+  // along K, rows that are a large power of two apart would all be read from a few memory channels.
+  const size_t first = split * per + wave;
+  const unsigned steps_here = first < end ? (unsigned)((end - first + WAVES - 1) / WAVES) : 0u, turn = steps_here ? blockIdx.x % steps_here : 0u;
+  auto step_at = [&](unsigned i) { return first + (size_t)(i + turn < steps_here ? i + turn : i + turn - steps_here) * WAVES; };
+  if (steps_here) load(step_at(0), 0);
+  for (unsigned i = 0; i < steps_here; i += 2) {  // the next step's chunks are on their way during a step
+    if (i + 1 < steps_here) load(step_at(i + 1), 1);
+    multiply(0);
+    if (i + 2 < steps_here) load(step_at(i + 2), 0);
+    if (i + 1 < steps_here) multiply(1);
   }
 #pragma unroll
   for (int i = 0; i < MT; i++) *reinterpret_cast<float4_t *>(&lds[wave][i][frow][4 * kq]) = acc[i];
@@ -301,7 +339,7 @@ __global__ __launch_bounds__(64 * WAVES) void fused_gemm_few_rows_kernel(FusedGe
       store_floats<8, true>(p.shares, ((size_t)split * p.M + row) * p.share_ld + col, 8, v);
     } else {
       if (p.bias) unpack_chunk<DT>(load_chunk_of<DT, WHOLE, false>(p.bias, col, count), bias);
-      fused_gemm_finish<DT, WHOLE>(p, row, col, count, v, bias);
+      fused_gemm_finish<DT, WHOLE>(p, row, col, 0u, 0u, count, v, bias);
     }
   }
 }
@@ -310,14 +348,15 @@ __global__ __launch_bounds__(64 * WAVES) void fused_gemm_few_rows_kernel(FusedGe
 struct PackRowsParams {
   const uint16_t *from;
   uint16_t *to;
-  size_t rows, width, from_ld, to_ld;
+  size_t rows, width, padded, from_ld, to_ld;  // padded: a multiple of 8; zeros from the width up to there
 };
 __global__ __launch_bounds__(256) inline void pack_rows_kernel(PackRowsParams p) {
-  const size_t chunks = (p.width + 7) / 8, at = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t chunks = p.padded / 8, at = (size_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= p.rows * chunks) return;
   const size_t row = at / chunks, col = at % chunks * 8;
-  const uint4_t c = load_chunk_of<kF16, false>(p.from, row * p.from_ld + col, p.width - col < 8 ? (int)(p.width - col) : 8);
-  *reinterpret_cast<uint4_t *>(p.to + row * p.to_ld + col) = c;  // to_ld: a multiple of 8, so what lies beyond the width is padding
+  const int count = col < p.width ? (p.width - col < 8 ? (int)(p.width - col) : 8) : 0;
+  const uint4_t c = load_chunk_of<kF16, false>(p.from, count ? row * p.from_ld + col : 0, count);
+  *reinterpret_cast<uint4_t *>(p.to + row * p.to_ld + col) = c;
 }
 
 // 64 x 64 tiles turned through LDS.  GRAD: what is turned is dZ = dD * act'(Z), written as it stands as well (dz, which may be
@@ -326,7 +365,7 @@ struct TransposeParams {
   const void *from, *Z;  // dD and Z with GRAD
   void *to, *dz;
   float *partial;        // [row strip][columns]
-  size_t rows, columns, from_ld, z_ld, to_ld, dz_ld;
+  size_t rows, columns, from_ld, z_ld, to_ld, dz_ld;  // to_ld, dz_ld: multiples of 64
   unsigned column_tiles;
   int act;
 };
@@ -355,7 +394,7 @@ __global__ __launch_bounds__(256) void transpose_kernel(TransposeParams p) {
         for (int e = 0; e < 8; e++) d[e] = e < count ? d[e] * slope[e] : 0.0f;
         c = pack_chunk<DT>(d);
       }
-      if (p.dz) store_chunk_of<DT, false>(p.dz, count ? row * p.dz_ld + col : 0, count, d);
+      if (p.dz && row < p.rows) store_chunk_of<DT, true>(p.dz, row * p.dz_ld + col, 8, d);  // its rows end in zeros
 #pragma unroll
       for (int e = 0; e < 8; e++) s[e] += d[e];
     }
@@ -380,11 +419,11 @@ __global__ __launch_bounds__(256) void transpose_kernel(TransposeParams p) {
   for (int h = 0; h < 2; h++) {  // row tr (+ 32) of the transpose: 8 chunks of 8 of the tile's rows
     const int r = h * 32 + tr;
     const size_t row = col0 + r, col = row0 + tc;
-    if (row >= p.columns || col >= p.rows) continue;
+    if (row >= p.columns) continue;  // the rows of the transpose end in zeros up to a multiple of 64
     uint4_t c;
 #pragma unroll
     for (int e = 0; e < 4; e++) c[e] = (unsigned)lds[(tc + 2 * e) * LD + r] | (unsigned)lds[(tc + 2 * e + 1) * LD + r] << 16;
-    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(p.to) + row * p.to_ld + col) = c;  // to_ld: a multiple of 8
+    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(p.to) + row * p.to_ld + col) = c;
   }
 }
 

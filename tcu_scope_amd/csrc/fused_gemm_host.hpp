@@ -13,6 +13,8 @@ namespace tcu {
 constexpr size_t kGemmFewRows = 64;               // up to this many rows the product is bound by reading B
 constexpr size_t kGemmMaxInner = (size_t)1 << 22; // a tile's rows of an operand lie within 32-bit byte offsets: 256 * 2^22 * 2 < 2^32
 
+constexpr size_t kGemmMaxLd = (size_t)1 << 28;    // 8 rows of an output lie within 32-bit offsets
+
 inline size_t up_to(size_t n, size_t step) { return (n + step - 1) / step * step; }
 // bytes of a part of a workspace
 inline size_t part_bytes(size_t bytes) { return up_to(bytes, 256); }
@@ -20,11 +22,24 @@ inline size_t part_bytes(size_t bytes) { return up_to(bytes, 256); }
 // How one product M x N over K runs, and what it takes of the workspace.
 struct GemmPlan {
   bool few_rows = false;
-  int few_tiles = 1;           // few rows: 16-row tiles
-  bool big = false;            // 256 x 256 tiles, else 128 x 128
+  int few_tiles = 1;  // few rows: 16-row tiles
+  int w8 = 8;         // block tiles of 32 w8 rows and columns
   size_t tiles = 0, splits = 1;
   size_t share_ld = 0, share_bytes = 0;
 };
+// The time of a tiling in microseconds: rounds of blocks over the compute units, each as long as its K steps (64 elements)
+// plus what a block spends before and after them, and the pass that joins split sums.  Measured with 8192 x 8192 x 4096 and
+// 4001 x 2056 x 4096 bf16: a step of a 256 x 256 tile takes a compute unit 1.5 us, of 192 x 192 0.9, and of two 128 x 128
+// tiles side by side 0.95.
+inline double gemm_tiling_us(size_t tiles, size_t splits, int w8, size_t M, size_t N, size_t K) {
+  const double step = w8 == 8 ? 1.5 : w8 == 6 ? 0.9 : 0.95, around = w8 == 8 ? 12.0 : w8 == 6 ? 8.0 : 6.0;
+  const size_t at_once = w8 == 4 ? 512 : 256, blocks = tiles * splits;
+  const double steps = (double)((K + 63) / 64 + splits - 1) / (double)splits;
+  const double alone = w8 == 4 && blocks <= 256 ? 0.65 : 1.0;  // a 128 x 128 tile that has its compute unit to itself
+  double us = (double)((blocks + at_once - 1) / at_once) * (steps * step * alone + around);
+  if (splits > 1) us += 5.0 + (double)splits * (double)M * (double)N * 8.0 / 4.0e6;
+  return us;
+}
 inline GemmPlan plan_gemm(size_t M, size_t N, size_t K) {
   GemmPlan g;
   g.share_ld = up_to(N, 8);
@@ -36,12 +51,18 @@ inline GemmPlan plan_gemm(size_t M, size_t N, size_t K) {
     const size_t steps = K / 1024;
     while (g.tiles * g.splits < 256 && g.splits * 2 <= steps) g.splits *= 2;
   } else {
-    const size_t t256 = (M + 255) / 256 * ((N + 255) / 256), t128 = (M + 127) / 128 * ((N + 127) / 128);
-    g.big = t256 >= 128;
-    g.tiles = g.big ? t256 : t128;
-    const size_t steps = K / 64;
-    if (!g.big)
-      while (g.tiles * g.splits * 2 <= 512 && g.splits * 2 * 4 <= steps) g.splits *= 2;
+    double best = 0.0;
+    for (int w8 : {8, 6, 4}) {
+      const size_t t = 32 * (size_t)w8, tiles = (M + t - 1) / t * ((N + t - 1) / t);
+      for (size_t splits = 1; splits <= 16 && (splits == 1 || (splits * 4 <= K / 64 && tiles * splits <= 512)); splits++) {
+        const double us = gemm_tiling_us(tiles, splits, w8, M, N, K);
+        if (g.tiles != 0 && us >= best) continue;
+        best = us;
+        g.w8 = w8;
+        g.tiles = tiles;
+        g.splits = splits;
+      }
+    }
   }
   if (g.splits > 1) g.share_bytes = part_bytes(g.splits * M * g.share_ld * 4);
   return g;
@@ -55,19 +76,23 @@ inline void launch_gemm(const GemmPlan &g, FusedGemmParams p, float *shares, boo
   p.share_ld = g.share_ld;
   p.shares = g.splits > 1 ? shares : nullptr;
   const unsigned grid = (unsigned)(g.tiles * g.splits);
-  if (g.few_rows) {
+  if (p.K == 0) {  // nothing to add up: the epilogue over a sum of no shares
+    p.splits = 0;
+  } else if (g.few_rows) {
 #define TCU_FEW(MT, UNROLL) \
   (WHOLE && whole_inner ? launch(fused_gemm_few_rows_kernel<DT, WHOLE, MT, 8, UNROLL>, grid, 512u, stream, p) : launch(fused_gemm_few_rows_kernel<DT, false, MT, 8, UNROLL>, grid, 512u, stream, p))
     if (g.few_tiles == 1) TCU_FEW(1, 4);
     else if (g.few_tiles == 2) TCU_FEW(2, 4);
     else TCU_FEW(4, 2);
 #undef TCU_FEW
-  } else if (g.big) {
-    launch(fused_gemm_tile_kernel<DT, WHOLE, 8>, grid, 256u, stream, p);
   } else {
-    launch(fused_gemm_tile_kernel<DT, WHOLE, 4>, grid, 256u, stream, p);
+#define TCU_TILES(W8) (p.K % 64 ? launch(fused_gemm_tile_kernel<DT, WHOLE, W8, true>, grid, 256u, stream, p) : launch(fused_gemm_tile_kernel<DT, WHOLE, W8, false>, grid, 256u, stream, p))
+    if (g.w8 == 8) TCU_TILES(8);
+    else if (g.w8 == 6) TCU_TILES(6);
+    else TCU_TILES(4);
+#undef TCU_TILES
   }
-  if (g.splits > 1) launch(fused_gemm_join_kernel<DT, WHOLE>, (unsigned)((p.M * (g.share_ld / 8) + 255) / 256), 256u, stream, p);
+  if (p.splits != 1) launch(fused_gemm_join_kernel<DT, WHOLE>, (unsigned)((p.M * (g.share_ld / 8) + 255) / 256), 256u, stream, p);
 }
 inline void run_gemm(int dtype, bool whole, const GemmPlan &g, const FusedGemmParams &p, float *shares, bool whole_inner, void *stream) {
   if (dtype == TCU_F16) {
@@ -86,9 +111,12 @@ inline int check_gemm_shape(const std::string &w, const tcu_fused_gemm_shape *s)
   if (!s) return report_failure(TCU_ERR_INVALID_ARG, w + ": null shape");
   if (s->dtype != TCU_F16 && s->dtype != TCU_BF16) return report_failure(TCU_ERR_INVALID_ARG, w + ": dtype must be TCU_F16 or TCU_BF16");
   if (!known_activation(s->activation)) return report_failure(TCU_ERR_INVALID_ARG, w + ": unknown activation");
-  const size_t most = (size_t)1 << 31;
-  if (s->M >= most || s->N >= most || s->K > kGemmMaxInner) return report_failure(TCU_ERR_UNSUPPORTED, w + ": M or N from 2^31 on, or K above 2^22");
+  if (s->M >= (size_t)1 << 31 || s->N > kGemmMaxLd || s->K > kGemmMaxInner) return report_failure(TCU_ERR_UNSUPPORTED, w + ": M from 2^31 on, N above 2^28, or K above 2^22");
   return TCU_OK;
+}
+inline int check_output(const std::string &w, const char *name, const void *p, size_t ld, size_t rows, size_t width, int dtype, bool *whole) {
+  if (ld > kGemmMaxLd) return report_failure(TCU_ERR_UNSUPPORTED, w + ": the leading dimension of " + name + " is above 2^28");
+  return check_matrix(w, name, p, ld, rows, width, dtype, whole);
 }
 // grids are counted in 32 bits: the smallest tiles any of the kernels may use
 inline int check_gemm_grid(const std::string &w, size_t M, size_t N) {
@@ -97,9 +125,10 @@ inline int check_gemm_grid(const std::string &w, size_t M, size_t N) {
   return TCU_OK;
 }
 
-inline void pack_rows(const void *from, size_t from_ld, void *to, size_t to_ld, size_t rows, size_t width, void *stream) {
-  const PackRowsParams q{static_cast<const uint16_t *>(from), static_cast<uint16_t *>(to), rows, width, from_ld, to_ld};
-  launch(pack_rows_kernel, (unsigned)((rows * ((width + 7) / 8) + 255) / 256), 256u, stream, q);
+// padded: a multiple of 8 from the width up to to_ld; the rows end in zeros up to there
+inline void pack_rows(const void *from, size_t from_ld, void *to, size_t to_ld, size_t rows, size_t width, size_t padded, void *stream) {
+  const PackRowsParams q{static_cast<const uint16_t *>(from), static_cast<uint16_t *>(to), rows, width, padded, from_ld, to_ld};
+  launch(pack_rows_kernel, (unsigned)((rows * (padded / 8) + 255) / 256), 256u, stream, q);
 }
 
 inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, size_t lda, const void *B, size_t ldb, const void *bias, const void *C, size_t ldc, void *D, size_t ldd, void *Z, size_t ldz,
@@ -109,8 +138,9 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   if (int rc = check_gemm_grid(w, s->M, s->N)) return rc;
   const size_t M = s->M, N = s->N, K = s->K;
   const GemmPlan g = plan_gemm(M, N, K);
-  const bool pack_a = !g.few_rows && K && !rows_ready(A, M > 1 ? lda : 8), pack_b = !g.few_rows && K && !rows_ready(B, N > 1 ? ldb : 8);
-  const size_t ldk = up_to(K, 8), a_bytes = pack_a ? part_bytes(M * ldk * 2) : 0, b_bytes = pack_b ? part_bytes(N * ldk * 2) : 0;
+  const bool few_k = K > 0 && K < 64;  // the tile kernels want a whole step
+  const bool pack_a = !g.few_rows && K && (few_k || !rows_ready(A, M > 1 ? lda : 8)), pack_b = !g.few_rows && K && (few_k || !rows_ready(B, N > 1 ? ldb : 8));
+  const size_t ldk = few_k ? 64 : up_to(K, 8), a_bytes = pack_a ? part_bytes(M * ldk * 2) : 0, b_bytes = pack_b ? part_bytes(N * ldk * 2) : 0;
   const size_t bytes = g.share_bytes + a_bytes + b_bytes, need = bytes < 256 ? 256 : bytes;
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
   if (!workspace) {
@@ -126,9 +156,9 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
     if (int rc = check_matrix(w, "d_A", A, lda, M, K, s->dtype, &whole_inner)) return rc;
   if (K)
     if (int rc = check_matrix(w, "d_B", B, ldb, N, K, s->dtype, &whole_inner)) return rc;
-  if (int rc = check_matrix(w, "d_D", D, ldd, M, N, s->dtype, &whole)) return rc;
-  if (int rc = use_c ? check_matrix(w, "d_C", C, ldc, M, N, s->dtype, &whole) : TCU_OK) return rc;
-  if (int rc = Z ? check_matrix(w, "d_Z", Z, ldz, M, N, s->dtype, &whole) : TCU_OK) return rc;
+  if (int rc = check_output(w, "d_D", D, ldd, M, N, s->dtype, &whole)) return rc;
+  if (int rc = use_c ? check_output(w, "d_C", C, ldc, M, N, s->dtype, &whole) : TCU_OK) return rc;
+  if (int rc = Z ? check_output(w, "d_Z", Z, ldz, M, N, s->dtype, &whole) : TCU_OK) return rc;
   if (int rc = check_vector(w, "d_bias", bias, 2, &whole)) return rc;
   if (D == A || D == B || D == Z || (Z && (Z == A || Z == B || (use_c && Z == C)))) return report_failure(TCU_ERR_INVALID_ARG, w + ": an output in the place of an operand other tiles still read, or of another output");
   char *at = static_cast<char *>(workspace) + g.share_bytes;
@@ -136,7 +166,7 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   p.A = A;
   p.lda = lda;
   if (pack_a) {
-    pack_rows(A, lda, at, ldk, M, K, stream);
+    pack_rows(A, lda, at, ldk, M, K, few_k ? 64 : up_to(K, 8), stream);
     p.A = at;
     p.lda = ldk;
     at += a_bytes;
@@ -144,7 +174,7 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   p.B = B;
   p.ldb = ldb;
   if (pack_b) {
-    pack_rows(B, ldb, at, ldk, N, K, stream);
+    pack_rows(B, ldb, at, ldk, N, K, few_k ? 64 : up_to(K, 8), stream);
     p.B = at;
     p.ldb = ldk;
   }
@@ -157,7 +187,7 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   p.ldz = ldz;
   p.M = M;
   p.N = N;
-  p.K = K;
+  p.K = pack_a && few_k ? 64 : K;
   p.beta = s->beta;
   p.act = s->activation;
   run_gemm(s->dtype, whole, g, p, static_cast<float *>(workspace), whole_inner, stream);
@@ -183,10 +213,11 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
     if (int rc = check_gemm_grid(w, mn.first, mn.second)) return rc;
   const bool act = s->activation != TCU_ACT_NONE;
   if (act && !Z) return report_failure(TCU_ERR_INVALID_ARG, w + ": the gradient of an activation needs d_Z");
-  const size_t ldm = up_to(M, 8), ldn = up_to(N, 8);
+  // the copies' rows end in zeros up to a whole step of the tile kernels
+  const size_t ldm = up_to(M, 64), ldn = up_to(N, 64);
   const GemmPlan ga = plan_gemm(M, K, N), gb = plan_gemm(N, K, M);
   // the gradient of the activation's argument: dD itself where there is no activation and its rows are ready
-  const bool own_dz = dA && (act || !rows_ready(dD, M > 1 ? lddd : 8));
+  const bool own_dz = dA && (act || N % 64 != 0 || !rows_ready(dD, M > 1 ? lddd : 8));
   const size_t dz_bytes = own_dz ? part_bytes(M * ldn * 2) : 0, dzt_bytes = dB ? part_bytes(N * ldm * 2) : 0, at_bytes = dB ? part_bytes(K * ldm * 2) : 0, bt_bytes = dA ? part_bytes(K * ldn * 2) : 0;
   const size_t strips = (M + 63) / 64, sums_bytes = dbias ? part_bytes(strips * N * 4) : 0;
   const size_t share_bytes = (dA ? ga.share_bytes : 0) > (dB ? gb.share_bytes : 0) ? ga.share_bytes : (dB ? gb.share_bytes : 0);
@@ -207,9 +238,9 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   if (dA && N && K)
     if (int rc = check_matrix(w, "d_B", B, ldb, N, K, s->dtype, &ignored)) return rc;
   if (dA && M && K)
-    if (int rc = check_matrix(w, "d_dA", dA, ldda, M, K, s->dtype, &whole_a)) return rc;
+    if (int rc = check_output(w, "d_dA", dA, ldda, M, K, s->dtype, &whole_a)) return rc;
   if (dB && N && K)
-    if (int rc = check_matrix(w, "d_dB", dB, lddb, N, K, s->dtype, &whole_b)) return rc;
+    if (int rc = check_output(w, "d_dB", dB, lddb, N, K, s->dtype, &whole_b)) return rc;
   if (int rc = check_vector(w, "d_dbias", dbias, 4, &ignored)) return rc;
   if ((dA && (dA == dD || dA == A || dA == B || dA == Z || dA == dB)) || (dB && (dB == dD || dB == A || dB == B || dB == Z)))
     return report_failure(TCU_ERR_INVALID_ARG, w + ": a gradient in the place of an operand, or of another gradient");
@@ -268,8 +299,8 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
     p.D = dA;
     p.ldd = ldda;
     p.M = M;
-    p.K = N;
-    run_gemm(s->dtype, whole_a, ga, p, shares, N % 8 == 0, stream);
+    p.K = ldn;
+    run_gemm(s->dtype, whole_a, ga, p, shares, true, stream);
   }
   if (dB && N && K) {
     if (M) {
@@ -289,8 +320,8 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
     p.D = dB;
     p.ldd = lddb;
     p.M = N;
-    p.K = M;
-    run_gemm(s->dtype, whole_b, gb, p, shares, M % 8 == 0, stream);
+    p.K = ldm;
+    run_gemm(s->dtype, whole_b, gb, p, shares, true, stream);
   }
   return TCU_OK;
 }

@@ -101,7 +101,7 @@ inline void launch_fused_norm_backward(const FusedNormBackParams &p, size_t bloc
   else if (ct <= 2) TCU_NORM(false, 2, 1, 2);
   else if (ct <= 4) TCU_NORM(false, 4, 1, 4);
   else if (ct <= 8) TCU_NORM(false, 8, 1, 8);
-  else if (ct <= 16) TCU_NORM(true, 8, 2, 8);
+  else if (ct <= 16) TCU_NORM(DT != kF32, 8, 2, 8);  // two chunks of fp32 are as many values as one of 16 bits
   else if (ct <= 32) TCU_NORM(true, 8, 4, 8);
   else TCU_NORM(true, 8, DT == kF32 ? 8 : 4, 8);  // 16-bit types end at ct = 32
 #undef TCU_NORM

@@ -27,6 +27,7 @@ inline void store_at(char *base, unsigned offset, uint4_t v) {
   if (WHOLE) *reinterpret_cast<uint4_t *>(base + offset) = v;
   else *reinterpret_cast<any_chunk_t *>(base + offset) = v;
 }
+inline float4_t opaque_zero() { return float4_t{0.0f, 0.0f, 0.0f, 0.0f}; }
 inline void keep_packed(uint4_t &) {}
 inline uint16_t bf16_bits(float v) {
   unsigned u = __float_as_uint(v);

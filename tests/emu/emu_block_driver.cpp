@@ -63,21 +63,22 @@ template <int DT, int W8>
 void emu_tiles(tcu::FusedGemmParams p) {
   const size_t tile = 32 * W8;
   p.tiles = (unsigned)((p.M + tile - 1) / tile * ((p.N + tile - 1) / tile));
-  tcu::launch(tcu::fused_gemm_tile_kernel<DT, false, W8>, p.tiles * p.splits, 256u, nullptr, p);
+  if (p.K % 64) tcu::launch(tcu::fused_gemm_tile_kernel<DT, false, W8, true>, p.tiles * p.splits, 256u, nullptr, p);
+  else tcu::launch(tcu::fused_gemm_tile_kernel<DT, false, W8, false>, p.tiles * p.splits, 256u, nullptr, p);
   if (p.splits > 1) tcu::launch(tcu::fused_gemm_join_kernel<DT, false>, (unsigned)((p.M * (p.share_ld / 8) + 255) / 256), 256u, nullptr, p);
 }
 }  // namespace
 
 extern "C" {
-// the tile kernels at sizes at which the library would not take them; rows of A and B begin on 16 bytes
+// the tile kernels at sizes at which the library would not take them; rows of A and B begin on 16 bytes, K is at least 64 for every split
 int emu_fused_gemm_tiles(int w8, unsigned splits, int dtype, int act, size_t M, size_t N, size_t K, float beta, const void *A, size_t lda, const void *B, size_t ldb, const void *bias, const void *C, size_t ldc,
                          void *D, size_t ldd, void *Z, size_t ldz, float *shares) {
   tcu::FusedGemmParams p{};
   p.A = A; p.lda = lda; p.B = B; p.ldb = ldb; p.bias = bias; p.C = C; p.ldc = ldc; p.D = D; p.ldd = ldd; p.Z = Z; p.ldz = ldz;
   p.M = M; p.N = N; p.K = K; p.beta = beta; p.act = act; p.splits = splits; p.share_ld = tcu::up_to(N, 8);
   p.shares = splits > 1 ? shares : nullptr;
-  if (dtype == TCU_F16) w8 == 8 ? emu_tiles<tcu::kF16, 8>(p) : emu_tiles<tcu::kF16, 4>(p);
-  else w8 == 8 ? emu_tiles<tcu::kBF16, 8>(p) : emu_tiles<tcu::kBF16, 4>(p);
+  if (dtype == TCU_F16) w8 == 8 ? emu_tiles<tcu::kF16, 8>(p) : w8 == 6 ? emu_tiles<tcu::kF16, 6>(p) : emu_tiles<tcu::kF16, 4>(p);
+  else w8 == 8 ? emu_tiles<tcu::kBF16, 8>(p) : w8 == 6 ? emu_tiles<tcu::kBF16, 6>(p) : emu_tiles<tcu::kBF16, 4>(p);
   return 0;
 }
 }

@@ -603,6 +603,8 @@ GEMMS = [
     (70, 130, 200, 8, "gelu", True, False, True),
     (129, 40, 37, 0, "none", False, True, False),
     (66, 9, 1100, 3, "sigmoid", True, True, False),
+    (70, 20, 0, 0, "silu", True, True, True),
+    (80, 30, 1, 0, "none", True, False, False),
 ]
 
 
@@ -633,7 +635,7 @@ def test_fused_gemm(emu, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("w8,splits,M,N,K", [(4, 1, 130, 250, 136), (4, 3, 140, 100, 330), (8, 1, 300, 257, 208), (8, 2, 256, 40, 61), (8, 1, 33, 300, 448), (4, 5, 100, 30, 128)])
+@pytest.mark.parametrize("w8,splits,M,N,K", [(4, 1, 130, 250, 136), (4, 3, 140, 100, 330), (8, 1, 300, 257, 208), (8, 2, 256, 40, 190), (8, 1, 33, 300, 448), (4, 2, 100, 30, 128), (6, 1, 200, 193, 150), (6, 2, 192, 384, 256)])
 def test_fused_gemm_tiles(emu, dtype, w8, splits, M, N, K):
     emu = gemm_emu(emu)
     rng = np.random.default_rng(M)
@@ -650,7 +652,7 @@ def test_fused_gemm_tiles(emu, dtype, w8, splits, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("M,N,K,gap,name", [(1, 1, 1, 0, "silu"), (70, 100, 72, 0, "silu"), (130, 8, 65, 1, "gelu"), (9, 67, 130, 0, "none"), (100, 16, 24, 3, "none"), (40, 80, 16, 8, "sigmoid"), (0, 5, 9, 0, "relu"), (66, 70, 68, 0, "relu")])
+@pytest.mark.parametrize("M,N,K,gap,name", [(1, 1, 1, 0, "silu"), (70, 100, 72, 0, "silu"), (130, 8, 65, 1, "gelu"), (9, 67, 130, 0, "none"), (100, 16, 24, 3, "none"), (40, 80, 16, 8, "sigmoid"), (0, 5, 9, 0, "relu"), (66, 70, 68, 0, "relu"), (70, 0, 72, 0, "none"), (3, 0, 8, 0, "none")])
 def test_fused_gemm_gradient(emu, dtype, M, N, K, gap, name):
     emu = gemm_emu(emu)
     rng = np.random.default_rng(M + N)
@@ -708,6 +710,7 @@ def test_fused_gemm_refusals(emu):
     assert fwd(dtype=2) == 1 and "dtype" in err()
     assert fwd(activation=9) == 1 and "activation" in err()
     assert fwd(K=(1 << 22) + 1) == 2 and fwd(M=1 << 31) == 2 and fwd(M=1 << 30, N=1 << 30) == 2
+    assert fwd(N=(1 << 28) + 1) == 2 and fwd(D=(p, (1 << 28) + 8)) == 2 and "leading dimension" in err()
     assert fwd(have=None) == 1 and fwd(have=sz(16)) == 4 and fwd(ws=ws0 + 8) == 1
     assert fwd(beta=1.0) == 1 and "beta without d_C" in err()
     assert fwd(A=(None, 8)) == 1 and "d_A" in err()
