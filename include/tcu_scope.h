@@ -366,7 +366,7 @@ typedef struct {
 } tcu_fused_gemm_shape;
 
 /* The size query (d_workspace NULL) goes by the same arguments as the call: operands whose rows do not begin on 16 bytes are
- * laid out anew in the workspace where the output has more than 64 rows. */
+ * laid out anew in the workspace where the output has more than 32 rows. */
 int tcu_fused_gemm(const tcu_fused_gemm_shape *shape, const void *d_A, size_t lda, const void *d_B, size_t ldb, const void *d_bias, const void *d_C, size_t ldc, void *d_D, size_t ldd, void *d_Z, size_t ldz, void *d_workspace, size_t *workspace_bytes, void *stream);
 
 /* The gradient: with dZ = dD act'(Z) (TCU_ACT_NONE: dD, and d_Z is not read), dA = dZ B^T (M x K), dB (N rows of K) = dZ^T A and

@@ -3,7 +3,7 @@
 //
 // Gradient: dZ = dD * act'(Z) element by element, dA = dZ B^T (M x K), dB = dZ^T A (N rows of K), dbias = the column sums of
 // dZ, dC = beta dD.  The two products sum over N and over M, along which B and A (and dZ for the second) are not contiguous:
-// they run on transposed copies, which one pass each writes into the workspace; dZ and its transpose come out of the same pass.
+// they run on transposed copies in the workspace, which one launch writes, dZ and its transpose in the same pass.
 //
 //   fused_gemm_tile_kernel : many rows.  256 x 256 or 128 x 128 block tiles on 16x16x32 MFMAs, K steps of 64, operands moved
 //                global -> LDS by transfers that run two steps ahead (three buffers for A, two for B), the loop of
@@ -11,7 +11,7 @@
 //                not stored), K too (a step with what is left of K goes through registers, zero-filled).
 //                Bound by the matrix unit.  Where the tiles are fewer than the compute units, several blocks share a tile's
 //                K steps and fused_gemm_join_kernel adds their fp32 shares in a fixed order.
-//   fused_gemm_few_rows_kernel : up to 64 rows.  Bound by reading B once: a block takes 16 columns of the output and all rows,
+//   fused_gemm_few_rows_kernel : up to 32 rows.  Bound by reading B once: a block takes 16 columns of the output and all rows,
 //                its waves share K and meet in LDS.
 // Sums are fp32; the epilogue is applied to the fp32 sum and each result rounded once.  dZ is rounded to the operands' type,
 // because the matrix unit takes operands of 16 bits; its column sums are taken before that.
@@ -103,8 +103,12 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
       const int row = (t * 256 + tid) / CPR, chunk = (t * 256 + tid) % CPR;
       const unsigned ra = (unsigned)row < last_a ? (unsigned)row : last_a, rb = (unsigned)row < last_b ? (unsigned)row : last_b;
       const int slot = row * ROWH + (chunk ^ ((row >> RS) & (CPR - 1))) * 8;
-      *reinterpret_cast<uint4_t *>(&lds_a[0][slot]) = load_chunk_of<DT, false>(A, ra * p.lda + k0 + chunk * 8, left - chunk * 8);
-      *reinterpret_cast<uint4_t *>(&lds_b[0][slot]) = load_chunk_of<DT, false>(B, rb * p.ldb + k0 + chunk * 8, left - chunk * 8);
+      // K is a multiple of 8, so a chunk is there or is not; one that is not reads the first of the step instead
+      const bool there = chunk * 8 < left;
+      const size_t k = k0 + (there ? chunk * 8 : 0);
+      const uint4_t ca = *reinterpret_cast<const uint4_t *>(A + (ra * p.lda + k) * 2), cb = *reinterpret_cast<const uint4_t *>(B + (rb * p.ldb + k) * 2), none = {0u, 0u, 0u, 0u};
+      *reinterpret_cast<uint4_t *>(&lds_a[0][slot]) = there ? ca : none;
+      *reinterpret_cast<uint4_t *>(&lds_b[0][slot]) = there ? cb : none;
     }
     __syncthreads();
 #pragma unroll
@@ -246,7 +250,7 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
   });
 }
 
-// K is at least 64, and each split has a whole step at least.  TAIL: K is no multiple of 64.
+// K is at least 64 and a multiple of 8, and each split has a whole step at least.  TAIL: K is no multiple of 64.
 template <int DT, bool WHOLE, int W8, bool TAIL>
 __global__ __launch_bounds__(256, W8 == 4 ? 2 : 1) void fused_gemm_tile_kernel(FusedGemmParams p) {
   constexpr int TILE = 32 * W8;
@@ -359,42 +363,47 @@ __global__ __launch_bounds__(256) inline void pack_rows_kernel(PackRowsParams p)
   *reinterpret_cast<uint4_t *>(p.to + row * p.to_ld + col) = c;
 }
 
-// 64 x 64 tiles turned through LDS.  GRAD: what is turned is dZ = dD * act'(Z), written as it stands as well (dz, which may be
-// null), with the column sums of each 64-row strip before rounding (partial, may be null).
+// 64 x 64 tiles turned through LDS.  The first job turns dZ = dD act'(Z), which is written
+// as it stands as well (dz, which may be null), and adds up the columns of each 64-row strip of it before it is rounded.
+struct TransposeJob {
+  const void *from;
+  void *to;                      // null: nothing is turned
+  size_t rows, columns, from_ld, to_ld;  // to_ld: a multiple of 64; the rows of the transpose end in zeros up to that
+  unsigned column_tiles, tiles;
+};
 struct TransposeParams {
-  const void *from, *Z;  // dD and Z with GRAD
-  void *to, *dz;
-  float *partial;        // [row strip][columns]
-  size_t rows, columns, from_ld, z_ld, to_ld, dz_ld;  // to_ld, dz_ld: multiples of 64
-  unsigned column_tiles;
+  TransposeJob job[3];  // dD (of bf16 or fp16), then A and B, whose bits move as they are
+  const void *Z;        // null: no activation
+  void *dz;
+  float *partial;       // [row strip][columns of dD], or null
+  size_t z_ld, dz_ld;   // dz_ld: a multiple of 64
   int act;
 };
+
 template <int DT, bool GRAD>
-__global__ __launch_bounds__(256) void transpose_kernel(TransposeParams p) {
+TCU_DEVICE void transpose_tile(const TransposeParams &p, const TransposeJob &j, unsigned tile, uint16_t *lds, float *sums) {
   constexpr int LD = 66;  // 16-bit elements per LDS row: 33 words, so a column of 16-bit pairs falls into different banks
-  __shared__ __attribute__((aligned(16))) uint16_t lds[64 * LD];
-  __shared__ float sums[GRAD ? 32 * 64 : 1];
-  const size_t row0 = (size_t)(blockIdx.x / p.column_tiles) * 64, col0 = (size_t)(blockIdx.x % p.column_tiles) * 64;
+  const size_t row0 = (size_t)(tile / j.column_tiles) * 64, col0 = (size_t)(tile % j.column_tiles) * 64;
   const int tid = (int)threadIdx.x, tr = tid / 8, tc = (tid % 8) * 8;  // 32 rows of 8 chunks a round
   float s[8] = {};
 #pragma unroll
   for (int h = 0; h < 2; h++) {
     const int r = h * 32 + tr;
     const size_t row = row0 + r, col = col0 + tc;
-    const int count = row < p.rows && col < p.columns ? (p.columns - col < 8 ? (int)(p.columns - col) : 8) : 0;
-    uint4_t c = load_chunk_of<DT, false>(p.from, count ? row * p.from_ld + col : 0, count);
+    const int count = row < j.rows && col < j.columns ? (j.columns - col < 8 ? (int)(j.columns - col) : 8) : 0;
+    uint4_t c = load_chunk_of<DT, false>(j.from, count ? row * j.from_ld + col : 0, count);
     if constexpr (GRAD) {
-      float d[8], z[8];
+      float d[8];
       unpack_chunk<DT>(c, d);
       if (p.Z) {
+        float z[8], value[8], slope[8];
         unpack_chunk<DT>(load_chunk_of<DT, false>(p.Z, count ? row * p.z_ld + col : 0, count), z);
-        float value[8], slope[8];
         activate_slope<false>(p.act, z, value, slope);
 #pragma unroll
         for (int e = 0; e < 8; e++) d[e] = e < count ? d[e] * slope[e] : 0.0f;
         c = pack_chunk<DT>(d);
       }
-      if (p.dz && row < p.rows) store_chunk_of<DT, true>(p.dz, row * p.dz_ld + col, 8, d);  // its rows end in zeros
+      if (p.dz && row < j.rows) store_packed<DT, true>(p.dz, row * p.dz_ld + col, 8, c);  // its rows end in zeros
 #pragma unroll
       for (int e = 0; e < 8; e++) s[e] += d[e];
     }
@@ -407,24 +416,39 @@ __global__ __launch_bounds__(256) void transpose_kernel(TransposeParams p) {
   }
   __syncthreads();
   if constexpr (GRAD) {
-    if (p.partial && tid < 64 && col0 + tid < p.columns) {
+    if (p.partial && tid < 64 && col0 + tid < j.columns) {
       float t = 0.0f;
 #pragma unroll
       for (int r = 0; r < 32; r++) t += sums[r * 64 + tid];
-      p.partial[row0 / 64 * p.columns + col0 + tid] = t;
+      p.partial[row0 / 64 * j.columns + col0 + tid] = t;
     }
   }
-  if (!p.to) return;
+  if (!j.to) return;
 #pragma unroll
   for (int h = 0; h < 2; h++) {  // row tr (+ 32) of the transpose: 8 chunks of 8 of the tile's rows
     const int r = h * 32 + tr;
     const size_t row = col0 + r, col = row0 + tc;
-    if (row >= p.columns) continue;  // the rows of the transpose end in zeros up to a multiple of 64
+    if (row >= j.columns) continue;
     uint4_t c;
 #pragma unroll
     for (int e = 0; e < 4; e++) c[e] = (unsigned)lds[(tc + 2 * e) * LD + r] | (unsigned)lds[(tc + 2 * e + 1) * LD + r] << 16;
-    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(p.to) + row * p.to_ld + col) = c;
+    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(j.to) + row * j.to_ld + col) = c;
   }
+}
+
+// All that the gradient's products need laid out anew, in one launch (4001 x 4096 x 2056 bf16: three launches 27 + 10 + 10 us).
+template <int DT>
+__global__ __launch_bounds__(256) void gradient_layout_kernel(TransposeParams p) {
+  __shared__ __attribute__((aligned(16))) uint16_t lds[64 * 66];
+  __shared__ float sums[32 * 64];
+  unsigned tile = blockIdx.x;
+  if (tile < p.job[0].tiles) {
+    transpose_tile<DT, true>(p, p.job[0], tile, lds, sums);
+    return;
+  }
+  tile -= p.job[0].tiles;
+  const bool second = tile >= p.job[1].tiles;
+  transpose_tile<kF16, false>(p, second ? p.job[2] : p.job[1], second ? tile - p.job[1].tiles : tile, lds, sums);
 }
 
 }  // namespace tcu

@@ -10,7 +10,9 @@
 
 namespace tcu {
 
-constexpr size_t kGemmFewRows = 64;               // up to this many rows the product is bound by reading B
+// Up to this many rows the product is bound by reading B.  Beyond it every block reading all of A costs more than the tile
+// kernels' empty rows (33 x 8192 x 4096 bf16: 31.7 us, tiles with split K 18.5; 16 x 4096 x 8192: 20.6).
+constexpr size_t kGemmFewRows = 32;
 constexpr size_t kGemmMaxInner = (size_t)1 << 22; // a tile's rows of an operand lie within 32-bit byte offsets: 256 * 2^22 * 2 < 2^32
 
 constexpr size_t kGemmMaxLd = (size_t)1 << 28;    // 8 rows of an output lie within 32-bit offsets
@@ -45,7 +47,7 @@ inline GemmPlan plan_gemm(size_t M, size_t N, size_t K) {
   g.share_ld = up_to(N, 8);
   if (M <= kGemmFewRows) {
     g.few_rows = true;
-    g.few_tiles = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+    g.few_tiles = M <= 16 ? 1 : 2;
     g.tiles = (N + 15) / 16;
     // a block per compute unit: below that the waves of one compute unit cannot keep its share of the memory's bandwidth in flight
     const size_t steps = K / 1024;
@@ -82,8 +84,7 @@ inline void launch_gemm(const GemmPlan &g, FusedGemmParams p, float *shares, boo
 #define TCU_FEW(MT, UNROLL) \
   (WHOLE && whole_inner ? launch(fused_gemm_few_rows_kernel<DT, WHOLE, MT, 8, UNROLL>, grid, 512u, stream, p) : launch(fused_gemm_few_rows_kernel<DT, false, MT, 8, UNROLL>, grid, 512u, stream, p))
     if (g.few_tiles == 1) TCU_FEW(1, 4);
-    else if (g.few_tiles == 2) TCU_FEW(2, 4);
-    else TCU_FEW(4, 2);
+    else TCU_FEW(2, 4);
 #undef TCU_FEW
   } else {
 #define TCU_TILES(W8) (p.K % 64 ? launch(fused_gemm_tile_kernel<DT, WHOLE, W8, true>, grid, 256u, stream, p) : launch(fused_gemm_tile_kernel<DT, WHOLE, W8, false>, grid, 256u, stream, p))
@@ -139,7 +140,8 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   const size_t M = s->M, N = s->N, K = s->K;
   const GemmPlan g = plan_gemm(M, N, K);
   const bool few_k = K > 0 && K < 64;  // the tile kernels want a whole step
-  const bool pack_a = !g.few_rows && K && (few_k || !rows_ready(A, M > 1 ? lda : 8)), pack_b = !g.few_rows && K && (few_k || !rows_ready(B, N > 1 ? ldb : 8));
+  const bool odd_k = few_k || K % 8 != 0;     // nor a part of a chunk
+  const bool pack_a = !g.few_rows && K && (odd_k || !rows_ready(A, M > 1 ? lda : 8)), pack_b = !g.few_rows && K && (odd_k || !rows_ready(B, N > 1 ? ldb : 8));
   const size_t ldk = few_k ? 64 : up_to(K, 8), a_bytes = pack_a ? part_bytes(M * ldk * 2) : 0, b_bytes = pack_b ? part_bytes(N * ldk * 2) : 0;
   const size_t bytes = g.share_bytes + a_bytes + b_bytes, need = bytes < 256 ? 256 : bytes;
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
@@ -187,20 +189,11 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   p.ldz = ldz;
   p.M = M;
   p.N = N;
-  p.K = pack_a && few_k ? 64 : K;
+  p.K = !g.few_rows && odd_k ? ldk : K;
   p.beta = s->beta;
   p.act = s->activation;
   run_gemm(s->dtype, whole, g, p, static_cast<float *>(workspace), whole_inner, stream);
   return TCU_OK;
-}
-
-// transpose (and, with Z or for its column sums, activation gradient) of rows x columns elements
-template <bool GRAD>
-inline void run_transpose(int dtype, TransposeParams q, void *stream) {
-  q.column_tiles = (unsigned)((q.columns + 63) / 64);
-  const unsigned grid = (unsigned)((q.rows + 63) / 64 * q.column_tiles);
-  if (dtype == TCU_F16 || !GRAD) launch(transpose_kernel<kF16, GRAD>, grid, 256u, stream, q);  // bits move as they are
-  else launch(transpose_kernel<kBF16, GRAD>, grid, 256u, stream, q);
 }
 
 inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const void *dD, size_t lddd, const void *A, size_t lda, const void *B, size_t ldb, const void *Z, size_t ldz, void *dA, size_t ldda,
@@ -209,7 +202,7 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   if (int rc = check_gemm_shape(w, s)) return rc;
   const size_t M = s->M, N = s->N, K = s->K;
   if (M > kGemmMaxInner || N > kGemmMaxInner) return report_failure(TCU_ERR_UNSUPPORTED, w + ": M or N above 2^22");
-  for (auto mn : {std::make_pair(M, N), std::make_pair(M, K), std::make_pair(N, K)})
+  for (auto mn : {std::make_pair(M, N), std::make_pair(M, K), std::make_pair(N, K)})  // a third of what a launch may have, in tiles of 64 x 64
     if (int rc = check_gemm_grid(w, mn.first, mn.second)) return rc;
   const bool act = s->activation != TCU_ACT_NONE;
   if (act && !Z) return report_failure(TCU_ERR_INVALID_ARG, w + ": the gradient of an activation needs d_Z");
@@ -253,21 +246,23 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   void *dz = take(dz_bytes), *dzt = take(dzt_bytes), *a_t = take(at_bytes), *b_t = take(bt_bytes);
   float *sums = static_cast<float *>(take(sums_bytes));
   float *shares = static_cast<float *>(workspace);
-  if (M && N && (own_dz || dB || dbias)) {
-    TransposeParams q{};
-    q.from = dD;
-    q.from_ld = lddd;
-    q.Z = act ? Z : nullptr;
-    q.z_ld = ldz;
-    q.to = dB ? dzt : nullptr;
-    q.to_ld = ldm;
-    q.dz = own_dz ? dz : nullptr;
-    q.dz_ld = ldn;
-    q.partial = dbias ? sums : nullptr;
-    q.rows = M;
-    q.columns = N;
-    q.act = s->activation;
-    run_transpose<true>(s->dtype, q, stream);
+  TransposeParams q{};
+  auto job = [&](int i, const void *from, size_t from_ld, void *to, size_t to_ld, size_t rows, size_t columns) {
+    const unsigned column_tiles = (unsigned)((columns + 63) / 64);
+    q.job[i] = TransposeJob{from, to, rows, columns, from_ld, to_ld, column_tiles, (unsigned)((rows + 63) / 64 * column_tiles)};
+  };
+  if (M && N && (own_dz || dB || dbias)) job(0, dD, lddd, dB ? dzt : nullptr, ldm, M, N);
+  if (dB && M && K) job(1, A, lda, a_t, ldm, M, K);
+  if (dA && N && K) job(2, B, ldb, b_t, ldn, N, K);
+  q.Z = act ? Z : nullptr;
+  q.z_ld = ldz;
+  q.dz = own_dz ? dz : nullptr;
+  q.dz_ld = ldn;
+  q.partial = dbias ? sums : nullptr;
+  q.act = s->activation;
+  if (const unsigned grid = q.job[0].tiles + q.job[1].tiles + q.job[2].tiles) {
+    if (s->dtype == TCU_F16) launch(gradient_layout_kernel<kF16>, grid, 256u, stream, q);
+    else launch(gradient_layout_kernel<kBF16>, grid, 256u, stream, q);
   }
   if (dbias && N) {
     ColumnSumParams q{};
@@ -282,16 +277,6 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   p.act = TCU_ACT_NONE;
   p.N = K;
   if (dA && M && K) {
-    if (N) {
-      TransposeParams q{};
-      q.from = B;
-      q.from_ld = ldb;
-      q.to = b_t;
-      q.to_ld = ldn;
-      q.rows = N;
-      q.columns = K;
-      run_transpose<false>(s->dtype, q, stream);
-    }
     p.A = own_dz ? dz : dD;
     p.lda = own_dz ? ldn : lddd;
     p.B = b_t;
@@ -303,16 +288,6 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
     run_gemm(s->dtype, whole_a, ga, p, shares, true, stream);
   }
   if (dB && N && K) {
-    if (M) {
-      TransposeParams q{};
-      q.from = A;
-      q.from_ld = lda;
-      q.to = a_t;
-      q.to_ld = ldm;
-      q.rows = M;
-      q.columns = K;
-      run_transpose<false>(s->dtype, q, stream);
-    }
     p.A = dzt;
     p.lda = ldm;
     p.B = a_t;

@@ -635,7 +635,7 @@ def test_fused_gemm(emu, dtype, case):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("w8,splits,M,N,K", [(4, 1, 130, 250, 136), (4, 3, 140, 100, 330), (8, 1, 300, 257, 208), (8, 2, 256, 40, 190), (8, 1, 33, 300, 448), (4, 2, 100, 30, 128), (6, 1, 200, 193, 150), (6, 2, 192, 384, 256)])
+@pytest.mark.parametrize("w8,splits,M,N,K", [(4, 1, 130, 250, 136), (4, 3, 140, 100, 328), (8, 1, 300, 257, 208), (8, 2, 256, 40, 192), (8, 1, 33, 300, 448), (4, 2, 100, 30, 128), (6, 1, 200, 193, 152), (6, 2, 192, 384, 256)])
 def test_fused_gemm_tiles(emu, dtype, w8, splits, M, N, K):
     emu = gemm_emu(emu)
     rng = np.random.default_rng(M)
