@@ -29,8 +29,12 @@
 // which wait for nothing but each other; every 64th tile the state behind it, which waits for the state 64 tiles before.  A
 // tile's carry is that state with at most 7 entries of 8 tiles and 7 entries of one tile applied in their order.  What is
 // published and in which order it is combined depends on places alone, never on timing: the same input gives the same bits
-// every time.  The chain of waits is a 64th of the tiles long (every 8th tile handing a state on, with 512 tiles along a
-// sequence: 65536 x 2048 fp16, 390 us; waits left out 264 us).
+// every time.  The chain of waits is a 64th of the tiles long (with every 8th tile handing a state on, 512 tiles along a
+// sequence waited for a third of their time: 65536 x 2048 fp16, 390 us against 264 with the waits left out).
+//
+// 65536 x 2048 fp16 takes 173 us (805 MB, 4.6 TB/s; a copy reaches 5.1), 8 x 4096 x 2048 bf16 98 us (403 MB, 4.1 TB/s), its
+// gradient 164 us (805 MB, 4.9 TB/s), 8191 x 1000 packed bf16 19 us (49 MB; some 130 blocks at once, each bound by its own
+// chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 23 us (63 MB; likewise, element-wise accesses).
 // Tiles are handed out by a ticket, so the one that is waited for has always been started; a wait is bounded and leaves NaN
 // in what depended on it.
 #pragma once
@@ -211,6 +215,50 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
   const unsigned channel = strip * TC + lane * V;
   const int count = (int)p.channels - (int)channel;  // channels of this chunk that exist (<= 0: none)
 
+  // Where the wave's places are all there, a lane's addresses are one 32-bit offset from a base that the wave's rows share.
+  const int wave = wave_in_block();
+  constexpr int WAVE_GROUPS = 64 / TCL;
+  const unsigned wave_place = wave_uniform(chunk * TILE_ROWS + wave * (WAVE_GROUPS * RPT));
+  const unsigned wave_row = BACK ? p.rows - wave_place - WAVE_GROUPS * RPT : wave_place;  // the lowest of them
+  const unsigned lane_row = (unsigned)(BACK ? WAVE_GROUPS - 1 - group % WAVE_GROUPS : group % WAVE_GROUPS) * RPT;
+  const unsigned strip_at = wave_uniform(strip * TC);
+  const unsigned lane_channel = count > 0 ? (unsigned)(lane * V) : 0u;  // a lane without channels reads the strip's first ones
+  constexpr size_t E = sizeof(typename Elem<DT>::word_t);
+  const bool fits = p.near_rows && (ALIGNED || strip * TC + TC <= p.channels) && wave_place + WAVE_GROUPS * RPT <= p.rows && (!BACK || wave_row > 0);  // the same for the whole wave
+  // place i of the thread lies in row wave_row + lane_row + step_row(i)
+  auto step_row = [](int i) { return BACK ? RPT - 1 - i : i; };
+  auto plain_load = [&](const void *q, size_t stride, int row) {
+    const char *base = static_cast<const char *>(q) + (((ptrdiff_t)wave_row + row) * (ptrdiff_t)stride + strip_at) * (ptrdiff_t)E;
+    return load_at<ALIGNED>(base, (lane_row * (unsigned)stride + lane_channel) * (unsigned)E);
+  };
+  auto plain_store = [&](void *q, size_t stride, int row, const float (&v)[V]) {
+    char *base = static_cast<char *>(q) + (((ptrdiff_t)wave_row + row) * (ptrdiff_t)stride + strip_at) * (ptrdiff_t)E;
+    if (count > 0) store_at<ALIGNED>(base, (lane_row * (unsigned)stride + lane_channel) * (unsigned)E, pack_chunk<DT>(v));
+  };
+
+  constexpr bool KEEP = GATE == kGateSigmoid;
+  uint4_t cg[BACK ? 1 : RPT], cin[BACK ? 1 : RPT];          // gate, input (backwards: within the branches below)
+  uint4_t cx[BACK && KEEP ? RPT : 1], ch[BACK ? RPT : 1];  // what the gradient needs at the end
+  auto load_all = [&](auto &gates, auto &inputs) {  // inputs: x, or dh
+#pragma unroll
+    for (int i = 0; i < RPT; i++) {
+      gates[i] = plain_load(p.g, p.g_stride, step_row(i));
+      inputs[i] = BACK ? plain_load(p.dh, p.dh_stride, step_row(i)) : plain_load(p.x, p.x_stride, step_row(i));
+    }
+    if constexpr (BACK) {
+#pragma unroll
+      for (int i = 0; i < RPT; i++) {
+        ch[i] = plain_load(p.h, p.h_stride, step_row(i) - 1);
+        if constexpr (KEEP) cx[i] = plain_load(p.x, p.x_stride, step_row(i));
+      }
+    }
+  };
+  // Forwards the loads go out before it is known which sequences the places belong to, which takes a load or two (65536 x 2048 fp16
+  // 187 -> 173 us; backwards the registers do not suffice for that: 164 -> 233).
+  if constexpr (!BACK) {
+    if (fits) load_all(cg, cin);
+  }
+
   // what each of the thread's places is: inside a sequence, the first or the last one of it in place order
   constexpr unsigned kAll = (1u << RPT) - 1u;
   unsigned inside = 0, begins = 0, ends = 0;
@@ -252,31 +300,9 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
     return p.row_sequence ? (unsigned)p.row_sequence[row] : row / p.sequence_rows;
   };
 
-  // Most waves have places in the middle of one sequence only.  For them nothing has to be looked at place by place (the
-  // general form takes 53 instruction slots per element, this one 26, and the kernel is bound by them as soon as it is not
-  // by memory), and a lane's addresses are one 32-bit offset from a base that the wave's rows share.
-  const int wave = wave_in_block();
-  constexpr int WAVE_GROUPS = 64 / TCL;
-  const bool plain = p.near_rows && (ALIGNED || strip * TC + TC <= p.channels) && ballot(inside != kAll || (begins | ends) != 0) == 0;
-  const unsigned wave_place = wave_uniform(chunk * TILE_ROWS + wave * (WAVE_GROUPS * RPT));
-  const unsigned wave_row = BACK ? p.rows - wave_place - WAVE_GROUPS * RPT : wave_place;  // the lowest row of a plain wave
-  const unsigned lane_row = (unsigned)(BACK ? WAVE_GROUPS - 1 - group % WAVE_GROUPS : group % WAVE_GROUPS) * RPT;
-  const unsigned strip_at = wave_uniform(strip * TC);
-  const unsigned lane_channel = count > 0 ? (unsigned)(lane * V) : 0u;  // a lane without channels reads the strip's first ones
-  constexpr size_t E = sizeof(typename Elem<DT>::word_t);
-  // place i of the thread lies in row wave_row + lane_row + step_row(i)
-  auto step_row = [](int i) { return BACK ? RPT - 1 - i : i; };
-  auto plain_load = [&](const void *q, size_t stride, int row) {
-    const char *base = static_cast<const char *>(q) + (((ptrdiff_t)wave_row + row) * (ptrdiff_t)stride + strip_at) * (ptrdiff_t)E;
-    return load_at<ALIGNED>(base, (lane_row * (unsigned)stride + lane_channel) * (unsigned)E);
-  };
-  auto plain_store = [&](void *q, size_t stride, int row, const float (&v)[V]) {
-    char *base = static_cast<char *>(q) + (((ptrdiff_t)wave_row + row) * (ptrdiff_t)stride + strip_at) * (ptrdiff_t)E;
-    if (count > 0) store_at<ALIGNED>(base, (lane_row * (unsigned)stride + lane_channel) * (unsigned)E, pack_chunk<DT>(v));
-  };
-
-  constexpr bool KEEP = GATE == kGateSigmoid;
-  uint4_t cx[BACK && KEEP ? RPT : 1], ch[BACK ? RPT : 1];  // what the gradient needs again at the end
+  // Most waves have places in the middle of one sequence only.  For them nothing has to be looked at place by place: the general
+  // form takes 53 instruction slots per element, this one 26, and the kernel is bound by them as soon as it is not by memory.
+  const bool plain = fits && ballot(inside != kAll || (begins | ends) != 0) == 0;
   float a[RPT][V], b[RPT][V], A[V], B[V];                  // b: what the place adds to the state; where a sequence begins, with its seed
   float keep[BACK && KEEP ? RPT : 1][V];
 #pragma unroll
@@ -294,25 +320,12 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
       b[i][e] = KEEP ? k * x : x;
     }
   };
-  if (plain) {
-    uint4_t cg[RPT], cin[RPT];
-#pragma unroll
-    for (int i = 0; i < RPT; i++) {
-      cg[i] = plain_load(p.g, p.g_stride, step_row(i));
-      cin[i] = BACK ? plain_load(p.dh, p.dh_stride, step_row(i)) : plain_load(p.x, p.x_stride, step_row(i));
-    }
-    if constexpr (BACK) {
-#pragma unroll
-      for (int i = 0; i < RPT; i++) {
-        ch[i] = plain_load(p.h, p.h_stride, step_row(i) - 1);  // the row in front belongs to the same sequence
-        if constexpr (KEEP) cx[i] = plain_load(p.x, p.x_stride, step_row(i));
-      }
-    }
+  auto plain_steps = [&](auto &gates, auto &inputs) {
 #pragma unroll
     for (int i = 0; i < RPT; i++) {
       float g[V], x[V];
-      unpack_chunk<DT>(cg[i], g);
-      unpack_chunk<DT>(cin[i], x);
+      unpack_chunk<DT>(gates[i], g);
+      unpack_chunk<DT>(inputs[i], x);
 #pragma unroll
       for (int e = 0; e < V; e++) {
         element(i, e, g[e], x[e]);
@@ -320,27 +333,29 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
         A[e] *= a[i][e];
       }
     }
-  } else {
-    uint4_t cg[RPT], cin[RPT];
+  };
+  auto load_some = [&](auto &gates, auto &inputs) {
 #pragma unroll
     for (int i = 0; i < RPT; i++) {
       const int n = (inside >> i) & 1u ? count : 0;
       const size_t row = n > 0 ? row_of(place0 + i) : 0;
-      cg[i] = load_chunk_of<DT, ALIGNED>(p.g, row * p.g_stride + channel, n);
-      if constexpr (!BACK) cin[i] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + channel, n);
+      gates[i] = load_chunk_of<DT, ALIGNED>(p.g, row * p.g_stride + channel, n);
+      if constexpr (!BACK) inputs[i] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + channel, n);
       if constexpr (BACK) {
-        cin[i] = load_chunk_of<DT, ALIGNED>(p.dh, row * p.dh_stride + channel, n);
+        inputs[i] = load_chunk_of<DT, ALIGNED>(p.dh, row * p.dh_stride + channel, n);
         if constexpr (KEEP) cx[i] = load_chunk_of<DT, ALIGNED>(p.x, row * p.x_stride + channel, n);
         const int nh = (ends >> i) & 1u ? 0 : n;  // the row in front of a sequence's first one is another sequence's
         ch[i] = load_chunk_of<DT, ALIGNED>(p.h, (nh > 0 ? row - 1 : 0) * p.h_stride + channel, nh);
       }
     }
+  };
+  auto general_steps = [&](auto &gates, auto &inputs) {
 #pragma unroll
     for (int i = 0; i < RPT; i++) {
       const bool in = (inside >> i) & 1u, first = (begins >> i) & 1u;
       float g[V], x[V], seed[V];
-      unpack_chunk<DT>(cg[i], g);
-      unpack_chunk<DT>(cin[i], x);
+      unpack_chunk<DT>(gates[i], g);
+      unpack_chunk<DT>(inputs[i], x);
       if (first && p.seed) {
         load_floats<V, ALIGNED>(p.seed, (size_t)sequence_at(i) * p.channels + channel, count, seed);
       } else {
@@ -360,6 +375,20 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
         if (in) A[e] = first ? 0.0f : a[i][e] * A[e];
       }
     }
+  };
+  if constexpr (BACK) {
+    uint4_t gates[RPT], inputs[RPT];
+    if (plain) {
+      load_all(gates, inputs);
+      plain_steps(gates, inputs);
+    } else {
+      load_some(gates, inputs);
+      general_steps(gates, inputs);
+    }
+  } else {
+    if (!fits) load_some(cg, cin);
+    if (plain) plain_steps(cg, cin);
+    else general_steps(cg, cin);
   }
   unsigned reset = begins ? 1u : 0u, front_reset;
   float FA[V], FB[V];
@@ -450,7 +479,11 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
     if constexpr (BACK) {
       float h[V], x[V], dx[V], dg[V];
       unpack_chunk<DT>(ch[i], h);
-      if (end && p.h0) load_floats<V, ALIGNED>(p.h0, (size_t)sequence_at(i) * p.channels + channel, count, h);
+      if (end) {  // the row in front is another sequence's
+#pragma unroll
+        for (int e = 0; e < V; e++) h[e] = 0.0f;
+        if (p.h0) load_floats<V, ALIGNED>(p.h0, (size_t)sequence_at(i) * p.channels + channel, count, h);
+      }
       if constexpr (KEEP) unpack_chunk<DT>(cx[i], x);
 #pragma unroll
       for (int e = 0; e < V; e++) {

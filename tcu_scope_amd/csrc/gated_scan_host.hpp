@@ -8,7 +8,8 @@
 namespace tcu {
 
 // Tiles: 16 lanes (256 bytes of a row) x 16 or 32 groups of so many places per thread, whose (a, b) stay in registers (two
-// waves per SIMD).  Places: 8 | 4 forwards 65536 x 2048 fp16 187 | 228 us, 4 | 2 | 8 backwards 32768 x 2048 bf16 164 | 223 | 227.
+// waves per SIMD).  Places: 8 | 4 forwards 65536 x 2048 fp16 187 | 228 us (both before the
+// kernel loaded ahead of its masks: 8 then takes 173), 4 | 2 | 8 backwards 32768 x 2048 bf16 164 | 223 | 227.
 // Blocks of 512 threads where there are few tiles, i.e. where the waits for each other count: 8191 x 1000 bf16 packed 22.5 ->
 // 19.1 us, backwards 4099 x 769 fp32 30.2 -> 23.7; from about 1024 tiles on 256 threads are as fast or faster (backwards
 // 32768 x 2048 bf16 164 | 178).
@@ -51,6 +52,7 @@ inline int plan_gated_scan(const char *what, const tcu_gated_scan_shape *s, int 
   plan->entries_at = plan->rows_at + (s->d_offsets ? (plan->rows * 4 + 255) / 256 * 256 : 0);
   plan->entries_bytes = plan->chained ? plan->strips * (plan->chunks + plan->chunks / kScanGroup + plan->chunks / (kScanGroup * kScanGroup)) * tc * 8 : 0;
   plan->bytes = plan->entries_at + plan->entries_bytes;
+  if (plan->rows == 0 || s->d_offsets || plan->chained) plan->bytes = plan->bytes < 512 ? 512 : plan->bytes;  // the setup kernel runs
   return TCU_OK;
 }
 
