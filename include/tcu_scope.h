@@ -272,8 +272,9 @@ int tcu_gemm_f16_f16(const void *d_A, const void *d_B, const void *d_C, void *d_
  * need base pointers aligned to 16 bytes and strides and widths that are multiples of 16 bytes; anything else takes the same
  * kernels with element-wise accesses.  All sums, states and statistics are fp32; a result is rounded once, to its type.
  * Calls run on the device of `stream` (NULL: the current device's default stream).  Workspaces follow the two-phase
- * protocol of the full-array entry points (256-byte aligned, never smaller than 256 bytes, nothing is kept in them from
- * one call to the next; calls that may overlap in time, captured graphs among them, need one each). */
+ * protocol of the full-array entry points (256-byte aligned, nothing is kept in them from one call to the next; calls that
+ * may overlap in time, captured graphs among them, need one each).  The smallest size is 256 bytes: it means that the call
+ * keeps nothing there, and calls that ask for no more may share it. */
 
 typedef enum { TCU_F16 = 0, TCU_BF16 = 1, TCU_F32 = 2 } tcu_dtype;
 
@@ -303,7 +304,7 @@ typedef struct {
   const void *d_offsets;  /* or num_sequences + 1 offsets in device memory that do not decrease: sequence j has the rows
                              offsets[j] ... offsets[j+1] - 1 (none if they are equal) */
   int offset_bits;        /* 32 or 64 */
-  int zero_outside;       /* rows outside all sequences are not read; in the outputs they are left as they are (0) or set
+  int zero_outside;       /* rows outside all sequences count for nothing; in the outputs they are left as they are (0) or set
                              to zero (anything else) */
 } tcu_gated_scan_shape;
 

@@ -2,6 +2,7 @@
 launches on torch's current stream unless told otherwise."""
 import ctypes
 import enum
+import functools
 import os
 import subprocess
 
@@ -473,7 +474,7 @@ def _enum(kind, value):
 def _matrix(t, name, like=None):
     """(pointer, rows, row stride) of a tensor whose leading dimensions can be read as one: rows of contiguous elements at an even distance."""
     sizes = t.shape
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or sizes != like.shape):
+    if like is not None and not (t.dtype is like.dtype and sizes == like.shape and t.device == like.device):
         raise ValueError(f"{name} must have the shape, type and device of the other operands ({tuple(like.shape)}, {like.dtype}, {like.device}); got {tuple(sizes)}, {t.dtype}, {t.device}")
     if len(sizes) < 2:
         raise ValueError(f"{name} must have at least two dimensions")
@@ -504,24 +505,52 @@ def _vector_f32(t, name, shape, device):
     return t.data_ptr()
 
 
-def _launch_on(device, stream, body):
-    """body(raw stream) with `device`, and the stream asked for, current: what the body allocates belongs to that stream."""
-    torch = _torch()
-    if stream is not None:
-        if stream.device != device:
-            raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
-        with torch.cuda.stream(stream):
-            return body(stream.cuda_stream)
-    if torch.cuda.current_device() == device.index:
-        return body(_current_raw_stream(device.index))
-    with torch.cuda.device(device):
-        return body(_current_raw_stream(device.index))
-
-
-def _current_raw_stream(index):
-    torch = _torch()
+def _raw_stream(torch, index):
     quick = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the handle without the object around it: 4 us less
     return quick(index) if quick is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _launches(fn):
+    """Runs a function whose `stream` is a raw handle on the stream asked for, or the current one of its first operand's device, with
+    that device and stream current: what it allocates belongs to that stream."""
+    first = fn.__code__.co_varnames[0]
+
+    @functools.wraps(fn)
+    def call(*args, stream=None, **kw):
+        torch = _torch()
+        operand = args[0] if args else kw.get(first)
+        if not (isinstance(operand, torch.Tensor) and operand.is_cuda):
+            raise ValueError(f"{first} must be a CUDA tensor")
+        device = operand.device
+        index = device.index
+        if stream is not None:
+            if stream.device != device:
+                raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+            with torch.cuda.stream(stream):
+                return fn(*args, stream=stream.cuda_stream, **kw)
+        if torch.cuda.current_device() == index:
+            return fn(*args, stream=_raw_stream(torch, index), **kw)
+        with torch.cuda.device(index):
+            return fn(*args, stream=_raw_stream(torch, index), **kw)
+
+    return call
+
+
+def _new(t):
+    """An uninitialised contiguous tensor like t."""
+    torch = _torch()
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+_untouched = {}
+
+
+def _untouched_workspace(device):
+    """256 bytes for the calls that ask for no more: they keep nothing there, so one piece of memory serves them all."""
+    ws = _untouched.get(device)
+    if ws is None:
+        ws = _untouched[device] = _torch().empty(256, dtype=_torch().uint8, device=device)
+    return ws
 
 
 # Workspace sizes by entry point and sizes of the operands, so that the size is asked for once and not at every call.
@@ -538,9 +567,10 @@ def _call_with_workspace(fn, args, sizes, workspace, device, raw):
         return
     torch = _torch()
     key = (fn.__name__, *sizes)
-    have = ctypes.c_size_t(_workspace_sizes.get(key, 0))
-    if have.value:
-        ws = torch.empty(have.value, dtype=torch.uint8, device=device)
+    size = _workspace_sizes.get(key, 0)
+    have = ctypes.c_size_t(size)
+    if size:
+        ws = _untouched_workspace(device) if size == 256 else torch.empty(size, dtype=torch.uint8, device=device)
         rc = fn(*args, ws.data_ptr(), ctypes.byref(have), raw)
         if rc != 4:  # the size also goes by the operands' alignment: another one may need more
             return _check(rc)
@@ -572,7 +602,8 @@ def _scan_shape(x, gate, offsets, h0, name="x"):
     return s
 
 
-def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=None, workspace=None, stream=None):
+@_launches
+def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=None, workspace=None, *, stream=None):
     """h[t] = a[t] h[t-1] + b[t] along each sequence (tcu_gated_scan): returns (h, h_last).
 
     x, g: (sequences, tokens, channels) or (tokens, channels), float16, bfloat16 or float32, or with `offsets` (int32 or
@@ -588,18 +619,16 @@ def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=
     p0 = _vector_f32(h0, "h0", states, x.device)
     s.zero_outside = out is None
 
-    def body(raw):
-        h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        last = torch.empty(states, dtype=torch.float32, device=x.device) if h_last is None else h_last
-        ph, _, sh = _matrix(h, "out", x)
-        args = (ctypes.byref(s), px, sx, pg, sg, ph, sh, p0, _vector_f32(last, "h_last", states, x.device))
-        _call_with_workspace(lib().tcu_gated_scan, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, x.device, raw)
-        return h, last
-
-    return _launch_on(x.device, stream, body)
+    h = _new(x) if out is None else out
+    last = torch.empty(states, dtype=torch.float32, device=x.device) if h_last is None else h_last
+    ph, _, sh = _matrix(h, "out", x)
+    args = (ctypes.byref(s), px, sx, pg, sg, ph, sh, p0, _vector_f32(last, "h_last", states, x.device))
+    _call_with_workspace(lib().tcu_gated_scan, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, x.device, stream)
+    return h, last
 
 
-def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, offsets=None, dx=None, dg=None, workspace=None, stream=None):
+@_launches
+def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, offsets=None, dx=None, dg=None, workspace=None, *, stream=None):
     """The gradient of gated_scan (tcu_gated_scan_backward): returns (dx, dg, dh0).
 
     dh, dh_last: gradients with respect to h and h_last (dh_last may be None); h: what gated_scan returned; x is read for
@@ -619,19 +648,17 @@ def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, o
         raise ValueError("dx and dg are given both or neither")
     s.zero_outside = dx is None
 
-    def body(raw):
-        out_x, out_g = (dx, dg) if dx is not None else (torch.empty(g.shape, dtype=g.dtype, device=g.device) for _ in range(2))
-        dh0 = torch.empty(states, dtype=torch.float32, device=g.device)
-        pox, _, sox = _matrix(out_x, "dx", g)
-        pog, _, sog = _matrix(out_g, "dg", g)
-        args = (ctypes.byref(s), pd, sd, px, sx, pg, sg, ph, sh, p0, pl, pox, sox, pog, sog, dh0.data_ptr())
-        _call_with_workspace(lib().tcu_gated_scan_backward, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, g.device, raw)
-        return out_x, out_g, dh0
-
-    return _launch_on(g.device, stream, body)
+    out_x, out_g = (dx, dg) if dx is not None else (_new(g), _new(g))
+    dh0 = torch.empty(states, dtype=torch.float32, device=g.device)
+    pox, _, sox = _matrix(out_x, "dx", g)
+    pog, _, sog = _matrix(out_g, "dg", g)
+    args = (ctypes.byref(s), pd, sd, px, sx, pg, sg, ph, sh, p0, pl, pox, sox, pog, sog, dh0.data_ptr())
+    _call_with_workspace(lib().tcu_gated_scan_backward, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, g.device, stream)
+    return out_x, out_g, dh0
 
 
-def gated_scan_step(x, g, state, gate=Gate.SIGMOID, slots=None, new_state=None, out=None, stream=None):
+@_launches
+def gated_scan_step(x, g, state, gate=Gate.SIGMOID, slots=None, new_state=None, out=None, *, stream=None):
     """One token for each running sequence (tcu_gated_scan_step): returns h (rows, channels).
 
     x, g: (rows, channels); state: (slots, channels) float32; slots: int32, the slot of each row (None: row i uses slot i; a
@@ -652,13 +679,10 @@ def gated_scan_step(x, g, state, gate=Gate.SIGMOID, slots=None, new_state=None, 
     if slots is not None and (slots.dtype != torch.int32 or slots.device != x.device or tuple(slots.shape) != (rows,) or not slots.is_contiguous()):
         raise ValueError("slots must be a contiguous int32 vector with one entry per row, on the same device")
 
-    def body(raw):
-        h = torch.empty((rows, channels), dtype=x.dtype, device=x.device) if out is None else out
-        ph, _, sh = _matrix(h, "out", x)
-        _check(lib().tcu_gated_scan_step(dtype, _enum(Gate, gate), channels, rows, px, sx, pg, sg, ph, sh, ps, pn, shape[0], slots.data_ptr() if slots is not None else None, out is None, raw))
-        return h
-
-    return _launch_on(x.device, stream, body)
+    h = _new(x) if out is None else out
+    ph, _, sh = _matrix(h, "out", x)
+    _check(lib().tcu_gated_scan_step(dtype, _enum(Gate, gate), channels, rows, px, sx, pg, sg, ph, sh, ps, pn, shape[0], slots.data_ptr() if slots is not None else None, out is None, stream))
+    return h
 
 
 def _vector(t, name, n, like):
@@ -682,7 +706,8 @@ def _norm_shape(x, gate, norm, order, activation, eps, scale, name):
     return p, stride, FusedNormShape(dtype=dtype, norm=_enum(Norm, norm), order=_enum(NormOrder, order), activation=_enum(Activation, activation), rows=rows, dim=x.shape[-1], eps=eps, scale=scale)
 
 
-def fused_norm(x, weight=None, bias=None, residual=None, gate=None, scale=1.0, channel_scale=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, out=None, residual_out=None, stream=None):
+@_launches
+def fused_norm(x, weight=None, bias=None, residual=None, gate=None, scale=1.0, channel_scale=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, out=None, residual_out=None, *, stream=None):
     """Norm of every row of x (..., dim), fused with a residual, its scale and a gate (tcu_fused_norm); s = scale * channel_scale.
 
     order "add_norm": z = residual + s x, returns (act(gate) y(z), z), or act(gate) y(x) alone without a residual.
@@ -696,17 +721,14 @@ def fused_norm(x, weight=None, bias=None, residual=None, gate=None, scale=1.0, c
     if residual_out is not None and not keep:
         raise ValueError("residual_out goes with the order add_norm and a residual")
 
-    def body(raw):
-        o = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
-        z = None if not keep else torch.empty(x.shape, dtype=x.dtype, device=x.device) if residual_out is None else residual_out
-        _check(lib().tcu_fused_norm(ctypes.byref(s), px, sx, *pr, *pg, *vectors, *_optional(o, "out", x), *_optional(z, "residual_out", x), raw))
-        return (o, z) if keep else o
-
-    return _launch_on(x.device, stream, body)
+    o = _new(x) if out is None else out
+    z = None if not keep else _new(x) if residual_out is None else residual_out
+    _check(lib().tcu_fused_norm(ctypes.byref(s), px, sx, *pr, *pg, *vectors, *_optional(o, "out", x), *_optional(z, "residual_out", x), stream))
+    return (o, z) if keep else o
 
 
-def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, channel_scale=None, x=None, dresidual_out=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, workspace=None,
-                        stream=None):
+@_launches
+def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, channel_scale=None, x=None, dresidual_out=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, workspace=None, *, stream=None):
     """The gradient of fused_norm (tcu_fused_norm_backward): a dict with "dx" and, where the operand is there, "dgate",
     "dweight", "dbias", "dscale" (of channel_scale) and "dresidual".
 
@@ -724,23 +746,20 @@ def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, c
         raise ValueError("the gradient of channel_scale needs x")
     px = _optional(x if add_norm and channel_scale is not None else None, "x", dout)
 
-    def body(raw):
-        new = lambda: torch.empty(dout.shape, dtype=dout.dtype, device=dout.device)
-        column = lambda: torch.empty(s.dim, dtype=torch.float32, device=dout.device)
-        got = {"dx": new()}
-        if gate is not None:
-            got["dgate"] = new()
-        if dresidual_out is not None:
-            got["dresidual"] = new()
-        for name, t in (("dweight", weight), ("dbias", bias), ("dscale", channel_scale)):
-            if t is not None:
-                got[name] = column()
-        args = (ctypes.byref(s), pd, sd, *pz, *pg, *vectors, *px, *ps, *(v for n in ("dx", "dgate", "dresidual") for v in ((got[n].data_ptr(), s.dim) if n in got else (None, 0))),
-                *(got[n].data_ptr() if n in got else None for n in ("dweight", "dbias", "dscale")))
-        _call_with_workspace(lib().tcu_fused_norm_backward, args, (s.dtype, s.rows, s.dim, weight is None, bias is None, channel_scale is None), workspace, dout.device, raw)
-        return got
-
-    return _launch_on(dout.device, stream, body)
+    new = lambda: _new(dout)
+    column = lambda: torch.empty(s.dim, dtype=torch.float32, device=dout.device)
+    got = {"dx": new()}
+    if gate is not None:
+        got["dgate"] = new()
+    if dresidual_out is not None:
+        got["dresidual"] = new()
+    for name, t in (("dweight", weight), ("dbias", bias), ("dscale", channel_scale)):
+        if t is not None:
+            got[name] = column()
+    args = (ctypes.byref(s), pd, sd, *pz, *pg, *vectors, *px, *ps, *(v for n in ("dx", "dgate", "dresidual") for v in ((got[n].data_ptr(), s.dim) if n in got else (None, 0))),
+            *(got[n].data_ptr() if n in got else None for n in ("dweight", "dbias", "dscale")))
+    _call_with_workspace(lib().tcu_fused_norm_backward, args, (s.dtype, s.rows, s.dim, weight is None, bias is None, channel_scale is None), workspace, dout.device, stream)
+    return got
 
 
 def _operand(t, name, rows, columns, like):
@@ -755,7 +774,8 @@ def _operand(t, name, rows, columns, like):
     return p, stride
 
 
-def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, out=None, preactivation=None, return_preactivation=False, workspace=None, stream=None):
+@_launches
+def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, out=None, preactivation=None, return_preactivation=False, workspace=None, *, stream=None):
     """D = act(A @ Bt.T + bias) + beta * C (tcu_fused_gemm): A (..., K), Bt (N, K), bias (N,), C and D (..., N), float16 or bfloat16.
 
     Returns D, or with return_preactivation or a `preactivation` tensor to fill (D, A @ Bt.T + bias); the second is what
@@ -769,18 +789,16 @@ def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, o
     s = FusedGemmShape(dtype=dtype, activation=_enum(Activation, activation), M=M, N=N, K=K, beta=beta if C is not None else 0.0)
     pb, pbias, pc = _operand(Bt, "Bt", N, K, A), _vector(bias, "bias", N, A), _operand(C, "C", M, N, A)
 
-    def body(raw):
-        new = lambda: torch.empty((*A.shape[:-1], N), dtype=A.dtype, device=A.device)
-        D = new() if out is None else out
-        Z = new() if preactivation is None and return_preactivation else preactivation
-        args = (ctypes.byref(s), pa, lda, *pb, pbias, *pc, *_operand(D, "out", M, N, A), *_operand(Z, "preactivation", M, N, A))
-        _call_with_workspace(lib().tcu_fused_gemm, args, (M, N, K), workspace, A.device, raw)
-        return D if Z is None else (D, Z)
-
-    return _launch_on(A.device, stream, body)
+    new = lambda: torch.empty((*A.shape[:-1], N), dtype=A.dtype, device=A.device)
+    D = new() if out is None else out
+    Z = new() if preactivation is None and return_preactivation else preactivation
+    args = (ctypes.byref(s), pa, lda, *pb, pbias, *pc, *_operand(D, "out", M, N, A), *_operand(Z, "preactivation", M, N, A))
+    _call_with_workspace(lib().tcu_fused_gemm, args, (M, N, K), workspace, A.device, stream)
+    return D if Z is None else (D, Z)
 
 
-def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_gradient=True, input_gradient=True, weight_gradient=True, workspace=None, stream=None):
+@_launches
+def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_gradient=True, input_gradient=True, weight_gradient=True, workspace=None, *, stream=None):
     """The gradient of fused_gemm (tcu_fused_gemm_backward): a dict with "dA" (like A), "dB" (like Bt) and "dbias" (float32),
     those that are asked for.  Z: what fused_gemm returned as the activation's argument; the gradient of C is beta * dD."""
     torch = _torch()
@@ -792,19 +810,16 @@ def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_grad
     s = FusedGemmShape(dtype=dtype, activation=_enum(Activation, activation), M=M, N=N, K=K)
     pd, pb, pz = _operand(dD, "dD", M, N, A), _operand(Bt, "Bt", N, K, A), _operand(Z, "Z", M, N, A)
 
-    def body(raw):
-        got = {}
-        if input_gradient:
-            got["dA"] = torch.empty(A.shape, dtype=A.dtype, device=A.device)
-        if weight_gradient:
-            got["dB"] = torch.empty(Bt.shape, dtype=A.dtype, device=A.device)
-        if bias_gradient:
-            got["dbias"] = torch.empty(N, dtype=torch.float32, device=A.device)
-        args = (ctypes.byref(s), *pd, pa, lda, *pb, *pz, *(v for n in ("dA", "dB") for v in ((got[n].data_ptr(), K) if n in got else (None, 0))), got["dbias"].data_ptr() if bias_gradient else None)
-        _call_with_workspace(lib().tcu_fused_gemm_backward, args, (M, N, K, s.activation == 0, input_gradient, weight_gradient, bias_gradient), workspace, A.device, raw)
-        return got
-
-    return _launch_on(A.device, stream, body)
+    got = {}
+    if input_gradient:
+        got["dA"] = _new(A)
+    if weight_gradient:
+        got["dB"] = _new(Bt)
+    if bias_gradient:
+        got["dbias"] = torch.empty(N, dtype=torch.float32, device=A.device)
+    args = (ctypes.byref(s), *pd, pa, lda, *pb, *pz, *(v for n in ("dA", "dB") for v in ((got[n].data_ptr(), K) if n in got else (None, 0))), got["dbias"].data_ptr() if bias_gradient else None)
+    _call_with_workspace(lib().tcu_fused_gemm_backward, args, (M, N, K, s.activation == 0, input_gradient, weight_gradient, bias_gradient), workspace, A.device, stream)
+    return got
 
 
 def fill(t, value, stream=None):

@@ -29,6 +29,8 @@ inline int check_vector(const std::string &w, const char *name, const void *p, s
   if (p && !aligned_to(p, 16)) *whole_chunks = false;
   return TCU_OK;
 }
+// The size a call reports for a workspace of which it uses `used` bytes: 256 says that it uses none.
+inline size_t smallest_workspace(size_t used) { return used == 0 ? 256 : used < 512 ? 512 : used; }
 inline int check_workspace(const std::string &w, const void *workspace, size_t have, size_t need) {
   if (have < need) return report_failure(TCU_ERR_WORKSPACE, w + ": workspace of " + std::to_string(have) + " bytes, needs " + std::to_string(need));
   if (!aligned_to(workspace, 256)) return report_failure(TCU_ERR_INVALID_ARG, w + ": the workspace must be 256-byte aligned");

@@ -252,13 +252,14 @@ TCU_DEVICE void activate_slope(int act, const float (&z)[N], float (&value)[N], 
     }
   } else {  // z s(v): s + z s (1 - s) v'
     const float cubic = act == kActGelu ? kGeluTwoA * kGeluB : 0.0f, linear = act == kActGelu ? kGeluTwoA : 1.0f;
+    const float most = act == kActGelu ? 32.0f : 3.0e38f;  // beyond +-32 the gelu's sigmoid is 0 or 1, and its argument need not grow (it could overflow)
 #pragma unroll
     for (int e = 0; e < N; e++) {
       float s, r;
-      const float cz = cubic * z[e];
-      sigmoid_pair<EXACT>(z[e] * __builtin_fmaf(cz, z[e], linear), &s, &r);
-      value[e] = z[e] * s;
-      slope[e] = __builtin_fmaf(value[e] * r, __builtin_fmaf(3.0f * cz, z[e], linear), s);
+      const float c = z[e] > most ? most : z[e] < -most ? -most : z[e], cz = cubic * c, v = c * __builtin_fmaf(cz, c, linear);
+      sigmoid_pair<EXACT>(v, &s, &r);
+      value[e] = v < -87.0f ? z[e] * 0.0f : z[e] * s;  // the pair's s does not go below e^-87
+      slope[e] = __builtin_fmaf(value[e] * r, __builtin_fmaf(3.0f * cz, c, linear), v < -87.0f ? 0.0f : s);
     }
   }
 }

@@ -143,7 +143,7 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   const bool odd_k = few_k || K % 8 != 0;     // nor a part of a chunk
   const bool pack_a = !g.few_rows && K && (odd_k || !rows_ready(A, M > 1 ? lda : 8)), pack_b = !g.few_rows && K && (odd_k || !rows_ready(B, N > 1 ? ldb : 8));
   const size_t ldk = few_k ? 64 : up_to(K, 8), a_bytes = pack_a ? part_bytes(M * ldk * 2) : 0, b_bytes = pack_b ? part_bytes(N * ldk * 2) : 0;
-  const size_t bytes = g.share_bytes + a_bytes + b_bytes, need = bytes < 256 ? 256 : bytes;
+  const size_t bytes = g.share_bytes + a_bytes + b_bytes, need = smallest_workspace(bytes);
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
   if (!workspace) {
     *workspace_bytes = need;
@@ -214,7 +214,7 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   const size_t dz_bytes = own_dz ? part_bytes(M * ldn * 2) : 0, dzt_bytes = dB ? part_bytes(N * ldm * 2) : 0, at_bytes = dB ? part_bytes(K * ldm * 2) : 0, bt_bytes = dA ? part_bytes(K * ldn * 2) : 0;
   const size_t strips = (M + 63) / 64, sums_bytes = dbias ? part_bytes(strips * N * 4) : 0;
   const size_t share_bytes = (dA ? ga.share_bytes : 0) > (dB ? gb.share_bytes : 0) ? ga.share_bytes : (dB ? gb.share_bytes : 0);
-  const size_t bytes = share_bytes + dz_bytes + dzt_bytes + at_bytes + bt_bytes + sums_bytes, need = bytes < 256 ? 256 : bytes;
+  const size_t bytes = share_bytes + dz_bytes + dzt_bytes + at_bytes + bt_bytes + sums_bytes, need = smallest_workspace(bytes);
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
   if (!workspace) {
     *workspace_bytes = need;

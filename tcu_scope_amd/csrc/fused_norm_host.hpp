@@ -87,7 +87,7 @@ inline NormBackPlan plan_norm_backward(const tcu_fused_norm_shape *s, size_t vec
   plan.parts = plan.blocks * rows_per_block;
   plan.vectors = vectors;
   const size_t bytes = plan.parts * vectors * s->dim * 4;
-  plan.bytes = bytes < 256 ? 256 : bytes;
+  plan.bytes = smallest_workspace(bytes);
   return plan;
 }
 

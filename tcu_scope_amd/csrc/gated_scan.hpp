@@ -31,12 +31,13 @@
 // published and in which order it is combined depends on places alone, never on timing: the same input gives the same bits
 // every time.  The chain of waits is a 64th of the tiles long (with every 8th tile handing a state on, 512 tiles along a
 // sequence waited for a third of their time: 65536 x 2048 fp16, 390 us against 264 with the waits left out).
-//
-// 65536 x 2048 fp16 takes 173 us (805 MB, 4.6 TB/s; a copy reaches 5.1), 8 x 4096 x 2048 bf16 98 us (403 MB, 4.1 TB/s), its
-// gradient 164 us (805 MB, 4.9 TB/s), 8191 x 1000 packed bf16 19 us (49 MB; some 130 blocks at once, each bound by its own
-// chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 23 us (63 MB; likewise, element-wise accesses).
 // Tiles are handed out by a ticket, so the one that is waited for has always been started; a wait is bounded and leaves NaN
 // in what depended on it.
+//
+// 65536 x 2048 fp16 takes 173 us (805 MB, 4.6 TB/s; a copy reaches 5.1), 8 x 4096 x 2048 bf16 98 us (403 MB, 4.1 TB/s), its
+// gradient 164 us (805 MB, 4.9 TB/s), 8191 x 1000 packed bf16 19 us (49 MB; 256 tiles, a block for each compute unit,
+// bound by its own chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 23 us (63 MB; likewise, with
+// element-wise accesses).
 #pragma once
 
 #include "elements.hpp"

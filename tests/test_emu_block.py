@@ -478,6 +478,29 @@ def test_fused_norm_and_gradient(emu, dtype, case):
             ref.check(v, got[name] * factor, err[name] * abs(factor) * 1.01, "f32", name)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("actn", ["relu", "gelu", "silu", "sigmoid"])
+def test_activations_at_the_ends_of_their_range(emu, dtype, actn):
+    """Gates as large as the type holds: the activation is 0, 1 or the gate itself there, its slope 0 or 1, and nothing overflows on the way."""
+    emu = norm_emu(emu)
+    big = 1e30
+    gate = ref.to_f64(ref.to_bits(np.array([[-big, -1e19, -1000.0, -200.0, -90.0, -40.0, 40.0, 90.0, 200.0, 1000.0, 1e19, big]]), dtype), dtype)
+    dim = gate.shape[1]
+    x, dout = np.ones((1, dim)), np.full((1, dim), 2.0 ** -100)  # y = 1 everywhere up to eps
+    low = gate < 0
+    want = {"relu": np.where(low, 0, gate), "gelu": np.where(low, 0, gate), "silu": np.where(low, 0, gate), "sigmoid": np.where(low, 0, 1.0)}[actn]
+    slope = {"sigmoid": np.zeros_like(gate)}.get(actn, np.where(low, 0.0, 1.0))
+    mx, mg, mo, md, mdx, mdg = (Matrix(v, dtype) for v in (x, gate, x, dout, x, x))
+    shape = NormShape(DTYPES[dtype], 0, 0, ACTS[actn], 1, dim, 1e-30, 1.0)
+    assert emu.emu_fused_norm(ctypes.byref(shape), *operand(mx), *NULL, *operand(mg), None, None, None, *operand(mo), *NULL) == 0
+    small = 40 * np.exp(-40.0) * 1.01  # silu and sigmoid at +-40 are this far from their limits
+    assert (np.abs(mo.get() - want) <= 2.0 ** -7 * np.abs(want) + small).all()
+    call = lambda ws, need: emu.emu_fused_norm_backward(ctypes.byref(shape), *operand(md), *operand(mx), *operand(mg), None, None, None, *NULL, *NULL, *operand(mdx), *operand(mdg), *NULL, None, None, None, ws, need)
+    kept, ws, have = workspace_for(call)
+    assert call(ws, ctypes.byref(have)) == 0
+    assert (np.abs(mdg.get() / 2.0 ** -100 - slope) <= 2.0 ** -7 * slope + small).all() and np.isfinite(mdx.get()).all()
+
+
 def test_fused_norm_many_rows(emu):
     """More rows than blocks in the gradient's kernel, one wave per row with several rows per block, and rows without any content."""
     emu = norm_emu(emu)
@@ -566,7 +589,8 @@ def test_fused_norm_refusals(emu):
     assert back(dr=m(2)) == 1 and "same buffer" in err()
     assert back(dw=p + 2) == 1 and "d_dweight" in err()
     need = sz(0)
-    assert back(ws=None, have=need, dw=p) == 0 and need.value == 256
+    assert back(ws=None, have=need, dw=p) == 0 and need.value == 512  # 256 says that nothing is kept there
+    assert back(ws=None, have=need) == 0 and need.value == 256
 
 
 # ---- fused product ----------------------------------------------------------------------------------------------
