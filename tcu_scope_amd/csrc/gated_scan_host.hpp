@@ -137,7 +137,7 @@ inline int gated_scan_dispatch(const tcu_gated_scan_shape *s, const void *x, siz
   }
   if (int rc = check_vector(w, "d_h0", h0, 4, &aligned)) return rc;
   if (int rc = check_vector(w, "d_h_last", h_last, 4, &aligned)) return rc;
-  if (s->num_sequences == 0) return TCU_OK;
+  if (s->num_sequences == 0 && (plan.rows == 0 || !s->zero_outside)) return TCU_OK;
   GatedScanParams p{};
   p.x = x;
   p.x_stride = x_stride;
@@ -177,7 +177,7 @@ inline int gated_scan_backward_dispatch(const tcu_gated_scan_shape *s, const voi
   if (int rc = check_vector(w, "d_h0", h0, 4, &aligned)) return rc;
   if (int rc = check_vector(w, "d_dh_last", dh_last, 4, &aligned)) return rc;
   if (int rc = check_vector(w, "d_dh0", dh0, 4, &aligned)) return rc;
-  if (s->num_sequences == 0) return TCU_OK;
+  if (s->num_sequences == 0 && (plan.rows == 0 || !s->zero_outside)) return TCU_OK;
   GatedScanParams p{};
   p.dh = dh;
   p.dh_stride = dh_stride;

@@ -220,6 +220,19 @@ def test_no_rows_and_empty_sequences(emu):
     assert run_scan(emu, s, empty, empty, empty, None, None) == 0
 
 
+@pytest.mark.parametrize("zero_outside", [0, 1])
+def test_rows_without_any_sequence(emu, zero_outside):
+    ones = Matrix(np.ones((5, 12)), "f32")
+    s, keep = shape_of("f32", "sigmoid", 5, 12, [0], 32, zero_outside=zero_outside)
+    h, dx, dg = (Matrix(np.full((5, 12), 5.0), "f32") for _ in range(3))
+    assert run_scan(emu, s, ones, ones, h, None, None) == 0
+    call = lambda ws, need: emu.emu_gated_scan_backward(ctypes.byref(s), *(v for m in (ones, ones, ones, ones) for v in (m.ptr, m.stride)), None, None, dx.ptr, dx.stride, dg.ptr, dg.stride, None, ws, need)
+    kept, ws, have = workspace_for(call)
+    assert call(ws, ctypes.byref(have)) == 0
+    for m in (h, dx, dg):
+        assert (m.get() == (0.0 if zero_outside else 5.0)).all()
+
+
 def test_states_do_not_pass_between_sequences(emu):
     """An infinite or NaN state stays in its sequence: a sequence's beginning replaces what came before, it does not multiply it by 0."""
     rows, channels = 400, 8

@@ -103,6 +103,11 @@ def test_empty(tcu):
     assert torch.equal(last, h0)
     _, _, d0 = tcu.gated_scan_backward(x, x, x, x, dh_last=h0, offsets=torch.zeros(3, dtype=torch.int64, device="cuda"))
     assert torch.equal(d0, h0)
+    # rows, and no sequence that has them
+    x, none = torch.ones(5, 8, device="cuda", dtype=torch.float16), torch.zeros(1, dtype=torch.int32, device="cuda")
+    h, last = tcu.gated_scan(x, x, offsets=none)
+    dx, dg, d0 = tcu.gated_scan_backward(x, x, x, x, offsets=none)
+    assert last.shape == d0.shape == (0, 8) and all((t == 0).all() for t in (h, dx, dg))
 
 
 def test_side_stream_and_graph(tcu):
