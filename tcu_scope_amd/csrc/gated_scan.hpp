@@ -36,8 +36,8 @@
 //
 // 65536 x 2048 fp16 takes 173 us (805 MB, 4.6 TB/s; a copy reaches 5.1), 8 x 4096 x 2048 bf16 98 us (403 MB, 4.1 TB/s), its
 // gradient 164 us (805 MB, 4.9 TB/s), 8191 x 1000 packed bf16 19 us (49 MB; 256 tiles, a block for each compute unit,
-// bound by its own chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 23 us (63 MB; likewise, with
-// element-wise accesses).
+// bound by its own chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 23 us (63 MB; likewise, its rows
+// beginning anywhere).
 #pragma once
 
 #include "elements.hpp"
