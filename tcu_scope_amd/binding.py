@@ -444,9 +444,14 @@ def gemm(A, Bt, alpha=1.0, beta=0.0, C=None, out=None, variant=Variant.AUTO, str
 # ---- recurrent blocks of language models ------------------------------------------------------------------------
 
 
+_dtype_codes = {}
+
+
 def _dtype_code(t, name):
-    torch = _torch()
-    code = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}.get(t.dtype)
+    if not _dtype_codes:
+        torch = _torch()
+        _dtype_codes.update({torch.float16: 0, torch.bfloat16: 1, torch.float32: 2})
+    code = _dtype_codes.get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be a float16, bfloat16 or float32 tensor")
     if not t.is_cuda:
@@ -474,7 +479,7 @@ def _enum(kind, value):
 def _matrix(t, name, like=None):
     """(pointer, rows, row stride) of a tensor whose leading dimensions can be read as one: rows of contiguous elements at an even distance."""
     sizes = t.shape
-    if like is not None and not (t.dtype is like.dtype and sizes == like.shape and t.device == like.device):
+    if like is not None and not (sizes == like.shape and t.dtype is like.dtype and t.get_device() == like.get_device()):
         raise ValueError(f"{name} must have the shape, type and device of the other operands ({tuple(like.shape)}, {like.dtype}, {like.device}); got {tuple(sizes)}, {t.dtype}, {t.device}")
     if len(sizes) < 2:
         raise ValueError(f"{name} must have at least two dimensions")
@@ -500,7 +505,7 @@ def _matrix(t, name, like=None):
 def _vector_f32(t, name, shape, device):
     if t is None:
         return None
-    if t.dtype != _torch().float32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+    if not (t.dtype is _torch().float32 and t.shape == shape and t.is_contiguous() and t.device == device):
         raise ValueError(f"{name} must be a contiguous float32 tensor of shape {tuple(shape)} on {device}")
     return t.data_ptr()
 
@@ -521,11 +526,10 @@ def _launches(fn):
         operand = args[0] if args else kw.get(first)
         if not (isinstance(operand, torch.Tensor) and operand.is_cuda):
             raise ValueError(f"{first} must be a CUDA tensor")
-        device = operand.device
-        index = device.index
+        index = operand.get_device()
         if stream is not None:
-            if stream.device != device:
-                raise ValueError(f"the stream belongs to {stream.device}, the tensors to {device}")
+            if stream.device != operand.device:
+                raise ValueError(f"the stream belongs to {stream.device}, the tensors to {operand.device}")
             with torch.cuda.stream(stream):
                 return fn(*args, stream=stream.cuda_stream, **kw)
         if torch.cuda.current_device() == index:
@@ -539,7 +543,20 @@ def _launches(fn):
 def _new(t):
     """An uninitialised contiguous tensor like t."""
     torch = _torch()
-    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _result(given, name, like):
+    """(tensor, pointer, row stride): the tensor given for a result like `like`, or a new one."""
+    if given is None:
+        t = _new(like)
+        return t, t.data_ptr(), like.shape[-1]
+    p, _, stride = _matrix(given, name, like)
+    return given, p, stride
+
+
+def _new_f32(t, shape):
+    return t.new_empty(shape, dtype=_torch().float32)
 
 
 _untouched = {}
@@ -611,7 +628,6 @@ def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=
     name: "decay" (a = g, b = x), "log" (a = exp(g), b = x), "sigmoid" (a = sigmoid(g), b = (1 - a) x).  h0, h_last:
     (sequences, channels) float32, the states in front of and behind the sequences.  Rows outside all sequences
     are left as they are in `out`, and zero in a result this call allocates.  out may be x or g."""
-    torch = _torch()
     s = _scan_shape(x, gate, offsets, h0)
     states = (s.num_sequences, s.channels)
     px, _, sx = _matrix(x, "x")
@@ -619,9 +635,8 @@ def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=
     p0 = _vector_f32(h0, "h0", states, x.device)
     s.zero_outside = out is None
 
-    h = _new(x) if out is None else out
-    last = torch.empty(states, dtype=torch.float32, device=x.device) if h_last is None else h_last
-    ph, _, sh = _matrix(h, "out", x)
+    h, ph, sh = _result(out, "out", x)
+    last = _new_f32(x, states) if h_last is None else h_last
     args = (ctypes.byref(s), px, sx, pg, sg, ph, sh, p0, _vector_f32(last, "h_last", states, x.device))
     _call_with_workspace(lib().tcu_gated_scan, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, x.device, stream)
     return h, last
@@ -634,7 +649,6 @@ def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, o
     dh, dh_last: gradients with respect to h and h_last (dh_last may be None); h: what gated_scan returned; x is read for
     the sigmoid gate only and may be None for the others.  dh0 is (sequences, channels) float32.  dx and dg may be given
     (both or neither), and be dh, x or g; rows outside all sequences are then left as they are, and otherwise zero."""
-    torch = _torch()
     s = _scan_shape(g, gate, offsets, h0, "g")
     states = (s.num_sequences, s.channels)
     if x is None and s.gate == Gate.SIGMOID:
@@ -648,10 +662,8 @@ def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, o
         raise ValueError("dx and dg are given both or neither")
     s.zero_outside = dx is None
 
-    out_x, out_g = (dx, dg) if dx is not None else (_new(g), _new(g))
-    dh0 = torch.empty(states, dtype=torch.float32, device=g.device)
-    pox, _, sox = _matrix(out_x, "dx", g)
-    pog, _, sog = _matrix(out_g, "dg", g)
+    (out_x, pox, sox), (out_g, pog, sog) = _result(dx, "dx", g), _result(dg, "dg", g)
+    dh0 = _new_f32(g, states)
     args = (ctypes.byref(s), pd, sd, px, sx, pg, sg, ph, sh, p0, pl, pox, sox, pog, sog, dh0.data_ptr())
     _call_with_workspace(lib().tcu_gated_scan_backward, args, (s.dtype, s.num_rows, s.channels, offsets is None), workspace, g.device, stream)
     return out_x, out_g, dh0
@@ -679,8 +691,7 @@ def gated_scan_step(x, g, state, gate=Gate.SIGMOID, slots=None, new_state=None, 
     if slots is not None and (slots.dtype != torch.int32 or slots.device != x.device or tuple(slots.shape) != (rows,) or not slots.is_contiguous()):
         raise ValueError("slots must be a contiguous int32 vector with one entry per row, on the same device")
 
-    h = _new(x) if out is None else out
-    ph, _, sh = _matrix(h, "out", x)
+    h, ph, sh = _result(out, "out", x)
     _check(lib().tcu_gated_scan_step(dtype, _enum(Gate, gate), channels, rows, px, sx, pg, sg, ph, sh, ps, pn, shape[0], slots.data_ptr() if slots is not None else None, out is None, stream))
     return h
 
@@ -689,9 +700,12 @@ def _vector(t, name, n, like):
     """Pointer of a vector operand of `like`'s type with n entries (None: null)."""
     if t is None:
         return None
-    if t.dtype != like.dtype or t.device != like.device or tuple(t.shape) != (n,) or not t.is_contiguous():
+    if not (t.dtype is like.dtype and t.shape == (n,) and t.is_contiguous() and t.get_device() == like.get_device()):
         raise ValueError(f"{name} must be a contiguous vector of {n} entries of {like.dtype} on {like.device}")
     return t.data_ptr()
+
+
+_ADD_NORM = int(NormOrder.ADD_NORM)
 
 
 def _optional(t, name, like):
@@ -701,7 +715,7 @@ def _optional(t, name, like):
 def _norm_shape(x, gate, norm, order, activation, eps, scale, name):
     dtype = _dtype_code(x, name)
     if activation is None:
-        activation = Activation.NONE if gate is None else Activation.SILU
+        activation = "none" if gate is None else "silu"
     p, rows, stride = _matrix(x, name)
     return p, stride, FusedNormShape(dtype=dtype, norm=_enum(Norm, norm), order=_enum(NormOrder, order), activation=_enum(Activation, activation), rows=rows, dim=x.shape[-1], eps=eps, scale=scale)
 
@@ -713,17 +727,17 @@ def fused_norm(x, weight=None, bias=None, residual=None, gate=None, scale=1.0, c
     order "add_norm": z = residual + s x, returns (act(gate) y(z), z), or act(gate) y(x) alone without a residual.
     order "norm_add": returns residual + s act(gate) y(x).  y is the rms or layer norm times weight plus bias.
     activation: of the gate, by default silu.  weight, bias, channel_scale: vectors of x's type."""
-    torch = _torch()
     px, sx, s = _norm_shape(x, gate, norm, order, activation, eps, scale, "x")
     pr, pg = _optional(residual, "residual", x), _optional(gate, "gate", x)
-    vectors = [_vector(t, n, s.dim, x) for t, n in ((weight, "weight"), (bias, "bias"), (channel_scale, "channel_scale"))]
-    keep = s.order == NormOrder.ADD_NORM and residual is not None
+    dim = x.shape[-1]
+    vectors = _vector(weight, "weight", dim, x), _vector(bias, "bias", dim, x), _vector(channel_scale, "channel_scale", dim, x)
+    keep = s.order == _ADD_NORM and residual is not None
     if residual_out is not None and not keep:
         raise ValueError("residual_out goes with the order add_norm and a residual")
 
-    o = _new(x) if out is None else out
-    z = None if not keep else _new(x) if residual_out is None else residual_out
-    _check(lib().tcu_fused_norm(ctypes.byref(s), px, sx, *pr, *pg, *vectors, *_optional(o, "out", x), *_optional(z, "residual_out", x), stream))
+    o, po, so = _result(out, "out", x)
+    z, pz, sz = _result(residual_out, "residual_out", x) if keep else (None, None, 0)
+    _check(lib().tcu_fused_norm(ctypes.byref(s), px, sx, *pr, *pg, *vectors, po, so, pz, sz, stream))
     return (o, z) if keep else o
 
 
@@ -736,9 +750,8 @@ def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, c
     dresidual_out is the gradient with respect to residual_out and "dresidual" is returned if it is given; the gradient of
     channel_scale needs the forward call's x.  order norm_add: the residual's gradient is dout itself.  The vectors'
     gradients are float32."""
-    torch = _torch()
     pd, sd, s = _norm_shape(dout, gate, norm, order, activation, eps, scale, "dout")
-    add_norm = s.order == NormOrder.ADD_NORM
+    add_norm = s.order == _ADD_NORM
     pz, pg = _matrix(z, "z", dout)[::2], _optional(gate, "gate", dout)
     vectors = [_vector(t, n, s.dim, dout) for t, n in ((weight, "weight"), (bias, "bias"), (channel_scale, "channel_scale"))]
     ps = _optional(dresidual_out, "dresidual_out", dout)
@@ -747,7 +760,7 @@ def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, c
     px = _optional(x if add_norm and channel_scale is not None else None, "x", dout)
 
     new = lambda: _new(dout)
-    column = lambda: torch.empty(s.dim, dtype=torch.float32, device=dout.device)
+    column = lambda: _new_f32(dout, s.dim)
     got = {"dx": new()}
     if gate is not None:
         got["dgate"] = new()
@@ -766,7 +779,7 @@ def _operand(t, name, rows, columns, like):
     """(pointer, leading dimension) of a matrix operand of the fused product (None: null)."""
     if t is None:
         return None, 0
-    if t.dtype != like.dtype or t.device != like.device:
+    if t.dtype is not like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{name} must have the type and device of the other operands ({like.dtype}, {like.device})")
     p, n, stride = _matrix(t, name)
     if n != rows or t.shape[-1] != columns:
@@ -780,7 +793,6 @@ def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, o
 
     Returns D, or with return_preactivation or a `preactivation` tensor to fill (D, A @ Bt.T + bias); the second is what
     fused_gemm_backward wants as Z.  C is not read when beta is 0; out may be C."""
-    torch = _torch()
     dtype = _dtype_code(A, "A")
     pa, M, lda = _matrix(A, "A")
     if Bt.dim() != 2 or Bt.shape[-1] != A.shape[-1]:
@@ -789,10 +801,15 @@ def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, o
     s = FusedGemmShape(dtype=dtype, activation=_enum(Activation, activation), M=M, N=N, K=K, beta=beta if C is not None else 0.0)
     pb, pbias, pc = _operand(Bt, "Bt", N, K, A), _vector(bias, "bias", N, A), _operand(C, "C", M, N, A)
 
-    new = lambda: torch.empty((*A.shape[:-1], N), dtype=A.dtype, device=A.device)
-    D = new() if out is None else out
-    Z = new() if preactivation is None and return_preactivation else preactivation
-    args = (ctypes.byref(s), pa, lda, *pb, pbias, *pc, *_operand(D, "out", M, N, A), *_operand(Z, "preactivation", M, N, A))
+    def result(given, name):
+        if given is not None:
+            return (given, *_operand(given, name, M, N, A))
+        t = A.new_empty((*A.shape[:-1], N))
+        return t, t.data_ptr(), N
+
+    D, *pd = result(out, "out")
+    Z, *pz = result(preactivation, "preactivation") if return_preactivation or preactivation is not None else (None, None, 0)
+    args = (ctypes.byref(s), pa, lda, *pb, pbias, *pc, *pd, *pz)
     _call_with_workspace(lib().tcu_fused_gemm, args, (M, N, K), workspace, A.device, stream)
     return D if Z is None else (D, Z)
 
@@ -801,7 +818,6 @@ def fused_gemm(A, Bt, bias=None, activation=Activation.NONE, C=None, beta=1.0, o
 def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_gradient=True, input_gradient=True, weight_gradient=True, workspace=None, *, stream=None):
     """The gradient of fused_gemm (tcu_fused_gemm_backward): a dict with "dA" (like A), "dB" (like Bt) and "dbias" (float32),
     those that are asked for.  Z: what fused_gemm returned as the activation's argument; the gradient of C is beta * dD."""
-    torch = _torch()
     dtype = _dtype_code(A, "A")
     pa, M, lda = _matrix(A, "A")
     if Bt.dim() != 2 or Bt.shape[-1] != A.shape[-1]:
@@ -816,7 +832,7 @@ def fused_gemm_backward(dD, A, Bt, Z=None, activation=Activation.NONE, bias_grad
     if weight_gradient:
         got["dB"] = _new(Bt)
     if bias_gradient:
-        got["dbias"] = torch.empty(N, dtype=torch.float32, device=A.device)
+        got["dbias"] = _new_f32(A, N)
     args = (ctypes.byref(s), *pd, pa, lda, *pb, *pz, *(v for n in ("dA", "dB") for v in ((got[n].data_ptr(), K) if n in got else (None, 0))), got["dbias"].data_ptr() if bias_gradient else None)
     _call_with_workspace(lib().tcu_fused_gemm_backward, args, (M, N, K, s.activation == 0, input_gradient, weight_gradient, bias_gradient), workspace, A.device, stream)
     return got
