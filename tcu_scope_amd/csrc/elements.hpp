@@ -250,16 +250,24 @@ TCU_DEVICE void activate_slope(int act, const float (&z)[N], float (&value)[N], 
       value[e] = s;
       slope[e] = s * r;
     }
-  } else {  // z s(v): s + z s (1 - s) v'
-    const float cubic = act == kActGelu ? kGeluTwoA * kGeluB : 0.0f, linear = act == kActGelu ? kGeluTwoA : 1.0f;
-    const float most = act == kActGelu ? 32.0f : 3.0e38f;  // beyond +-32 the gelu's sigmoid is 0 or 1, and its argument need not grow (it could overflow)
+  } else if (act == kActSilu) {  // z s(z): s + z s (1 - s)
 #pragma unroll
     for (int e = 0; e < N; e++) {
       float s, r;
-      const float c = z[e] > most ? most : z[e] < -most ? -most : z[e], cz = cubic * c, v = c * __builtin_fmaf(cz, c, linear);
-      sigmoid_pair<EXACT>(v, &s, &r);
-      value[e] = v < -87.0f ? z[e] * 0.0f : z[e] * s;  // the pair's s does not go below e^-87
-      slope[e] = __builtin_fmaf(value[e] * r, __builtin_fmaf(3.0f * cz, c, linear), v < -87.0f ? 0.0f : s);
+      const float y = z[e] < -87.0f ? -87.0f : z[e];  // below it the value and the slope are 0 but for 1e-36
+      sigmoid_pair<EXACT>(y, &s, &r);
+      value[e] = y * s;
+      slope[e] = __builtin_fmaf(value[e], r, s);
+    }
+  } else {  // z s(v): s + z s (1 - s) v'
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      float s, r;
+      // beyond +-32 the sigmoid is 0 or 1, and its argument and v' need not grow any more (they could overflow)
+      const float low = z[e] < -32.0f ? -32.0f : z[e], c = low > 32.0f ? 32.0f : low, cz = kGeluTwoA * kGeluB * c;
+      sigmoid_pair<EXACT>(c * __builtin_fmaf(cz, c, kGeluTwoA), &s, &r);
+      value[e] = low * s;
+      slope[e] = __builtin_fmaf(value[e] * r, __builtin_fmaf(3.0f * cz, c, kGeluTwoA), s);
     }
   }
 }
