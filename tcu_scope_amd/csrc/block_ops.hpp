@@ -63,5 +63,13 @@ TCU_DEVICE float4_t mfma_16x16x32_chunks(uint4_t a, uint4_t b, float4_t c) {
     return mfma_16x16x32(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c);
 }
 
+// 16 lanes read a block of 4 rows of 16 elements of 16 bits, lane 4 r + c the elements 4 c ... 4 c + 3 of row r (8 bytes at `q`);
+// lane i gets column i of it.
+TCU_DEVICE uint2_t read_column_of_four(const half_t *q) {
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  using lds_ptr_t = __attribute__((address_space(3))) short4_t *;
+  return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr_t)(uintptr_t)lds_address_of(q)));
+}
+
 }  // namespace tcu
 #endif  // TCU_BLOCK_OPS_HPP

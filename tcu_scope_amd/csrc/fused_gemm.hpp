@@ -3,7 +3,9 @@
 //
 // Gradient: dZ = dD * act'(Z) element by element, dA = dZ B^T (M x K), dB = dZ^T A (N rows of K), dbias = the column sums of
 // dZ, dC = beta dD.  The two products sum over N and over M, along which B and A (and dZ for the second) are not contiguous:
-// they run on transposed copies in the workspace, which one launch writes, dZ and its transpose in the same pass.
+// the tile kernel takes such operands as they are, rows of K one below the other, and turns them on the way from LDS to registers.
+// Where their rows are no whole chunks, or fewer than a step, it runs on transposed copies in the workspace instead.  One launch
+// writes those, dZ, and its column sums.
 //
 //   fused_gemm_tile_kernel : many rows.  256 x 256, 192 x 192 or 128 x 128 block tiles on 16x16x32 MFMAs, K steps of 64, operands
 //                moved global -> LDS by transfers that run two steps ahead (three buffers for A, two for B; three for B too where
@@ -15,8 +17,9 @@
 //                fused_gemm_join_kernel adds their fp32 shares in a fixed order.
 //   fused_gemm_few_rows_kernel : up to 32 rows.  Bound by reading B once: a block takes 16 columns of the output and all rows,
 //                its waves share K and meet in LDS.  5 x 4096 x 8192 fp16 (67 MB) 16 us = 4.1 TB/s, launch included.
-//   gradient_layout_kernel : what the gradient's products need laid out, bound by HBM traffic; with 4001 x 4096 x 2056 bf16 38 us,
-//                and the products on it 67 and 66 us (1.0 PFLOP/s: the tiles fill their last round of compute units badly).
+//   gradient_layout_kernel : dZ and what has to be transposed, bound by HBM traffic.  4001 x 4096 x 2056 bf16 with silu: 17 us, and the
+//                products 76 and 78 (0.9 PFLOP/s); on transposed copies 38, 67 and 66.  8192 x 8192 x 2048: 437 us together, on
+//                transposed copies 469; 130 x 7616 x 4120: 82 and 103.
 // Sums are fp32; the epilogue is applied to the fp32 sum and each result rounded once.  dZ is rounded to the operands' type,
 // because the matrix unit takes operands of 16 bits; its column sums are taken before that.
 #pragma once
@@ -61,7 +64,18 @@ TCU_DEVICE void fused_gemm_finish(const FusedGemmParams &p, size_t row, size_t c
 // rows of either lie within 4 GiB.  A 192 x 192 tile has room for three buffers of B as well: the tiles of step s + 3 go out
 // behind the barrier of step s, into its buffers, and have two steps to arrive.  The product is formed transposed (B fragment first), so a lane owns row (lane & 15)
 // and four adjacent columns of every 16 x 16 tile.
-template <int DT, bool WHOLE, int W8, bool TAIL>
+constexpr int kAlong = 0, kDownB = 1, kDownBoth = 2;  // LAYOUT: K along the rows of both operands, down the rows of B, of both
+// Where a tile of 16 U columns and 64 rows of K holds its 32-byte unit u of row k in LDS.  Two groups of 16 lanes read at a time, rows
+// 8 g + 4 h + 0 ... 3 of two neighbouring g; the units of one column in those 8 rows lie in different banks (U = 12: in four of
+// twelve columns pairs of them share banks).  Its own inverse.
+template <unsigned U>
+TCU_DEVICE unsigned unit_place(unsigned k, unsigned u) {
+  const unsigned odd = (k >> 3) & 1;
+  if constexpr (U == 12) return ((u & 3) ^ (k & 3)) | (((u >> 2) < 2 ? (u >> 2) ^ odd : u >> 2) << 2);
+  return u ^ ((k & 3) | odd << 2);
+}
+
+template <int DT, bool WHOLE, int W8, bool TAIL, int LAYOUT>
 TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t tile_n, size_t step0, size_t steps, bool tail, float *share) {
   constexpr int BK = 64, ROWH = BK, CPR = 8, RPT = 8, RS = 1, SUB = 2, NA = 3, NB = W8 == 6 ? 3 : 2;
   constexpr int TILE = 32 * W8, WT = 16 * W8;
@@ -76,8 +90,12 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wm = wave >> 1, wn = wave & 1;
   const size_t row0 = tile_m * TILE, col0 = tile_n * TILE;
-  const unsigned last_a = (unsigned)(p.M - row0 < TILE ? p.M - row0 : TILE) - 1, last_b = (unsigned)(p.N - col0 < TILE ? p.N - col0 : TILE) - 1;
-  const char *A = static_cast<const char *>(p.A) + row0 * p.lda * 2, *B = static_cast<const char *>(p.B) + col0 * p.ldb * 2;
+  constexpr bool DOWN_A = LAYOUT == kDownBoth, DOWN_B = LAYOUT != kAlong;
+  constexpr unsigned UNITS = 2 * W8, CHUNKS = 2 * UNITS;  // of a row of the tile of an operand whose K runs down the rows
+  // the last row of the tile that exists; of an operand whose K runs down the rows, where the last chunk of 8 columns begins
+  auto last_of = [](size_t left, bool down) { return down ? (unsigned)((left < TILE ? left : TILE) + 7) / 8 * 8 - 8 : (unsigned)(left < TILE ? left : TILE) - 1; };
+  const unsigned last_a = last_of(p.M - row0, DOWN_A), last_b = last_of(p.N - col0, DOWN_B);
+  const char *A = static_cast<const char *>(p.A) + row0 * (DOWN_A ? 1 : p.lda) * 2, *B = static_cast<const char *>(p.B) + col0 * (DOWN_B ? 1 : p.ldb) * 2;
 
   float4_t acc[W8][W8];
 #pragma unroll
@@ -94,7 +112,27 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
   int ko[SUB];
 #pragma unroll
   for (int kk = 0; kk < SUB; kk++) ko[kk] = ((4 * kk + kq) ^ fsw) * 8;
+  // operands whose K runs down the rows: the lane's piece of unit w W8 + i
+  int da[W8], db[W8];
+#pragma unroll
+  for (int i = 0; i < W8; i++) {
+    const unsigned k = (unsigned)(8 * kq + (frow >> 2));
+    da[i] = (int)(k * TILE + unit_place<UNITS>(k, wm * W8 + i) * 16) + 4 * (frow & 3);
+    db[i] = (int)(k * TILE + unit_place<UNITS>(k, wn * W8 + i) * 16) + 4 * (frow & 3);
+  }
   auto fragment = [](const half_t *q) { return *reinterpret_cast<const uint4_t *>(q); };
+  auto turned = [](const half_t *q) {  // 8 elements of K in two blocks of four rows
+    const uint2_t lo = read_column_of_four(q), hi = read_column_of_four(q + 4 * TILE);
+    return uint4_t{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto fragment_a = [&](int buf, int i, int kk) {
+    if constexpr (DOWN_A) return turned(&lds_a[buf][da[i] + kk * 32 * TILE]);
+    else return fragment(&lds_a[buf][fa0 + i * 16 * ROWH + ko[kk]]);
+  };
+  auto fragment_b = [&](int buf, int i, int kk) {
+    if constexpr (DOWN_B) return turned(&lds_b[buf][db[i] + kk * 32 * TILE]);
+    else return fragment(&lds_b[buf][fb0 + i * 16 * ROWH + ko[kk]]);
+  };
 
   // What is left of K behind the last whole step, zero-filled, through registers into the first buffers.  It comes first, so that
   // the accumulators run through the loop below and into the epilogue without a branch between them (with one, the compiler
@@ -104,15 +142,28 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
     const int left = (int)(p.K - k0);
 #pragma unroll
     for (int t = 0; t < TILE * CPR / 256; t++) {
-      const int row = (t * 256 + tid) / CPR, chunk = (t * 256 + tid) % CPR;
-      const unsigned ra = (unsigned)row < last_a ? (unsigned)row : last_a, rb = (unsigned)row < last_b ? (unsigned)row : last_b;
-      const int slot = row * ROWH + (chunk ^ ((row >> RS) & (CPR - 1))) * 8;
-      // K is a multiple of 8, so a chunk is there or is not; one that is not reads the first of the step instead
-      const bool there = chunk * 8 < left;
-      const size_t k = k0 + (there ? chunk * 8 : 0);
-      const uint4_t ca = *reinterpret_cast<const uint4_t *>(A + (ra * p.lda + k) * 2), cb = *reinterpret_cast<const uint4_t *>(B + (rb * p.ldb + k) * 2), none = {0u, 0u, 0u, 0u};
-      *reinterpret_cast<uint4_t *>(&lds_a[0][slot]) = there ? ca : none;
-      *reinterpret_cast<uint4_t *>(&lds_b[0][slot]) = there ? cb : none;
+      // along the rows, K is a multiple of 8 or its rows go on in zeros up to one, so a chunk is there or is not; one that is not
+      // reads the first of the step instead
+      auto move = [&](const char *from, size_t ld, unsigned last, bool down, half_t *to) {
+        const int at = t * 256 + tid, row = down ? at / (int)CHUNKS : at / CPR, place = down ? at % (int)CHUNKS : at % CPR;
+        const bool there = (down ? row : place * 8) < left;
+        size_t r, c;
+        int slot;
+        if (down) {
+          const unsigned column = unit_place<UNITS>(row, place / 2) * 16 + (place & 1) * 8;
+          r = k0 + (there ? row : 0);
+          c = column < last ? column : last;
+          slot = at * 8;
+        } else {
+          r = (unsigned)row < last ? (unsigned)row : last;
+          c = k0 + (there ? place * 8 : 0);
+          slot = row * ROWH + (place ^ ((row >> RS) & (CPR - 1))) * 8;
+        }
+        const uint4_t chunk = *reinterpret_cast<const uint4_t *>(from + (r * ld + c) * 2), none = {0u, 0u, 0u, 0u};
+        *reinterpret_cast<uint4_t *>(to + slot) = there ? chunk : none;
+      };
+      move(A, p.lda, last_a, DOWN_A, lds_a[0]);
+      move(B, p.ldb, last_b, DOWN_B, lds_b[0]);
     }
     __syncthreads();
 #pragma unroll
@@ -120,8 +171,8 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
       uint4_t fa[W8], fb[W8];
 #pragma unroll
       for (int i = 0; i < W8; i++) {
-        fa[i] = fragment(&lds_a[0][fa0 + i * 16 * ROWH + ko[kk]]);
-        fb[i] = fragment(&lds_b[0][fb0 + i * 16 * ROWH + ko[kk]]);
+        fa[i] = fragment_a(0, i, kk);
+        fb[i] = fragment_b(0, i, kk);
       }
 #pragma unroll
       for (int t = 0; t < NM; t++) acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[t % W8], fa[t / W8], acc[t / W8][t % W8]);
@@ -132,19 +183,26 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
     uint32_t off_a[TPW], off_b[TPW];
 #pragma unroll
     for (int t = 0; t < TPW; t++) {
-      const unsigned row = (unsigned)((wave * TPW + t) * RPT + lane / CPR);
-      const unsigned chunk = (unsigned)(lane % CPR) ^ ((row >> RS) & (CPR - 1));
-      const unsigned ra = row < last_a ? row : last_a, rb = row < last_b ? row : last_b;
-      off_a[t] = (uint32_t)((ra * p.lda + chunk * 8) * 2);
-      off_b[t] = (uint32_t)((rb * p.ldb + chunk * 8) * 2);
+      auto offset = [&](size_t ld, unsigned last, bool down) {
+        const unsigned at = (unsigned)((wave * TPW + t) * 64 + lane);
+        if (down) {
+          const unsigned row = at / CHUNKS, place = at % CHUNKS, column = unit_place<UNITS>(row, place / 2) * 16 + (place & 1) * 8;
+          return (uint32_t)((row * ld + (column < last ? column : last)) * 2);
+        }
+        const unsigned row = at / CPR, chunk = at % CPR ^ ((row >> RS) & (CPR - 1));
+        return (uint32_t)(((row < last ? row : last) * ld + chunk * 8) * 2);
+      };
+      off_a[t] = offset(p.lda, last_a, DOWN_A);
+      off_b[t] = offset(p.ldb, last_b, DOWN_B);
     }
-    constexpr lds_addr_t STAGE = OPH * 2, TBYTES = 1024, STEPB = BK * 2;
-    const char *ga = A + step0 * STEPB, *gb = B + step0 * STEPB;
+    constexpr lds_addr_t STAGE = OPH * 2, TBYTES = 1024;
+    const size_t step_a = BK * 2 * (DOWN_A ? p.lda : 1), step_b = BK * 2 * (DOWN_B ? p.ldb : 1);
+    const char *ga = A + step0 * step_a, *gb = B + step0 * step_b;
     const lds_addr_t ta = wave_uniform(lds_address_of(&lds_a[0][0]) + wave * TPW * TBYTES);
     const lds_addr_t tb = wave_uniform(lds_address_of(&lds_b[0][0]) + wave * TPW * TBYTES);
     // steps past the end: a harmless re-read of the last step into a free buffer
-    auto issue_a = [&](size_t step, int buf, int t) { load_chunk_to_lds(ga + (step < steps ? step : steps - 1) * STEPB, off_a[t], ta + buf * STAGE + t * TBYTES); };
-    auto issue_b = [&](size_t step, int buf, int t) { load_chunk_to_lds(gb + (step < steps ? step : steps - 1) * STEPB, off_b[t], tb + buf * STAGE + t * TBYTES); };
+    auto issue_a = [&](size_t step, int buf, int t) { load_chunk_to_lds(ga + (step < steps ? step : steps - 1) * step_a, off_a[t], ta + buf * STAGE + t * TBYTES); };
+    auto issue_b = [&](size_t step, int buf, int t) { load_chunk_to_lds(gb + (step < steps ? step : steps - 1) * step_b, off_b[t], tb + buf * STAGE + t * TBYTES); };
     // in flight at the first barrier: A0 B0 | A1 B1 (| A2 B2) (the wave's counter returns in issue order)
 #pragma unroll
     for (int d = 0; d < NB; d++) {
@@ -158,8 +216,8 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
     uint4_t fa[2][W8], fb[2][W8];
 #pragma unroll
     for (int i = 0; i < W8; i++) {
-      fa[0][i] = fragment(&lds_a[0][fa0 + i * 16 * ROWH + ko[0]]);
-      fb[0][i] = fragment(&lds_b[0][fb0 + i * 16 * ROWH + ko[0]]);
+      fa[0][i] = fragment_a(0, i, 0);
+      fb[0][i] = fragment_b(0, i, 0);
     }
     int ca = 0, cb = 0;  // s % NA, s % NB
     for (size_t s = 0; s < steps; s++) {
@@ -171,9 +229,9 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
       for (int t = 0; t < NM; t++) {
         if (t < 4 * W8 && t % 2 == 0) {
           const int k = t / 2;
-          if (k == 0) fa[1][0] = fragment(&lds_a[ca][fa0 + ko[1]]);
-          else if (k <= W8) fb[1][k - 1] = fragment(&lds_b[cb][fb0 + (k - 1) * 16 * ROWH + ko[1]]);
-          else fa[1][k - W8] = fragment(&lds_a[ca][fa0 + (k - W8) * 16 * ROWH + ko[1]]);
+          if (k == 0) fa[1][0] = fragment_a(ca, 0, 1);
+          else if (k <= W8) fb[1][k - 1] = fragment_b(cb, k - 1, 1);
+          else fa[1][k - W8] = fragment_a(ca, k - W8, 1);
         }
         if (NB == 2 && t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_a(s + 2, fill_a, (t - NM / 2) / TEVERY);
         acc[t / W8][t % W8] = mfma_16x16x32_chunks<BF16>(fb[0][t % W8], fa[0][t / W8], acc[t / W8][t % W8]);
@@ -188,9 +246,9 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
       for (int t = 0; t < NM; t++) {
         if (t < 4 * W8 && t % 2 == 0) {
           const int k = t / 2;
-          if (k == 0) fa[0][0] = fragment(&lds_a[na][fa0 + ko[0]]);
-          else if (k <= W8) fb[0][k - 1] = fragment(&lds_b[nb][fb0 + (k - 1) * 16 * ROWH + ko[0]]);
-          else fa[0][k - W8] = fragment(&lds_a[na][fa0 + (k - W8) * 16 * ROWH + ko[0]]);
+          if (k == 0) fa[0][0] = fragment_a(na, 0, 0);
+          else if (k <= W8) fb[0][k - 1] = fragment_b(nb, k - 1, 0);
+          else fa[0][k - W8] = fragment_a(na, k - W8, 0);
         }
         if (NB == 2 && t >= NM / 2 && (t - NM / 2) % TEVERY == 0) issue_b(s + 2, cb, (t - NM / 2) / TEVERY);
         if (NB == 3 && t % TEVERY == 0) {  // the buffers of step s are free behind the barrier
@@ -254,15 +312,16 @@ TCU_DEVICE void fused_gemm_tile(const FusedGemmParams &p, size_t tile_m, size_t 
   });
 }
 
-// K is at least 64 and a multiple of 8, and each split has a whole step at least.  TAIL: K is no multiple of 64.
-template <int DT, bool WHOLE, int W8, bool TAIL>
+// K is at least 64, and each split has a whole step at least.  TAIL: K may be no multiple of 64.  (Where K runs down the rows of B the
+// kernels all have the tail's code: without it the compiler copies the accumulators of 256 x 256 tiles every step, 3 times slower.)
+template <int DT, bool WHOLE, int W8, bool TAIL, int LAYOUT = kAlong>
 __global__ __launch_bounds__(256, W8 == 4 ? 2 : 1) void fused_gemm_tile_kernel(FusedGemmParams p) {
   constexpr int TILE = 32 * W8;
   const unsigned split = blockIdx.x / p.tiles, tile = blockIdx.x % p.tiles;
   size_t tile_m, tile_n;
   gemm_tile_of_block((p.M + TILE - 1) / TILE, (p.N + TILE - 1) / TILE, tile, &tile_m, &tile_n);
   const size_t full = p.K / 64, step0 = split * full / p.splits, end = (split + 1) * full / p.splits;
-  fused_gemm_tile<DT, WHOLE, W8, TAIL>(p, tile_m, tile_n, step0, end - step0, split + 1 == p.splits, p.shares ? p.shares + (size_t)split * p.M * p.share_ld : nullptr);
+  fused_gemm_tile<DT, WHOLE, W8, TAIL, LAYOUT>(p, tile_m, tile_n, step0, end - step0, split + 1 == p.splits && p.K % 64 != 0, p.shares ? p.shares + (size_t)split * p.M * p.share_ld : nullptr);
 }
 
 // The epilogue over the sum of the shares, one thread per 8 adjacent columns, the shares in order.
@@ -440,7 +499,8 @@ TCU_DEVICE void transpose_tile(const TransposeParams &p, const TransposeJob &j, 
   }
 }
 
-// All that the gradient's products need laid out anew, in one launch (4001 x 4096 x 2056 bf16: three launches 27 + 10 + 10 us).
+// All that the gradient's products need laid out anew, in one launch (three transposes of 4001 x 4096 x 2056 bf16 one by one 27 + 10 + 10 us,
+// together 38).
 template <int DT>
 __global__ __launch_bounds__(256) void gradient_layout_kernel(TransposeParams p) {
   __shared__ __attribute__((aligned(16))) uint16_t lds[64 * 66];

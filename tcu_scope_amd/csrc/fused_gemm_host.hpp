@@ -26,15 +26,17 @@ struct GemmPlan {
   bool few_rows = false;
   int few_tiles = 1;  // few rows: 16-row tiles
   int w8 = 8;         // block tiles of 32 w8 rows and columns
+  int layout = kAlong;
   size_t tiles = 0, splits = 1;
   size_t share_ld = 0, share_bytes = 0;
 };
 // The time of a tiling in microseconds: rounds of blocks over the compute units, each as long as its K steps (64 elements)
 // plus what a block spends before and after them, and the pass that joins split sums.  Measured with 8192 x 8192 x 4096 and
 // 4001 x 2056 x 4096 bf16: a step of a 256 x 256 tile takes a compute unit 1.5 us, of 192 x 192 0.9, and of two 128 x 128
-// tiles side by side 0.95.
+// tiles side by side 0.95; and with few steps, i.e. mostly what stands around them: 256 | 192 | 128 tiles 7616 x 4120 x 130 40 | 52 | 34 us,
+// 8192 x 8192 x 200 79 | 107 | 71, 4032 x 3112 x 283 24 | 30 | 22.
 inline double gemm_tiling_us(size_t tiles, size_t splits, int w8, size_t M, size_t N, size_t K) {
-  const double step = w8 == 8 ? 1.5 : w8 == 6 ? 0.9 : 0.95, around = w8 == 8 ? 12.0 : w8 == 6 ? 8.0 : 6.0;
+  const double step = w8 == 8 ? 1.5 : w8 == 6 ? 0.9 : 0.95, around = w8 == 8 ? 15.0 : w8 == 6 ? 10.0 : 5.5;
   const size_t at_once = w8 == 4 ? 512 : 256, blocks = tiles * splits;
   const double steps = (double)((K + 63) / 64 + splits - 1) / (double)splits;
   const double alone = w8 == 4 && blocks <= 256 ? 0.65 : 1.0;  // a 128 x 128 tile that has its compute unit to itself
@@ -42,10 +44,11 @@ inline double gemm_tiling_us(size_t tiles, size_t splits, int w8, size_t M, size
   if (splits > 1) us += 5.0 + (double)splits * (double)M * (double)N * 8.0 / 4.0e6;
   return us;
 }
-inline GemmPlan plan_gemm(size_t M, size_t N, size_t K) {
+inline GemmPlan plan_gemm(size_t M, size_t N, size_t K, int layout = kAlong) {
   GemmPlan g;
+  g.layout = layout;
   g.share_ld = up_to(N, 8);
-  if (M <= kGemmFewRows) {
+  if (M <= kGemmFewRows && layout == kAlong) {
     g.few_rows = true;
     g.few_tiles = M <= 16 ? 1 : 2;
     g.tiles = (N + 15) / 16;
@@ -87,10 +90,13 @@ inline void launch_gemm(const GemmPlan &g, FusedGemmParams p, float *shares, boo
     else TCU_FEW(2, 4);
 #undef TCU_FEW
   } else {
-#define TCU_TILES(W8) (p.K % 64 ? launch(fused_gemm_tile_kernel<DT, WHOLE, W8, true>, grid, 256u, stream, p) : launch(fused_gemm_tile_kernel<DT, WHOLE, W8, false>, grid, 256u, stream, p))
-    if (g.w8 == 8) TCU_TILES(8);
-    else if (g.w8 == 6) TCU_TILES(6);
-    else TCU_TILES(4);
+#define TCU_TILE(W8, TAIL, LAYOUT) launch(fused_gemm_tile_kernel<DT, WHOLE || LAYOUT != kAlong, W8, TAIL, LAYOUT>, grid, 256u, stream, p)
+#define TCU_TILES(TAIL, LAYOUT) (g.w8 == 8 ? TCU_TILE(8, TAIL, LAYOUT) : g.w8 == 6 ? TCU_TILE(6, TAIL, LAYOUT) : TCU_TILE(4, TAIL, LAYOUT))
+    if (g.layout == kDownB) TCU_TILES(true, kDownB);  // taken for whole chunks only
+    else if (g.layout == kDownBoth) TCU_TILES(true, kDownBoth);
+    else if (p.K % 64) TCU_TILES(true, kAlong);
+    else TCU_TILES(false, kAlong);
+#undef TCU_TILE
 #undef TCU_TILES
   }
   if (p.splits != 1) launch(fused_gemm_join_kernel<DT, WHOLE>, (unsigned)((p.M * (g.share_ld / 8) + 255) / 256), 256u, stream, p);
@@ -208,10 +214,15 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   if (act && !Z) return report_failure(TCU_ERR_INVALID_ARG, w + ": the gradient of an activation needs d_Z");
   // the copies' rows end in zeros up to a whole step of the tile kernels
   const size_t ldm = up_to(M, 64), ldn = up_to(N, 64);
-  const GemmPlan ga = plan_gemm(M, K, N), gb = plan_gemm(N, K, M);
+  // the operands along whose rows the sums do not run, as they are: whole chunks, and a whole step of rows at least
+  // (up to 32 rows the few-row kernel on a turned B is faster: 8 x 4096 x 4096 bf16 45 us, 51 with B as it is)
+  const bool down_a = dA && M > kGemmFewRows && N >= 64 && K % 8 == 0 && rows_ready(B, ldb) && rows_ready(dA, M > 1 ? ldda : 8);
+  const bool down_b = dB && M >= 64 && K % 8 == 0 && rows_ready(A, lda) && rows_ready(dB, N > 1 ? lddb : 8);
+  const GemmPlan ga = plan_gemm(M, K, N, down_a ? kDownB : kAlong), gb = plan_gemm(N, K, M, down_b ? kDownBoth : kAlong);
   // the gradient of the activation's argument: dD itself where there is no activation and its rows are ready
-  const bool own_dz = dA && (act || N % 64 != 0 || !rows_ready(dD, M > 1 ? lddd : 8));
-  const size_t dz_bytes = own_dz ? part_bytes(M * ldn * 2) : 0, dzt_bytes = dB ? part_bytes(N * ldm * 2) : 0, at_bytes = dB ? part_bytes(K * ldm * 2) : 0, bt_bytes = dA ? part_bytes(K * ldn * 2) : 0;
+  const bool own_dz = (dA || down_b) && (act || N % (dA && !down_a ? 64 : 8) != 0 || !rows_ready(dD, M > 1 ? lddd : 8));
+  const bool turn_a = dB && !down_b, turn_b = dA && !down_a;  // A and dZ; B
+  const size_t dz_bytes = own_dz ? part_bytes(M * ldn * 2) : 0, dzt_bytes = turn_a ? part_bytes(N * ldm * 2) : 0, at_bytes = turn_a ? part_bytes(K * ldm * 2) : 0, bt_bytes = turn_b ? part_bytes(K * ldn * 2) : 0;
   const size_t strips = (M + 63) / 64, sums_bytes = dbias ? part_bytes(strips * N * 4) : 0;
   const size_t share_bytes = (dA ? ga.share_bytes : 0) > (dB ? gb.share_bytes : 0) ? ga.share_bytes : (dB ? gb.share_bytes : 0);
   const size_t bytes = share_bytes + dz_bytes + dzt_bytes + at_bytes + bt_bytes + sums_bytes, need = smallest_workspace(bytes);
@@ -251,9 +262,9 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
     const unsigned column_tiles = (unsigned)((columns + 63) / 64);
     q.job[i] = TransposeJob{from, to, rows, columns, from_ld, to_ld, column_tiles, (unsigned)((rows + 63) / 64 * column_tiles)};
   };
-  if (M && N && (own_dz || dB || dbias)) job(0, dD, lddd, dB ? dzt : nullptr, ldm, M, N);
-  if (dB && M && K) job(1, A, lda, a_t, ldm, M, K);
-  if (dA && N && K) job(2, B, ldb, b_t, ldn, N, K);
+  if (M && N && (own_dz || turn_a || dbias)) job(0, dD, lddd, turn_a ? dzt : nullptr, ldm, M, N);
+  if (turn_a && M && K) job(1, A, lda, a_t, ldm, M, K);
+  if (turn_b && N && K) job(2, B, ldb, b_t, ldn, N, K);
   q.Z = act ? Z : nullptr;
   q.z_ld = ldz;
   q.dz = own_dz ? dz : nullptr;
@@ -279,23 +290,23 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   if (dA && M && K) {
     p.A = own_dz ? dz : dD;
     p.lda = own_dz ? ldn : lddd;
-    p.B = b_t;
-    p.ldb = ldn;
+    p.B = down_a ? B : b_t;
+    p.ldb = down_a ? ldb : ldn;
     p.D = dA;
     p.ldd = ldda;
     p.M = M;
-    p.K = ldn;
+    p.K = down_a ? N : ldn;
     run_gemm(s->dtype, whole_a, ga, p, shares, true, stream);
   }
   if (dB && N && K) {
-    p.A = dzt;
-    p.lda = ldm;
-    p.B = a_t;
-    p.ldb = ldm;
+    p.A = !down_b ? dzt : own_dz ? dz : dD;
+    p.lda = !down_b ? ldm : own_dz ? ldn : lddd;
+    p.B = down_b ? A : a_t;
+    p.ldb = down_b ? lda : ldm;
     p.D = dB;
     p.ldd = lddb;
     p.M = N;
-    p.K = ldm;
+    p.K = down_b ? M : ldm;
     run_gemm(s->dtype, whole_b, gb, p, shares, true, stream);
   }
   return TCU_OK;

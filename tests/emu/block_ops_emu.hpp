@@ -36,6 +36,18 @@ inline uint16_t bf16_bits(float v) {
 }
 inline unsigned pack_bf16x2(float lo, float hi) { return (unsigned)bf16_bits(lo) | ((unsigned)bf16_bits(hi) << 16); }
 
+inline uint2_t read_column_of_four(const half_t *q) {
+  auto &w = my_wave();
+  const int lane = lane_id();
+  memcpy(&w.slot[lane][0], q, 8);
+  emu::wave_sync();
+  uint16_t column[4];
+  for (int r = 0; r < 4; r++) memcpy(&column[r], reinterpret_cast<const char *>(&w.slot[(lane & 48) + 4 * r + (lane & 15) / 4][0]) + 2 * (lane & 3), 2);
+  emu::wave_sync();
+  uint2_t got;
+  memcpy(&got, column, 8);
+  return got;
+}
 template <bool BF16>
 inline float4_t mfma_16x16x32_chunks(uint4_t a, uint4_t b, float4_t c) {
   auto &w = my_wave();

@@ -67,9 +67,27 @@ void emu_tiles(tcu::FusedGemmParams p) {
   else tcu::launch(tcu::fused_gemm_tile_kernel<DT, false, W8, false>, p.tiles * p.splits, 256u, nullptr, p);
   if (p.splits > 1) tcu::launch(tcu::fused_gemm_join_kernel<DT, false>, (unsigned)((p.M * (p.share_ld / 8) + 255) / 256), 256u, nullptr, p);
 }
+template <int DT, int W8, int LAYOUT>
+void emu_down(tcu::FusedGemmParams p) {
+  const size_t tile = 32 * W8;
+  p.tiles = (unsigned)((p.M + tile - 1) / tile * ((p.N + tile - 1) / tile));
+  tcu::launch(tcu::fused_gemm_tile_kernel<DT, true, W8, true, LAYOUT>, p.tiles * p.splits, 256u, nullptr, p);
+  if (p.splits > 1) tcu::launch(tcu::fused_gemm_join_kernel<DT, true>, (unsigned)((p.M * (p.share_ld / 8) + 255) / 256), 256u, nullptr, p);
+}
 }  // namespace
 
 extern "C" {
+// the same with K down the rows of B (layout 1) or of both operands (2)
+int emu_fused_gemm_down(int w8, int layout, unsigned splits, int dtype, size_t M, size_t N, size_t K, const void *A, size_t lda, const void *B, size_t ldb, void *D, size_t ldd, float *shares) {
+  tcu::FusedGemmParams p{};
+  p.A = A; p.lda = lda; p.B = B; p.ldb = ldb; p.D = D; p.ldd = ldd; p.M = M; p.N = N; p.K = K; p.splits = splits; p.share_ld = tcu::up_to(N, 8);
+  p.shares = splits > 1 ? shares : nullptr;
+#define EMU_DOWN(DT, W8) (layout == 1 ? emu_down<DT, W8, tcu::kDownB>(p) : emu_down<DT, W8, tcu::kDownBoth>(p))
+  if (dtype == TCU_F16) w8 == 8 ? EMU_DOWN(tcu::kF16, 8) : w8 == 6 ? EMU_DOWN(tcu::kF16, 6) : EMU_DOWN(tcu::kF16, 4);
+  else w8 == 8 ? EMU_DOWN(tcu::kBF16, 8) : w8 == 6 ? EMU_DOWN(tcu::kBF16, 6) : EMU_DOWN(tcu::kBF16, 4);
+#undef EMU_DOWN
+  return 0;
+}
 // the tile kernels at sizes at which the library would not take them; rows of A and B begin on 16 bytes, K is at least 64 for every split
 int emu_fused_gemm_tiles(int w8, unsigned splits, int dtype, int act, size_t M, size_t N, size_t K, float beta, const void *A, size_t lda, const void *B, size_t ldb, const void *bias, const void *C, size_t ldc,
                          void *D, size_t ldd, void *Z, size_t ldz, float *shares) {

@@ -618,6 +618,7 @@ def gemm_emu(emu):
     emu.emu_fused_gemm.argtypes = [shape, *m * 2, vp, *m * 3, vp, psz]
     emu.emu_fused_gemm_backward.argtypes = [shape, *m * 6, vp, vp, psz]
     emu.emu_fused_gemm_tiles.argtypes = [ci, ctypes.c_uint, ci, ci, sz, sz, sz, cf, *m * 2, vp, *m * 3, vp]
+    emu.emu_fused_gemm_down.argtypes = [ci, ci, ctypes.c_uint, ci, sz, sz, sz, *m * 3, vp]
     return emu
 
 
@@ -689,7 +690,27 @@ def test_fused_gemm_tiles(emu, dtype, w8, splits, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("M,N,K,gap,name", [(1, 1, 1, 0, "silu"), (70, 100, 72, 0, "silu"), (130, 8, 65, 1, "gelu"), (9, 67, 130, 0, "none"), (100, 16, 24, 3, "none"), (40, 80, 16, 8, "sigmoid"), (0, 5, 9, 0, "relu"), (66, 70, 68, 0, "relu"), (70, 0, 72, 0, "none"), (3, 0, 8, 0, "none")])
+@pytest.mark.parametrize("layout", [1, 2])
+@pytest.mark.parametrize("w8,splits,M,N,K", [(4, 1, 130, 248, 131), (4, 3, 33, 104, 328), (8, 1, 301, 264, 207), (8, 2, 40, 256, 192), (6, 1, 200, 200, 151), (6, 2, 192, 384, 256)])
+def test_fused_gemm_tiles_down_the_rows(emu, dtype, layout, w8, splits, M, N, K):
+    """Operands whose K runs down their rows: parts of a step, of a chunk of columns, and rows further apart than they are long.  What the padding
+    of a row holds beyond the operand must not be used."""
+    emu = gemm_emu(emu)
+    rng = np.random.default_rng(M + layout)
+    A, B, _, _ = gemm_operands(rng, dtype, M, N, K, False, False)
+    up = lambda n: (n + 7) // 8 * 8
+    wide = lambda m: np.concatenate([m, np.zeros((m.shape[0], up(m.shape[1]) - m.shape[1]))], 1)
+    mA = Matrix(wide(A.T if layout == 2 else A), dtype)
+    mB, mD = Matrix(B.T, dtype, N + 16), Matrix(np.zeros((M, N)), dtype, N + 8)
+    shares = floats(np.full(splits * M * N, np.nan))
+    emu.emu_fused_gemm_down(w8, layout, splits, DTYPES[dtype], M, N, K, *operand(mA), *operand(mB), *operand(mD), shares.ctypes.data)
+    d, _, ed, _ = ref.product(A, B, np.zeros(N), "none", None, 0.0)
+    ref.check(mD.get(), d, ed, dtype, "D")
+    assert mD.untouched_between()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,N,K,gap,name", [(1, 1, 1, 0, "silu"), (70, 100, 72, 0, "silu"), (130, 8, 65, 1, "gelu"), (9, 67, 130, 0, "none"), (100, 16, 24, 3, "none"), (40, 80, 16, 8, "sigmoid"), (0, 5, 9, 0, "relu"), (66, 70, 68, 0, "relu"), (150, 67, 136, 8, "silu"), (65, 144, 72, 0, "none"), (20, 200, 64, 0, "none"), (130, 24, 80, 8, "none"), (70, 0, 72, 0, "none"), (3, 0, 8, 0, "none")])
 def test_fused_gemm_gradient(emu, dtype, M, N, K, gap, name):
     emu = gemm_emu(emu)
     rng = np.random.default_rng(M + N)
