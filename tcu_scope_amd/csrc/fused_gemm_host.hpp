@@ -215,8 +215,9 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   // the copies' rows end in zeros up to a whole step of the tile kernels
   const size_t ldm = up_to(M, 64), ldn = up_to(N, 64);
   // the operands along whose rows the sums do not run, as they are: whole chunks, and a whole step of rows at least
-  // (up to 32 rows the few-row kernel on a turned B is faster: 8 x 4096 x 4096 bf16 45 us, 51 with B as it is)
-  const bool down_a = dA && M > kGemmFewRows && N >= 64 && K % 8 == 0 && rows_ready(B, ldb) && rows_ready(dA, M > 1 ? ldda : 8);
+  // (also where M is small enough for the few-row kernel, which would need B turned: 20 x 8192 x 8192 bf16 83 us, turned 149;
+  // 8 x 4096 x 4096 39 | 37)
+  const bool down_a = dA && N >= 64 && K % 8 == 0 && rows_ready(B, ldb) && rows_ready(dA, M > 1 ? ldda : 8);
   const bool down_b = dB && M >= 64 && K % 8 == 0 && rows_ready(A, lda) && rows_ready(dB, N > 1 ? lddb : 8);
   const GemmPlan ga = plan_gemm(M, K, N, down_a ? kDownB : kAlong), gb = plan_gemm(N, K, M, down_b ? kDownBoth : kAlong);
   // the gradient of the activation's argument: dD itself where there is no activation and its rows are ready

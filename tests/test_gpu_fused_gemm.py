@@ -44,7 +44,8 @@ def test_product(tcu, dtype, M, N, K, stride, name):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("M,N,K,stride,name", [(1, 1, 1, None, "silu"), (200, 520, 264, None, "silu"), (333, 77, 129, None, "gelu"), (64, 2048, 512, None, "none"), (1000, 96, 40, 48, "none"), (2100, 600, 4097, None, "relu"), (4111, 512, 64, None, "sigmoid")])
+@pytest.mark.parametrize("M,N,K,stride,name", [(1, 1, 1, None, "silu"), (200, 520, 264, None, "silu"), (333, 77, 129, None, "gelu"), (64, 2048, 512, None, "none"), (1000, 96, 40, 48, "none"), (2100, 600, 4097, None, "relu"), (4111, 512, 64, None, "sigmoid"), (31, 700, 1032, None, "gelu"), (130, 2120, 1064, 1072, "none"),
+                                               (1100, 4096, 4096, 4104, "silu")])
 def test_gradient(tcu, dtype, M, N, K, stride, name):
     import torch
 
