@@ -77,9 +77,11 @@ extern "C" {
  *                     kernel (and of the look-back path of tcu_seg_scan_f16 for segments of 2^21 halves and more)
  *                     looks again for a value another block has not published yet before it gives up.  Giving up
  *                     never yields a finite wrong number: the reduction's result, or the scan's outputs from the
- *                     waiting partition to the end of the array (or segment), become NaN
+ *                     waiting partition to the end of the array (or segment), become NaN.  Also of tcu_gated_scan and its
+ *                     gradient, whose waiting tiles leave NaN to the end of their sequences
  *   "test_mute_partition"  default 0; p > 0: partition p - 1 of those kernels publishes nothing, so every wait
- *                     for it expires (for tests of the rule above; all kernels still run to their end)
+ *                     for it expires (for tests of the rule above; all kernels still run to their end); of the gated
+ *                     scan: tile p - 1
  * Unknown names return TCU_ERR_INVALID_ARG. */
 int tcu_set_option(const char *name, int value);
 
