@@ -505,7 +505,7 @@ __global__ __launch_bounds__(THREADS) void gated_scan_kernel(GatedScanParams p) 
 }
 
 // Ahead of the scan: clears the ticket and the entries, finds every row's sequence from the offsets (rows of no
-// sequence get -1), and hands the seed of each empty sequence on as the state behind it.
+// sequence get -1), and hands the seed of each sequence without rows on as the state behind it.
 struct GatedScanSetup {
   unsigned *head;          // 64 words: ticket, expired waits
   uint4_t *clear;          // entries
@@ -537,7 +537,10 @@ __global__ __launch_bounds__(256) inline void gated_scan_setup_kernel(GatedScanS
   if (s.last && (s.offsets || s.rows == 0)) {
     // one block per sequence and round: most have tokens and are passed over after two reads
     for (unsigned j = blockIdx.x; j < s.sequences; j += gridDim.x) {
-      if (s.rows != 0 && offset_at(s, j + 1) > offset_at(s, j)) continue;
+      if (s.rows != 0) {
+        const long long from = offset_at(s, j), to = offset_at(s, j + 1);
+        if ((from > 0 ? from : 0) < (to < (long long)s.rows ? to : (long long)s.rows)) continue;  // it has rows that exist
+      }
       for (unsigned c = threadIdx.x; c < s.channels; c += blockDim.x) s.last[(size_t)j * s.channels + c] = s.seed ? s.seed[(size_t)j * s.channels + c] : 0.0f;
     }
   }

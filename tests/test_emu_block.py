@@ -233,6 +233,21 @@ def test_rows_without_any_sequence(emu, zero_outside):
         assert (m.get() == (0.0 if zero_outside else 5.0)).all()
 
 
+def test_offsets_that_pass_the_rows(emu):
+    """Only rows that exist count: a sequence that ends behind the last one stops there, one that begins there (or ends in front of the first) has none."""
+    rng = np.random.default_rng(12)
+    rows, channels, offsets = 20, 12, [-7, -3, 9, 26, 40]
+    x, g, _ = scan_case(rng, "f32", "sigmoid", [0, rows], rows, channels)
+    h0 = rng.standard_normal((4, channels)).astype(np.float32).astype(np.float64)
+    s, keep = shape_of("f32", "sigmoid", rows, channels, offsets, 64)
+    mx, mg, mh = Matrix(x, "f32"), Matrix(g, "f32"), Matrix(x, "f32")
+    f0, last = floats(h0), floats(np.full(h0.shape, 9.0))
+    assert run_scan(emu, s, mx, mg, mh, f0.ctypes.data, last.ctypes.data) == 0
+    h, want, e, elast = ref.scan("sigmoid", x, g, [0, 0, 9, rows, rows], h0)
+    ref.check(mh.get(), h, e, "f32", "h")
+    ref.check(last.reshape(h0.shape), want, elast, "f32", "h_last")
+
+
 def test_states_do_not_pass_between_sequences(emu):
     """An infinite or NaN state stays in its sequence: a sequence's beginning replaces what came before, it does not multiply it by 0."""
     rows, channels = 400, 8
