@@ -372,7 +372,8 @@ int tcu_fused_gemm(const tcu_fused_gemm_shape *shape, const void *d_A, size_t ld
 
 /* The gradient: with dZ = dD act'(Z) (TCU_ACT_NONE: dD, and d_Z is not read), dA = dZ B^T (M x K), dB (N rows of K) = dZ^T A and
  * dbias (N fp32 values) = the sums of dZ over its rows, those that are not NULL; the gradient of C is beta dD.  shape->beta is
- * not used.  dZ is rounded to the operands' type in front of the products, not of its sums.  M, N and K up to 2^22. */
+ * not used.  dZ is rounded to the operands' type in front of the products, not of its sums.  M, N and K up to 2^22.  The size
+ * query goes by the same arguments as the call: operands and gradients whose rows are no whole 16-byte chunks take more. */
 int tcu_fused_gemm_backward(const tcu_fused_gemm_shape *shape, const void *d_dD, size_t lddd, const void *d_A, size_t lda, const void *d_B, size_t ldb, const void *d_Z, size_t ldz, void *d_dA, size_t ldda, void *d_dB, size_t lddb, float *d_dbias, void *d_workspace, size_t *workspace_bytes, void *stream);
 
 /* ---- fills, conversions, inputs ---------------------------------------------------------------- */

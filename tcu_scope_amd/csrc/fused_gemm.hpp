@@ -12,7 +12,7 @@
 //                they fit), the loop of gemm_dlds_a3b2_m16_kernel.  M and N may be anything (rows beyond the last one are read
 //                as the last one and not stored), K a multiple of 8 (a step with what is left of K goes through registers,
 //                zero-filled; operands of another K are copied to padded rows first).
-//                Bound by the matrix unit: 8192 x 8192 x 4096 bf16 with bias, silu and Z 443 us = 1.24 PFLOP/s.
+//                Bound by the matrix unit: 8192 x 8192 x 4096 bf16 with bias, silu and Z 431 us = 1.28 PFLOP/s.
 //                Where the tiles are fewer than the compute units, several blocks share a tile's K steps and
 //                fused_gemm_join_kernel adds their fp32 shares in a fixed order.
 //   fused_gemm_few_rows_kernel : up to 32 rows.  Bound by reading B once: a block takes 16 columns of the output and all rows,

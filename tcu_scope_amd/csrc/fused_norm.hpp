@@ -17,7 +17,7 @@
 // of the vectors are sums over rows: a block walks many rows with its columns' sums in registers, writes them once as
 // partial sums, and a second launch adds the partial sums of each column in a fixed order (no atomics: the same input
 // gives the same bits).  16384 x 4096 bf16 with residual 89 us (537 MB, 6.0 TB/s, part of it served by the last-level cache), the
-// gradient of the gated layer form with 8192 x 4096 77 us + 4.7 for the partial sums (336 MB, 4.1 TB/s: every row passes through
+// gradient of the gated layer form with 8192 x 4096 79 us + 4.7 for the partial sums (336 MB, 4.1 TB/s: every row passes through
 // two reductions over its 8 waves), 12 x 2048 fp16 3.8 us.
 #pragma once
 
