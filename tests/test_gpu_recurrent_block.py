@@ -127,3 +127,28 @@ def test_block_in_a_graph(tcu):
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(held, eager))
+
+
+def test_two_streams_at_once(tcu):
+    """Blocks on two streams that run side by side get what each gets alone, to the bit: no call keeps anything where another finds it."""
+    import torch
+
+    sets = [(make(torch.bfloat16, B, T, D, E), E) for B, T, D, E in ((2, 1500, 256, 320), (3, 900, 256, 264))]
+
+    def step(p, E):
+        out, (n1, s1, proj, h, y) = forward(tcu, p, E, lambda v, g: tcu.gated_scan(v, g)[0])
+        g_out = tcu.fused_gemm_backward(out, y, p["w_out"])
+        g_n2 = tcu.fused_norm_backward(g_out["dA"], h, p["w2"], gate=proj[..., 2 * E:], norm="layer")
+        return [out, *g_out.values(), *g_n2.values(), *tcu.gated_scan_backward(g_n2["dx"], proj[..., :E], proj[..., E:2 * E], h)]
+
+    alone = [step(*a) for a in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, (a, s) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(step(*a))
+    torch.cuda.synchronize()
+    for want, runs in zip(alone, got):
+        assert all(torch.equal(a, b) for r in runs for a, b in zip(r, want))
