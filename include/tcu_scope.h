@@ -310,6 +310,9 @@ typedef struct {
 
 /* d_h = the states after every row, d_h_last (num_sequences x channels fp32, may be NULL) = the state behind each sequence
  * (behind an empty one: its d_h0, or 0).  d_h0: num_sequences x channels fp32.  d_h may be d_x or d_g (same stride).
+ * Products of a along up to 2048 rows are formed in fp32.  Where |a| is above 1 one may pass 2^128: a state of zero in front of it
+ * still gives what the recurrence says, any other becomes an infinity or a NaN (also one so small that the recurrence would
+ * stay finite).  Products below 2^-126 count as 0.
  * Bit-reproducible.  A wait of one tile for another that expires ("lookback_poll_limit") leaves NaN from there to the end
  * of the sequence, and word 1 of the workspace, where offsets are given or the rows take several tiles, counts it. */
 int tcu_gated_scan(const tcu_gated_scan_shape *shape, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, void *d_h, size_t h_stride, const float *d_h0, float *d_h_last, void *d_workspace, size_t *workspace_bytes, void *stream);
