@@ -311,7 +311,7 @@ def seg_scan_by_key(keys, x, out=None, workspace=None, stream=None):
     _check(lib().tcu_seg_scan_by_key_f16(None, None, None, n, bits, None, ctypes.byref(need), None))
     if workspace is None:
         workspace = torch.empty(max(need.value, 256), dtype=torch.uint8, device=x.device)
-    have = ctypes.c_size_t(workspace.numel())
+    have = ctypes.c_size_t(_workspace_bytes(workspace, x.device, need.value))
     _check(lib().tcu_seg_scan_by_key_f16(_ptr(keys), _ptr(x), _ptr(out), n, bits, _ptr(workspace), ctypes.byref(have), _stream(stream)))
     return out
 
@@ -332,9 +332,20 @@ def seg_reduce_by_key(keys, x, workspace=None, stream=None):
     _check(lib().tcu_seg_reduce_by_key_f16(None, None, None, None, None, n, bits, None, ctypes.byref(need), None))
     if workspace is None:
         workspace = torch.empty(max(need.value, 256), dtype=torch.uint8, device=x.device)
-    have = ctypes.c_size_t(workspace.numel())
+    have = ctypes.c_size_t(_workspace_bytes(workspace, x.device, need.value))
     _check(lib().tcu_seg_reduce_by_key_f16(_ptr(keys), _ptr(x), _ptr(keys_out), _ptr(out), _ptr(num_runs), n, bits, _ptr(workspace), ctypes.byref(have), _stream(stream)))
     return keys_out, out, num_runs
+
+
+def _workspace_bytes(workspace, device, need):
+    """Bytes of a workspace the caller gives.  An empty tensor has a null pointer, which the library takes as a question for the size: the
+    call would return without having computed anything."""
+    if workspace.device != device or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be a contiguous tensor on {device}")
+    have = workspace.numel() * workspace.element_size()
+    if have == 0 and need > 0:
+        raise ValueError(f"workspace is empty; the call needs {need} bytes at least")
+    return have
 
 
 def add_partial_sums(out, partial_sums, segment_size, stream=None):
@@ -350,7 +361,7 @@ def _workspace(fn, x, out, n, strategy, segment_size, waves_per_block, workspace
     _check(fn(_ptr(x), None, n, None, ctypes.byref(need), int(strategy), segment_size, waves_per_block, _stream(stream)))
     if workspace is None:
         workspace = torch.empty(max(need.value, 256), dtype=torch.uint8, device=x.device)
-    have = ctypes.c_size_t(workspace.numel() * workspace.element_size())
+    have = ctypes.c_size_t(_workspace_bytes(workspace, x.device, need.value))
     _check(fn(_ptr(x), _ptr(out), n, _ptr(workspace), ctypes.byref(have), int(strategy), segment_size, waves_per_block, _stream(stream)))
     return workspace
 
@@ -586,9 +597,7 @@ _workspace_sizes = {}
 def _call_with_workspace(fn, args, sizes, workspace, device, raw):
     """fn(*args, workspace, its size, stream) with the caller's workspace, or a new one of the size the call needs."""
     if workspace is not None:
-        if workspace.device != device or not workspace.is_contiguous():
-            raise ValueError(f"workspace must be a contiguous tensor on {device}")
-        have = ctypes.c_size_t(workspace.numel() * workspace.element_size())
+        have = ctypes.c_size_t(_workspace_bytes(workspace, device, 256))
         _check(fn(*args, workspace.data_ptr(), ctypes.byref(have), raw))
         return
     torch = _torch()
