@@ -760,13 +760,13 @@ def fused_norm(x, weight=None, bias=None, residual=None, gate=None, scale=1.0, c
 
 
 @_launches
-def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, channel_scale=None, x=None, dresidual_out=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, workspace=None, *, stream=None):
+def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, channel_scale=None, x=None, dresidual_out=None, norm=Norm.RMS, order=NormOrder.ADD_NORM, activation=None, eps=1e-6, workspace=None, residual_gradient=None, *, stream=None):
     """The gradient of fused_norm (tcu_fused_norm_backward): a dict with "dx" and, where the operand is there, "dgate",
     "dweight", "dbias", "dscale" (of channel_scale) and "dresidual".
 
     z: what was normed: the residual_out of the forward call (order add_norm with a residual), else its x.  order add_norm:
-    dresidual_out is the gradient with respect to residual_out and "dresidual" is returned if it is given; the gradient of
-    channel_scale needs the forward call's x.  order norm_add: the residual's gradient is dout itself.  The vectors'
+    dresidual_out is the gradient with respect to residual_out (None: nothing came from it) and "dresidual" is returned if it is given, or as
+    residual_gradient says; the gradient of channel_scale needs the forward call's x.  order norm_add: the residual's gradient is dout itself.  The vectors'
     gradients are float32."""
     pd, sd, s = _norm_shape(dout, gate, norm, order, activation, eps, scale, "dout")
     add_norm = s.order == _ADD_NORM
@@ -782,7 +782,7 @@ def fused_norm_backward(dout, z, weight=None, bias=None, gate=None, scale=1.0, c
     got = {"dx": new()}
     if gate is not None:
         got["dgate"] = new()
-    if dresidual_out is not None:
+    if dresidual_out is not None if residual_gradient is None else residual_gradient:
         got["dresidual"] = new()
     for name, t in (("dweight", weight), ("dbias", bias), ("dscale", channel_scale)):
         if t is not None:
