@@ -100,3 +100,17 @@ int emu_fused_gemm_tiles(int w8, unsigned splits, int dtype, int act, size_t M, 
   return 0;
 }
 }
+
+// which kernels the library takes
+extern "C" {
+int emu_scan_threads(const tcu_gated_scan_shape *s, int back) {
+  tcu::GatedScanPlan plan;
+  return tcu::plan_gated_scan("plan", s, back ? tcu::kScanBackPlaces : tcu::kScanPlaces, &plan) == 0 ? plan.threads : 0;
+}
+// layout: 0 K along the rows of both operands, 1 down the rows of B, 2 down those of both; 0 for the form of few rows, else tiles of 32 times the result
+int emu_gemm_tile(size_t M, size_t N, size_t K, int layout, size_t *splits) {
+  const tcu::GemmPlan g = tcu::plan_gemm(M, N, K, layout);
+  *splits = g.splits;
+  return g.few_rows ? 0 : g.w8;
+}
+}
