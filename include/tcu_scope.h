@@ -271,6 +271,7 @@ int tcu_gemm_f16_f16(const void *d_A, const void *d_B, const void *d_C, void *d_
  * elements from row to row (so a slice of a wider matrix can be passed as it is); rows are tokens.  Whole 16-byte accesses
  * need base pointers aligned to 16 bytes and strides and widths that are multiples of 16 bytes; anything else takes the same
  * kernels with accesses that need no alignment.  All sums, states and statistics are fp32; a result is rounded once, to its type.
+ * Sizes that would take a launch of 2^32 threads or more are refused (TCU_ERR_UNSUPPORTED), though within the limits of the parts.
  * Calls run on the device of `stream` (NULL: the current device's default stream).  Workspaces follow the two-phase
  * protocol of the full-array entry points (256-byte aligned, nothing is kept in them from one call to the next; calls that
  * may overlap in time, captured graphs among them, need one each).  The smallest size is 256 bytes: it means that the call

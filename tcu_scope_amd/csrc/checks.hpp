@@ -10,6 +10,9 @@ inline size_t element_bytes(int dtype) { return dtype == TCU_F32 ? 4 : 2; }
 inline bool known_dtype(int dtype) { return dtype == TCU_F16 || dtype == TCU_BF16 || dtype == TCU_F32; }
 inline bool known_activation(int act) { return act >= TCU_ACT_NONE && act <= TCU_ACT_SIGMOID; }
 
+// HIP launches fewer than 2^32 threads at a time.
+inline bool launch_fits(size_t blocks, size_t threads) { return blocks <= 0xffffffffu / threads; }
+
 // A matrix of `rows` x `width` elements whose rows are `stride` elements apart; clears *whole_chunks if its rows do not all
 // begin on 16 bytes.
 inline int check_matrix(const std::string &w, const char *name, const void *p, size_t stride, size_t rows, size_t width, int dtype, bool *whole_chunks) {

@@ -125,10 +125,14 @@ inline int check_output(const std::string &w, const char *name, const void *p, s
   if (ld > kGemmMaxLd) return report_failure(TCU_ERR_UNSUPPORTED, w + ": the leading dimension of " + name + " is above 2^28");
   return check_matrix(w, name, p, ld, rows, width, dtype, whole);
 }
-// grids are counted in 32 bits: the smallest tiles any of the kernels may use
+// a launch with one thread for each chunk of 8 elements of a matrix
 inline int check_gemm_grid(const std::string &w, size_t M, size_t N) {
   size_t chunks = 0;
-  if (!product_fits(M, up_to(N, 8) / 8, &chunks) || chunks / 256 >= ((size_t)1 << 30)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": output too large");
+  if (!product_fits(M, up_to(N, 8) / 8, &chunks) || !launch_fits((chunks + 255) / 256, 256)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": a matrix of 2^35 elements or more");
+  return TCU_OK;
+}
+inline int check_gemm_tiles(const std::string &w, const GemmPlan &g) {
+  if (!launch_fits(g.tiles * g.splits, g.few_rows ? 512 : 256)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": the output takes more tiles than a launch can have");
   return TCU_OK;
 }
 
@@ -145,9 +149,14 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   if (int rc = check_gemm_grid(w, s->M, s->N)) return rc;
   const size_t M = s->M, N = s->N, K = s->K;
   const GemmPlan g = plan_gemm(M, N, K);
+  if (int rc = check_gemm_tiles(w, g)) return rc;
   const bool few_k = K > 0 && K < 64;  // the tile kernels want a whole step
   const bool odd_k = few_k || K % 8 != 0;     // nor a part of a chunk
   const bool pack_a = !g.few_rows && K && (odd_k || !rows_ready(A, M > 1 ? lda : 8)), pack_b = !g.few_rows && K && (odd_k || !rows_ready(B, N > 1 ? ldb : 8));
+  if (pack_a)
+    if (int rc = check_gemm_grid(w, M, K)) return rc;
+  if (pack_b)
+    if (int rc = check_gemm_grid(w, N, K)) return rc;
   const size_t ldk = few_k ? 64 : up_to(K, 8), a_bytes = pack_a ? part_bytes(M * ldk * 2) : 0, b_bytes = pack_b ? part_bytes(N * ldk * 2) : 0;
   const size_t bytes = g.share_bytes + a_bytes + b_bytes, need = smallest_workspace(bytes);
   if (!workspace_bytes) return report_failure(TCU_ERR_INVALID_ARG, w + ": workspace_bytes is null");
@@ -208,8 +217,12 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   if (int rc = check_gemm_shape(w, s)) return rc;
   const size_t M = s->M, N = s->N, K = s->K;
   if (M > kGemmMaxInner || N > kGemmMaxInner) return report_failure(TCU_ERR_UNSUPPORTED, w + ": M or N above 2^22");
-  for (auto mn : {std::make_pair(M, N), std::make_pair(M, K), std::make_pair(N, K)})  // a third of what a launch may have, in tiles of 64 x 64
+  size_t tiles = 0;  // of 64 x 64 elements, of all that may have to be laid out anew in one launch
+  for (auto mn : {std::make_pair(M, N), std::make_pair(M, K), std::make_pair(N, K)}) {
     if (int rc = check_gemm_grid(w, mn.first, mn.second)) return rc;
+    tiles += (mn.first + 63) / 64 * ((mn.second + 63) / 64);
+  }
+  if (!launch_fits(tiles, 256)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": the matrices take more tiles than a launch can have");
   const bool act = s->activation != TCU_ACT_NONE;
   if (act && !Z) return report_failure(TCU_ERR_INVALID_ARG, w + ": the gradient of an activation needs d_Z");
   // the copies' rows end in zeros up to a whole step of the tile kernels
@@ -220,6 +233,8 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   const bool down_a = dA && N >= 64 && K % 8 == 0 && rows_ready(B, ldb) && rows_ready(dA, M > 1 ? ldda : 8);
   const bool down_b = dB && M >= 64 && K % 8 == 0 && rows_ready(A, lda) && rows_ready(dB, N > 1 ? lddb : 8);
   const GemmPlan ga = plan_gemm(M, K, N, down_a ? kDownB : kAlong), gb = plan_gemm(N, K, M, down_b ? kDownBoth : kAlong);
+  if (int rc = dA ? check_gemm_tiles(w, ga) : TCU_OK) return rc;
+  if (int rc = dB ? check_gemm_tiles(w, gb) : TCU_OK) return rc;
   // the gradient of the activation's argument: dD itself where there is no activation and its rows are ready
   const bool own_dz = (dA || down_b) && (act || N % (dA && !down_a ? 64 : 8) != 0 || !rows_ready(dD, M > 1 ? lddd : 8));
   const bool turn_a = dB && !down_b, turn_b = dA && !down_a;  // A and dZ; B

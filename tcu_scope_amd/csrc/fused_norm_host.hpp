@@ -8,6 +8,7 @@
 
 namespace tcu {
 
+constexpr size_t kNormLaunchRows = (size_t)1 << 21;  // of one launch: up to 1024 threads a row, fewer than 2^32 in all
 constexpr size_t kNormMaxDim = 16384;    // beyond it a block cannot hold a row and its columns' sums in registers
 // Waves that share a row in the gradient's kernel, by the chunks per lane that one wave would need.
 inline int norm_back_waves(size_t chunks) { return chunks <= 1 ? 1 : chunks <= 2 ? 2 : chunks <= 4 ? 4 : 8; }
@@ -31,7 +32,7 @@ inline int check_norm_shape(const std::string &w, const tcu_fused_norm_shape *s)
 // 4096 bf16 with residual: 4 waves 89.8 us, 1 wave with 8 chunks per lane 92.7; and the shorter way through a row counts where
 // there are few).
 template <int DT, bool ALIGNED>
-inline void launch_fused_norm(const FusedNormParams &p, void *stream) {
+inline void launch_fused_norm_rows(const FusedNormParams &p, void *stream) {
   const size_t ct = (p.dim + 64 * Elem<DT>::V - 1) / (64 * Elem<DT>::V);  // chunks per lane if one wave takes the row
   const size_t rows = p.rows, quads = (rows + 3) / 4;
 #define TCU_NORM(W, C, BW, blocks) launch(fused_norm_kernel<DT, ALIGNED, W, C, BW>, (unsigned)(blocks), 64u * (BW), stream, p)
@@ -43,6 +44,21 @@ inline void launch_fused_norm(const FusedNormParams &p, void *stream) {
   else if (ct <= 32) TCU_NORM(8, 4, 8, rows);
   else TCU_NORM(16, 4, 16, rows);
 #undef TCU_NORM
+}
+template <int DT, bool ALIGNED>
+inline void launch_fused_norm(FusedNormParams p, void *stream) {
+  for (size_t left = p.rows; left > 0; left -= p.rows) {
+    p.rows = left < kNormLaunchRows ? left : kNormLaunchRows;
+    launch_fused_norm_rows<DT, ALIGNED>(p, stream);
+    auto ahead = [&](auto &q, size_t stride) {
+      if (q) q = (char *)q + p.rows * stride * sizeof(typename Elem<DT>::word_t);
+    };
+    ahead(p.x, p.x_stride);
+    ahead(p.residual, p.residual_stride);
+    ahead(p.gate, p.gate_stride);
+    ahead(p.out, p.out_stride);
+    ahead(p.z_out, p.z_out_stride);
+  }
 }
 
 inline int fused_norm_dispatch(const tcu_fused_norm_shape *s, const void *x, size_t x_stride, const void *residual, size_t residual_stride, const void *gate, size_t gate_stride, const void *weight,

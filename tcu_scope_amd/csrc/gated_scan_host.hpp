@@ -46,7 +46,7 @@ inline int plan_gated_scan(const char *what, const tcu_gated_scan_shape *s, int 
   auto chunks = [&](int threads) { return (plan->rows + threads / kScanLanes * places - 1) / (threads / kScanLanes * places); };
   if (plan->strips * chunks(256) < kScanManyTiles) plan->threads = 512;
   plan->chunks = chunks(plan->threads);
-  if (plan->strips * plan->chunks >= ((size_t)1 << 31)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": 2^31 tiles or more");
+  if (!launch_fits(plan->strips * plan->chunks, plan->threads)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": rows and channels take more tiles than a launch can have");
   plan->chained = plan->chunks > 1;
   plan->rows_at = 256;
   plan->entries_at = plan->rows_at + (s->d_offsets ? (plan->rows * 4 + 255) / 256 * 256 : 0);
@@ -237,7 +237,7 @@ inline int gated_scan_step_dispatch(int dtype, int gate, size_t channels, size_t
   const size_t per_block = (size_t)kStepThreads * (16 / element_bytes(dtype));
   p.chunks = (unsigned)((channels + per_block - 1) / per_block);
   size_t grid = 0;
-  if (!product_fits(rows, p.chunks, &grid) || grid >= ((size_t)1 << 31)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": 2^31 blocks or more");
+  if (!product_fits(rows, p.chunks, &grid) || !launch_fits(grid, kStepThreads)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": rows and channels take more blocks than a launch can have");
 #define TCU_STEP(DT_, G_) (aligned ? launch(gated_scan_step_kernel<DT_, G_, true>, (unsigned)grid, (unsigned)kStepThreads, stream, p) : launch(gated_scan_step_kernel<DT_, G_, false>, (unsigned)grid, (unsigned)kStepThreads, stream, p))
 #define TCU_STEP_GATES(DT_) (gate == TCU_GATE_DECAY ? TCU_STEP(DT_, kGateDecay) : gate == TCU_GATE_LOG ? TCU_STEP(DT_, kGateLog) : TCU_STEP(DT_, kGateSigmoid))
   if (dtype == TCU_F16) TCU_STEP_GATES(kF16);
