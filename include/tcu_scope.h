@@ -271,6 +271,8 @@ int tcu_gemm_f16_f16(const void *d_A, const void *d_B, const void *d_C, void *d_
  * elements from row to row (so a slice of a wider matrix can be passed as it is); rows are tokens.  Whole 16-byte accesses
  * need base pointers aligned to 16 bytes and strides and widths that are multiples of 16 bytes; anything else takes the same
  * kernels with accesses that need no alignment.  All sums, states and statistics are fp32; a result is rounded once, to its type.
+ * An output may stand in the place of an input (same address and stride) where that is said below, and shares no memory with
+ * any other operand; calls that break this are refused.  Slices of one matrix that lie side by side share none.
  * Sizes that would take a launch of 2^32 threads or more are refused (TCU_ERR_UNSUPPORTED), though within the limits of the parts.
  * Calls run on the device of `stream` (NULL: the current device's default stream).  Workspaces follow the two-phase
  * protocol of the full-array entry points (256-byte aligned, nothing is kept in them from one call to the next; calls that
@@ -310,7 +312,7 @@ typedef struct {
 } tcu_gated_scan_shape;
 
 /* d_h = the states after every row, d_h_last (num_sequences x channels fp32, may be NULL) = the state behind each sequence
- * (behind an empty one: its d_h0, or 0).  d_h0: num_sequences x channels fp32.  d_h may be d_x or d_g (same stride).
+ * (behind an empty one: its d_h0, or 0).  d_h0: num_sequences x channels fp32.  d_h may be d_x or d_g (same stride), d_h_last may be d_h0.
  * Products of a along up to 2048 rows are formed in fp32.  Where |a| is above 1 one may pass 2^128: a state of zero in front of it
  * still gives what the recurrence says, any other becomes an infinity or a NaN (also one so small that the recurrence would
  * stay finite).  Products below 2^-126 count as 0.
@@ -320,12 +322,12 @@ int tcu_gated_scan(const tcu_gated_scan_shape *shape, const void *d_x, size_t x_
 
 /* The gradient: from d_dh (with respect to d_h) and d_dh_last (with respect to d_h_last, may be NULL), d_dx, d_dg and, if
  * not NULL, d_dh0 (num_sequences x channels fp32).  d_h: the states the forward call returned; d_x is read for
- * TCU_GATE_SIGMOID only.  d_dx and d_dg may take the place of d_dh, d_x or d_g, not of d_h.  Bit-reproducible; waits as above. */
+ * TCU_GATE_SIGMOID only.  d_dx and d_dg may take the place of d_dh, d_x or d_g, not of d_h, d_dh0 that of d_h0 or d_dh_last.  Bit-reproducible; waits as above. */
 int tcu_gated_scan_backward(const tcu_gated_scan_shape *shape, const void *d_dh, size_t dh_stride, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, const void *d_h, size_t h_stride, const float *d_h0, const float *d_dh_last, void *d_dx, size_t dx_stride, void *d_dg, size_t dg_stride, float *d_dh0, void *d_workspace, size_t *workspace_bytes, void *stream);
 
 /* One token for each of num_rows running sequences: row i advances the state in slot d_slots[i] of d_state (num_slots x
  * channels fp32; d_slots NULL: slot i), writes it to the same slot of d_new_state (which may be d_state; slots that no row
- * names are not written) and, rounded, to row i of d_h.  Rows whose slot is negative or not below num_slots are padding:
+ * names are not written) and, rounded, to row i of d_h (which may be d_x or d_g).  Rows whose slot is negative or not below num_slots are padding:
  * not read, and in d_h left as they are (zero_padding 0) or set to zero.  Rows that name the same slot advance it one after the other, in row order. */
 int tcu_gated_scan_step(int dtype, int gate, size_t channels, size_t num_rows, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, void *d_h, size_t h_stride, const float *d_state, float *d_new_state, size_t num_slots, const int32_t *d_slots, int zero_padding, void *stream);
 

@@ -178,6 +178,9 @@ inline int fused_gemm_dispatch(const tcu_fused_gemm_shape *s, const void *A, siz
   if (int rc = Z ? check_output(w, "d_Z", Z, ldz, M, N, s->dtype, &whole) : TCU_OK) return rc;
   if (int rc = check_vector(w, "d_bias", bias, 2, &whole)) return rc;
   if (D == A || D == B || D == Z || (Z && (Z == A || Z == B || (use_c && Z == C)))) return report_failure(TCU_ERR_INVALID_ARG, w + ": an output in the place of an operand other tiles still read, or of another output");
+  const Place pa{"d_A", A, lda, M, K, 2}, pb{"d_B", B, ldb, N, K, 2}, pbias{"d_bias", bias, 0, 1, N, 2}, pc{"d_C", use_c ? C : nullptr, ldc, M, N, 2}, pd{"d_D", D, ldd, M, N, 2}, pz{"d_Z", Z, ldz, M, N, 2};
+  if (int rc = check_output_place(w, pd, {pc}, {pa, pb, pbias, pz})) return rc;
+  if (int rc = check_output_place(w, pz, {}, {pa, pb, pbias, pc})) return rc;
   char *at = static_cast<char *>(workspace) + g.share_bytes;
   FusedGemmParams p{};
   p.A = A;
@@ -264,6 +267,11 @@ inline int fused_gemm_backward_dispatch(const tcu_fused_gemm_shape *s, const voi
   if (int rc = check_vector(w, "d_dbias", dbias, 4, &ignored)) return rc;
   if ((dA && (dA == dD || dA == A || dA == B || dA == Z || dA == dB)) || (dB && (dB == dD || dB == A || dB == B || dB == Z)))
     return report_failure(TCU_ERR_INVALID_ARG, w + ": a gradient in the place of an operand, or of another gradient");
+  const Place pd{"d_dD", dD, lddd, M, N, 2}, pz{"d_Z", act ? Z : nullptr, ldz, M, N, 2}, pa{"d_A", dB ? A : nullptr, lda, M, K, 2}, pb{"d_B", dA ? B : nullptr, ldb, N, K, 2}, oa{"d_dA", dA, ldda, M, K, 2},
+      ob{"d_dB", dB, lddb, N, K, 2}, obias{"d_dbias", dbias, 0, 1, N, 4};
+  if (int rc = check_output_place(w, oa, {}, {pd, pz, pa, pb, ob, obias})) return rc;
+  if (int rc = check_output_place(w, ob, {}, {pd, pz, pa, pb, obias})) return rc;
+  if (int rc = check_output_place(w, obias, {}, {pd, pz, pa, pb})) return rc;
   char *at = static_cast<char *>(workspace) + share_bytes;
   auto take = [&](size_t n) {
     char *q = at;

@@ -81,6 +81,10 @@ inline int fused_norm_dispatch(const tcu_fused_norm_shape *s, const void *x, siz
   if (int rc = check_vector(w, "d_bias", bias, e, &aligned)) return rc;
   if (int rc = check_vector(w, "d_channel_scale", channel_scale, e, &aligned)) return rc;
   if (residual_out == out) return report_failure(TCU_ERR_INVALID_ARG, w + ": d_out and d_residual_out are the same buffer");
+  const Place px{"d_x", x, x_stride, s->rows, s->dim, e}, pr{"d_residual", residual, residual_stride, s->rows, s->dim, e}, pg{"d_gate", gate, gate_stride, s->rows, s->dim, e}, pw{"d_weight", weight, 0, 1, s->dim, e},
+      pb{"d_bias", bias, 0, 1, s->dim, e}, pc{"d_channel_scale", channel_scale, 0, 1, s->dim, e}, po{"d_out", out, out_stride, s->rows, s->dim, e}, pz{"d_residual_out", residual_out, residual_out_stride, s->rows, s->dim, e};
+  if (int rc = check_output_place(w, po, {px, pr, pg}, {pw, pb, pc, pz})) return rc;
+  if (int rc = check_output_place(w, pz, {px, pr, pg}, {pw, pb, pc})) return rc;
   const FusedNormParams p{x, residual, gate, weight, bias, channel_scale, out, residual_out, x_stride, residual_stride, gate_stride, out_stride, residual_out_stride, s->rows, (unsigned)s->dim, s->eps, s->scale, s->norm, s->order, s->activation};
 #define TCU_NORM_TYPE(DT) (aligned ? launch_fused_norm<DT, true>(p, stream) : launch_fused_norm<DT, false>(p, stream))
   if (s->dtype == TCU_F16) TCU_NORM_TYPE(kF16);
@@ -171,6 +175,17 @@ inline int fused_norm_backward_dispatch(const tcu_fused_norm_shape *s, const voi
   if (int rc = check_vector(w, "d_dweight", dweight, 4, &ignored)) return rc;
   if (int rc = check_vector(w, "d_dbias", dbias, 4, &ignored)) return rc;
   if (int rc = check_vector(w, "d_dchannel_scale", dchannel_scale, 4, &ignored)) return rc;
+  const size_t n = s->rows, d = s->dim;
+  const Place pd{"d_dout", dout, dout_stride, n, d, e}, pz{"d_z", z, z_stride, n, d, e}, pg{"d_gate", gate, gate_stride, n, d, e}, px{"d_x", dchannel_scale && add_norm ? x : nullptr, x_stride, n, d, e},
+      ps{"d_dresidual_out", dresidual_out, dresidual_out_stride, n, d, e}, pw{"d_weight", weight, 0, 1, d, e}, pb{"d_bias", bias, 0, 1, d, e}, pc{"d_channel_scale", channel_scale, 0, 1, d, e},
+      odx{"d_dx", dx, dx_stride, n, d, e}, odg{"d_dgate", dgate, dgate_stride, n, d, e}, odr{"d_dresidual", dresidual, dresidual_stride, n, d, e}, odw{"d_dweight", dweight, 0, 1, d, 4}, odb{"d_dbias", dbias, 0, 1, d, 4},
+      odc{"d_dchannel_scale", dchannel_scale, 0, 1, d, 4};
+  if (int rc = check_output_place(w, odx, {pd, pz, pg, px, ps}, {pw, pb, pc, odg, odr, odw, odb, odc})) return rc;
+  if (int rc = check_output_place(w, odg, {pd, pz, pg, px, ps}, {pw, pb, pc, odr, odw, odb, odc})) return rc;
+  if (int rc = check_output_place(w, odr, {pd, pz, pg, px, ps}, {pw, pb, pc, odw, odb, odc})) return rc;
+  if (int rc = check_output_place(w, odw, {}, {pd, pz, pg, px, ps, pw, pb, pc, odb, odc})) return rc;
+  if (int rc = check_output_place(w, odb, {}, {pd, pz, pg, px, ps, pw, pb, pc, odc})) return rc;
+  if (int rc = check_output_place(w, odc, {}, {pd, pz, pg, px, ps, pw, pb, pc})) return rc;
   if (s->rows) {
     FusedNormBackParams p{};
     p.dout = dout;

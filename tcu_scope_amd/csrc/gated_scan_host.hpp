@@ -137,6 +137,10 @@ inline int gated_scan_dispatch(const tcu_gated_scan_shape *s, const void *x, siz
   }
   if (int rc = check_vector(w, "d_h0", h0, 4, &aligned)) return rc;
   if (int rc = check_vector(w, "d_h_last", h_last, 4, &aligned)) return rc;
+  const size_t e = element_bytes(s->dtype), n = plan.rows, c = s->channels, states = s->num_sequences;
+  const Place px{"d_x", x, x_stride, n, c, e}, pg{"d_g", g, g_stride, n, c, e}, ph{"d_h", h, h_stride, n, c, e}, p0{"d_h0", h0, c, states, c, 4}, pl{"d_h_last", h_last, c, states, c, 4};
+  if (int rc = check_output_place(w, ph, {px, pg}, {p0, pl})) return rc;
+  if (int rc = check_output_place(w, pl, {p0}, {px, pg})) return rc;
   if (s->num_sequences == 0 && (plan.rows == 0 || !s->zero_outside)) return TCU_OK;
   GatedScanParams p{};
   p.x = x;
@@ -177,6 +181,12 @@ inline int gated_scan_backward_dispatch(const tcu_gated_scan_shape *s, const voi
   if (int rc = check_vector(w, "d_h0", h0, 4, &aligned)) return rc;
   if (int rc = check_vector(w, "d_dh_last", dh_last, 4, &aligned)) return rc;
   if (int rc = check_vector(w, "d_dh0", dh0, 4, &aligned)) return rc;
+  const size_t e = element_bytes(s->dtype), n = plan.rows, c = s->channels, states = s->num_sequences;
+  const Place pd{"d_dh", dh, dh_stride, n, c, e}, px{"d_x", s->gate == TCU_GATE_SIGMOID ? x : nullptr, x_stride, n, c, e}, pg{"d_g", g, g_stride, n, c, e}, ph{"d_h", h, h_stride, n, c, e},
+      p0{"d_h0", h0, c, states, c, 4}, pl{"d_dh_last", dh_last, c, states, c, 4}, odx{"d_dx", dx, dx_stride, n, c, e}, odg{"d_dg", dg, dg_stride, n, c, e}, od0{"d_dh0", dh0, c, states, c, 4};
+  if (int rc = check_output_place(w, odx, {pd, px, pg}, {ph, p0, pl, odg, od0})) return rc;
+  if (int rc = check_output_place(w, odg, {pd, px, pg}, {ph, p0, pl, od0})) return rc;
+  if (int rc = check_output_place(w, od0, {p0, pl}, {pd, px, pg, ph})) return rc;
   if (s->num_sequences == 0 && (plan.rows == 0 || !s->zero_outside)) return TCU_OK;
   GatedScanParams p{};
   p.dh = dh;
@@ -238,6 +248,11 @@ inline int gated_scan_step_dispatch(int dtype, int gate, size_t channels, size_t
   p.chunks = (unsigned)((channels + per_block - 1) / per_block);
   size_t grid = 0;
   if (!product_fits(rows, p.chunks, &grid) || !launch_fits(grid, kStepThreads)) return report_failure(TCU_ERR_UNSUPPORTED, w + ": rows and channels take more blocks than a launch can have");
+  const size_t e = element_bytes(dtype);
+  const Place px{"d_x", x, x_stride, rows, channels, e}, pg{"d_g", g, g_stride, rows, channels, e}, ph{"d_h", h, h_stride, rows, channels, e}, ps{"d_state", state, channels, num_slots, channels, 4},
+      pn{"d_new_state", new_state, channels, num_slots, channels, 4}, pi{"d_slots", slots, rows, 1, rows, 4};
+  if (int rc = check_output_place(w, ph, {px, pg}, {ps, pn, pi})) return rc;
+  if (int rc = check_output_place(w, pn, {ps}, {px, pg, pi})) return rc;
 #define TCU_STEP(DT_, G_) (aligned ? launch(gated_scan_step_kernel<DT_, G_, true>, (unsigned)grid, (unsigned)kStepThreads, stream, p) : launch(gated_scan_step_kernel<DT_, G_, false>, (unsigned)grid, (unsigned)kStepThreads, stream, p))
 #define TCU_STEP_GATES(DT_) (gate == TCU_GATE_DECAY ? TCU_STEP(DT_, kGateDecay) : gate == TCU_GATE_LOG ? TCU_STEP(DT_, kGateLog) : TCU_STEP(DT_, kGateSigmoid))
   if (dtype == TCU_F16) TCU_STEP_GATES(kF16);
