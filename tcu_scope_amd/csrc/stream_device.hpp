@@ -4,37 +4,45 @@
 
 #include <hip/hip_runtime.h>
 
-#include <exception>
-
 #include "host_support.hpp"
 #include "launch.hpp"
 
 namespace tcu {
 
+// makes `device` current again when it goes out of scope
+struct DeviceBack {
+  int device = -1;
+  ~DeviceBack() {
+    if (device >= 0) (void)hipSetDevice(device);
+  }
+};
+
 template <typename Body>
 inline int on_stream_device(const char *what, void *stream, Body &&body) {
   try {
+    DeviceBack back;
     const unsigned long before = launch_count();
-    int current = 0;
-    bool moved = false;
     if (stream) {
+      int current = 0;
       hipDevice_t of_stream = 0;
       hipError_t e = hipStreamGetDevice(static_cast<hipStream_t>(stream), &of_stream);
       if (e == hipSuccess) e = hipGetDevice(&current);
       if (e == hipSuccess && (int)of_stream != current) {
         e = hipSetDevice((int)of_stream);
-        moved = e == hipSuccess;
+        if (e == hipSuccess) back.device = current;
       }
       if (e != hipSuccess) {
         (void)hipGetLastError();
         return report_failure(TCU_ERR_RUNTIME, std::string(what) + ": device of the stream: " + hipGetErrorString(e));
       }
     }
-    const int rc = launch_outcome(what, before, body());
-    if (moved) (void)hipSetDevice(current);
-    return rc;
-  } catch (const std::exception &) {  // out of host memory; no message, which would need some
-    return TCU_ERR_RUNTIME;
+    return launch_outcome(what, before, body());
+  } catch (...) {  // out of host memory
+    try {
+      return report_failure(TCU_ERR_RUNTIME, std::string(what) + ": out of host memory");
+    } catch (...) {  // not even for the message
+      return TCU_ERR_RUNTIME;
+    }
   }
 }
 
