@@ -301,7 +301,7 @@ typedef struct {
   int dtype;              /* tcu_dtype of all matrices */
   int gate;               /* tcu_gate */
   size_t channels;        /* columns */
-  size_t num_rows;        /* rows of every matrix, below 2^31 - 4096 */
+  size_t num_rows;        /* rows of every matrix, up to 2^31 - 4096 */
   size_t num_sequences;
   size_t sequence_length; /* d_offsets NULL: num_rows = num_sequences * sequence_length */
   const void *d_offsets;  /* or num_sequences + 1 offsets in device memory that do not decrease: sequence j has the rows
@@ -328,7 +328,9 @@ int tcu_gated_scan_backward(const tcu_gated_scan_shape *shape, const void *d_dh,
 /* One token for each of num_rows running sequences: row i advances the state in slot d_slots[i] of d_state (num_slots x
  * channels fp32; d_slots NULL: slot i), writes it to the same slot of d_new_state (which may be d_state; slots that no row
  * names are not written) and, rounded, to row i of d_h (which may be d_x or d_g).  Rows whose slot is negative or not below num_slots are padding:
- * not read, and in d_h left as they are (zero_padding 0) or set to zero.  Rows that name the same slot advance it one after the other, in row order. */
+ * what they hold counts for nothing, and in d_h they are left as they are (zero_padding 0) or set to zero.  Rows that name the same
+ * slot advance it one after the other, in row order.  With d_slots the time grows with the square of the rows beyond some
+ * thousand: the form is meant for the requests of one decoding step. */
 int tcu_gated_scan_step(int dtype, int gate, size_t channels, size_t num_rows, const void *d_x, size_t x_stride, const void *d_g, size_t g_stride, void *d_h, size_t h_stride, const float *d_state, float *d_new_state, size_t num_slots, const int32_t *d_slots, int zero_padding, void *stream);
 
 /* Fused norm of every row, with s = scale * d_channel_scale (one number per channel, NULL: 1):
@@ -357,8 +359,8 @@ int tcu_fused_norm(const tcu_fused_norm_shape *shape, const void *d_x, size_t x_
  * d_dresidual_out (ADD_NORM, may be NULL): the gradient with respect to d_residual_out, added to that of z.  Written: d_dx,
  * and those of d_dgate, d_dresidual (ADD_NORM; with NORM_ADD the residual's gradient is d_dout itself), d_dweight, d_dbias
  * and d_dchannel_scale that are not NULL; the last three are fp32, summed over all rows (zero without rows).
- * d_dchannel_scale with ADD_NORM reads d_x.  A gradient may take the place of a matrix with the same stride.
- * Bit-reproducible. */
+ * d_dchannel_scale with ADD_NORM reads d_x.  d_dresidual may be asked for without d_dresidual_out.  A gradient may take the
+ * place of a matrix with the same stride.  The size query goes by which of the last three are not NULL.  Bit-reproducible. */
 int tcu_fused_norm_backward(const tcu_fused_norm_shape *shape, const void *d_dout, size_t dout_stride, const void *d_z, size_t z_stride, const void *d_gate, size_t gate_stride, const void *d_weight, const void *d_bias, const void *d_channel_scale, const void *d_x, size_t x_stride, const void *d_dresidual_out, size_t dresidual_out_stride, void *d_dx, size_t dx_stride, void *d_dgate, size_t dgate_stride, void *d_dresidual, size_t dresidual_stride, float *d_dweight, float *d_dbias, float *d_dchannel_scale, void *d_workspace, size_t *workspace_bytes, void *stream);
 
 /* Product with its epilogue: D = act(A B + bias) + beta C; A: M x K, B: K x N given as N rows of K (the operand layouts of

@@ -617,7 +617,7 @@ def _call_with_workspace(fn, args, sizes, workspace, device, raw):
     _check(fn(*args, ws.data_ptr(), ctypes.byref(have), raw))
 
 
-def _scan_shape(x, gate, offsets, h0, name="x"):
+def _scan_shape(x, gate, offsets, name="x"):
     torch = _torch()
     dtype = _dtype_code(x, name)
     s = GatedScanShape(dtype=dtype, gate=_enum(Gate, gate), channels=x.shape[-1])
@@ -646,7 +646,7 @@ def gated_scan(x, g, gate=Gate.SIGMOID, h0=None, offsets=None, out=None, h_last=
     name: "decay" (a = g, b = x), "log" (a = exp(g), b = x), "sigmoid" (a = sigmoid(g), b = (1 - a) x).  h0, h_last:
     (sequences, channels) float32, the states in front of and behind the sequences.  Rows outside all sequences
     are left as they are in `out`, and zero in a result this call allocates.  out may be x or g."""
-    s = _scan_shape(x, gate, offsets, h0)
+    s = _scan_shape(x, gate, offsets)
     states = (s.num_sequences, s.channels)
     px, _, sx = _matrix(x, "x")
     pg, _, sg = _matrix(g, "g", x)
@@ -667,7 +667,7 @@ def gated_scan_backward(dh, x, g, h, gate=Gate.SIGMOID, h0=None, dh_last=None, o
     dh, dh_last: gradients with respect to h and h_last (dh_last may be None); h: what gated_scan returned; x is read for
     the sigmoid gate only and may be None for the others.  dh0 is (sequences, channels) float32.  dx and dg may be given
     (both or neither), and be dh, x or g; rows outside all sequences are then left as they are, and otherwise zero."""
-    s = _scan_shape(g, gate, offsets, h0, "g")
+    s = _scan_shape(g, gate, offsets, "g")
     states = (s.num_sequences, s.channels)
     if x is None and s.gate == Gate.SIGMOID:
         raise ValueError("the sigmoid gate's gradient needs x")

@@ -51,7 +51,6 @@ TCU_DEVICE unsigned pack_bf16x2(float lo, float hi) {
   bf16x2_t v = {(__bf16)lo, (__bf16)hi};
   return __builtin_bit_cast(unsigned, v);
 }
-TCU_DEVICE uint16_t bf16_bits(float v) { return __builtin_bit_cast(uint16_t, (__bf16)v); }
 
 // D = A B + C on 16x16x32 MFMAs of either 16-bit type, operands as 16-byte chunks (layouts: wave_ops.hpp)
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));

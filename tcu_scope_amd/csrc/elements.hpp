@@ -15,7 +15,6 @@ struct Elem<kF16> {
   using word_t = uint16_t;
   static constexpr int V = 8;  // elements per 16-byte chunk
   TCU_DEVICE static float load(uint16_t w) { return (float)__builtin_bit_cast(half_t, w); }
-  TCU_DEVICE static uint16_t round(float v) { return f16_bits(v); }
   TCU_DEVICE static unsigned pack(float lo, float hi) { return pack_f16x2(lo, hi); }
 };
 template <>
@@ -23,7 +22,6 @@ struct Elem<kBF16> {
   using word_t = uint16_t;
   static constexpr int V = 8;
   TCU_DEVICE static float load(uint16_t w) { return __uint_as_float((unsigned)w << 16); }
-  TCU_DEVICE static uint16_t round(float v) { return bf16_bits(v); }
   TCU_DEVICE static unsigned pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
 };
 template <>
@@ -31,7 +29,6 @@ struct Elem<kF32> {
   using word_t = uint32_t;
   static constexpr int V = 4;
   TCU_DEVICE static float load(uint32_t w) { return __uint_as_float(w); }
-  TCU_DEVICE static uint32_t round(float v) { return __float_as_uint(v); }
 };
 
 // chunk -> V fp32 values
@@ -180,8 +177,10 @@ TCU_DEVICE void store_floats(float *p, size_t at, int count, const float (&v)[V]
   }
 }
 
-// e^x.  EXACT carries the rounding error of x * log2(e) along (a relative error of |x| 2^-24 otherwise, which results that
-// are rounded to 16 bits do not show and fp32 ones would).
+// e^x.  EXACT carries the rounding error of x * log2(e) along, a relative error of |x| 2^-24 otherwise.  It is taken where the matrices are
+// fp32.  With 16-bit ones, results of 16 bits do not show that error; their fp32 results (states behind a sequence, states of the
+// one-token form, gradients of vectors) do carry it: at most |x| / 2 times what the exponential itself may be off, on gates whose own
+// rounding to 16 bits moves e^x by up to |x| 2^-8 (bf16) or |x| 2^-11.  The correction would be 6 instructions more on some 26 an element in the scan.
 template <bool EXACT>
 TCU_DEVICE float exp_of(float x) {
   constexpr float kLog2E = 1.44269504088896340736f, kLog2ELow = 1.92596299112661746887e-8f, kLn2 = 0.69314718055994530942f;

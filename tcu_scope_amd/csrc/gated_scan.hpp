@@ -38,10 +38,10 @@
 // Tiles are handed out by a ticket, so the one that is waited for has always been started; a wait is bounded and leaves NaN
 // in what depended on it.
 //
-// 65536 x 2048 fp16 takes 173 us (805 MB, 4.6 TB/s; a copy reaches 5.1), 8 x 4096 x 2048 bf16 98 us (403 MB, 4.1 TB/s), its
-// gradient 164 us (805 MB, 4.9 TB/s), 8191 x 1000 packed bf16 19 us (49 MB; 256 tiles, a block for each compute unit,
-// bound by its own chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 23 us (63 MB; likewise, its rows
-// beginning anywhere).
+// Calls in a row, set-up launch included: 65536 x 2048 fp16 178 us (805 MB, 4.5 TB/s; a copy reaches 5.1), 8 x 4096 x 2048 bf16 97
+// (403 MB, 4.1 TB/s), its gradient 165 (805 MB, 4.9 TB/s), 8191 x 1000 packed bf16 24 (49 MB; this kernel 19: 256 tiles, a block for
+// each compute unit, bound by its own chain of load, combine, wait and store), 4099 x 769 packed fp32 backwards 27 (63 MB; this kernel 24:
+// likewise, its rows beginning anywhere).
 #pragma once
 
 #include "elements.hpp"
@@ -612,7 +612,9 @@ __global__ __launch_bounds__(256) inline void gated_scan_setup_kernel(GatedScanS
 }
 
 // One token for each of `rows` running sequences.  A block takes one row (and kStepThreads chunks of channels); rows that
-// name the same slot are advanced one after the other, in row order, by the block of the first of them.
+// name the same slot are advanced one after the other, in row order, by the block of the first of them.  Every block looks through all
+// slots for that, so the time grows with the square of the rows from some thousand on: 48 ... 512 rows of 2048 bf16 9 us a call (the
+// host's), 2048 rows 21, 8192 rows 189, 32768 rows 2570 (without slots 10, 39 and 159).
 struct GatedStepParams {
   const void *x, *g;
   void *out;
