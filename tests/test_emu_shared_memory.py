@@ -43,7 +43,7 @@ def test_gated_scan(emu, memory):
     assert back(h0=p + 2048, d0=p + 2048) == 0 and back(dl=p + 2048, d0=p + 2048) == 0
     assert back(h0=p + 2048, d0=p + 2064) == 1 and back(d0=p + 768) == 1
     step = lambda x=(p, 8), g=(p + 256, 8), h=(p + 512, 8), state=p + 1024, new=p + 1024, slots=p + 2048: emu.emu_gated_scan_step(0, 2, 8, 4, *x, *g, *h, state, new, 4, slots, 0)
-    assert step() == 0 and step(h=(p, 8)) == 0 and step(new=p + 3072) == 0
+    assert step() == 0 and step(h=(p, 8)) == 0 and step(new=p + 3328) == 0
     assert step(new=p + 1040) == 1 and step(h=(p + 1024, 8)) == 1 and step(h=(p + 2048, 8)) == 1 and step(h=(p, 9)) == 1 and step(new=p) == 1
 
 
